@@ -183,6 +183,36 @@ RENG_HIP_API int reng_hip_gemm_fp8_scaled(const uint8_t *a, int a_format, const 
                                           size_t N, size_t K, uint16_t *out, void *stream);
 
 /* ---------------------------------------------------------------------------
+ * Block scales: one scale per 128 x 128 block of a weight and per 1 x 128 group
+ * of an activation row (no counterpart in the reference, whose scales are per
+ * output row)
+ * ------------------------------------------------------------------------- */
+
+#define RENG_HIP_SCALE_BLOCK 128
+
+/* reng_hip_quantize's per-channel scheme with a block of block_rows x 128
+ * values in the place of a row: s = absmax / (max_finite * backoff), 1 for a zero
+ * block, code = encode(w / s). block_rows is 1 (activation rows) or 128
+ * (weights). w [rows, ld] as in reng_hip_quantize, aligned to its elements; codes
+ * [rows, cols]; scales f32 [ceil(rows / block_rows), ceil(cols / 128)], row-major;
+ * blocks at the right and lower edge are short. rows, cols, ld < 2^31. */
+RENG_HIP_API int reng_hip_quantize_blocks(const void *w, int dtype, size_t rows, size_t cols, size_t ld, int format,
+                                          size_t block_rows, float backoff, uint8_t *codes, float *scales,
+                                          void *stream);
+
+/* The product of block-scaled operands, on fp8 MFMA with f32 sums:
+ *   out[M, N] (bf16, RNE) = sum_kb scale_a[m, kb] scale_b[n / 128, kb] *
+ *                           sum_{k / 128 = kb} decode(a[m, k]) decode(b[n, k])
+ * a [M, K] codes with scale_a [M, ceil(K / 128)] (reng_hip_quantize_blocks with
+ * block_rows 1, or reng_hip_residual_norm_fp8), b [N, K] codes with scale_b
+ * [ceil(N / 128), ceil(K / 128)] (block_rows 128). Finite codes of either format
+ * each; K a multiple of 16, a and b 16-byte aligned. Any M; it allocates nothing
+ * and keeps nothing between calls. */
+RENG_HIP_API int reng_hip_gemm_fp8_blocks(const uint8_t *a, int a_format, const float *scale_a, const uint8_t *b,
+                                          int b_format, const float *scale_b, size_t M, size_t N, size_t K,
+                                          uint16_t *out, void *stream);
+
+/* ---------------------------------------------------------------------------
  * Decode step of one Llama decoder layer around its fp8 GEMVs
  *
  * The reference's fp8 load path stops at a refusal where the quantized codes
@@ -299,6 +329,57 @@ RENG_HIP_API int reng_hip_attention_decode_split(const uint16_t *q, const uint16
                                                  const uint16_t *v_cache, size_t n_heads, size_t n_kv_heads,
                                                  size_t head_dim, size_t len, float scale, void *workspace,
                                                  size_t workspace_bytes, uint16_t *out, void *stream);
+
+/* Most drafted tokens of one reng_hip_attention_tree call. */
+#define RENG_HIP_TREE_MAX_TOKENS 1024
+
+/* Bytes of device workspace reng_hip_attention_tree asks for, for every call
+ * with these heads, up to len context rows and up to tokens tokens. */
+RENG_HIP_API size_t reng_hip_attention_tree_workspace_bytes(size_t n_heads, size_t n_kv_heads, size_t head_dim,
+                                                            size_t len, size_t tokens);
+
+/* Attention of a tree of drafted tokens (no counterpart in the reference): the
+ * cache rows 0 .. len - 1 are context that every token sees, rows len .. len +
+ * tokens - 1 the drafted tokens' own. mask [tokens, ceil(tokens / 32)] words:
+ * token i sees drafted row j if bit j % 32 of word j / 32 of its row is set
+ * (bits from tokens on are not read); NULL is a chain (j <= i). q and out bf16
+ * [tokens, n_heads * head_dim]; otherwise as reng_hip_attention_decode, whose
+ * case it is at one token that sees itself. Rows a token does not see take no
+ * part, whatever they hold; a token that sees nothing gives zeros, one whose
+ * scores are all -inf, or with a NaN among them, gives NaN. len >= 0, 1 <=
+ * tokens <= RENG_HIP_TREE_MAX_TOKENS, len + tokens <= RENG_HIP_ATTENTION_MAX_LEN;
+ * pointers 4-byte aligned, workspace 16-byte aligned with workspace_bytes >=
+ * reng_hip_attention_tree_workspace_bytes(...). Fast for heads of 64, 96, 128 and
+ * 256 dimensions over 16-byte aligned q and caches. Asynchronous on stream; calls
+ * that share a workspace must be ordered (one stream). */
+RENG_HIP_API int reng_hip_attention_tree(const uint16_t *q, const uint16_t *k_cache, const uint16_t *v_cache,
+                                         size_t n_heads, size_t n_kv_heads, size_t head_dim, size_t len,
+                                         size_t tokens, const uint32_t *mask, float scale, void *workspace,
+                                         size_t workspace_bytes, uint16_t *out, void *stream);
+
+/* The steps between two branches of a layer in one pass (no counterpart in the
+ * reference's Llama form, whose residual add and norm are
+ * reng_hip_add_rms_norm_bf16's), per row in f32:
+ *   b = d;  b = rms_norm(b) * post_gamma (if given);  b = b * gate (if given)
+ *   h = x + residual_scale * b;  out = bf16(rms_norm(h) * gamma)
+ * x and h f32 [rows, cols] (h may be x, else must not overlap the inputs), d
+ * bf16 [rows, cols] the branch's output, post_gamma and gamma f32 [cols], gate
+ * bf16, one row for all tokens (gate_ld 0) or [rows, gate_ld], out bf16 [rows,
+ * cols]. d may be NULL (no branch: h = x; then post_gamma and gate are NULL and h
+ * may be NULL). rows < 4194304. */
+RENG_HIP_API int reng_hip_residual_norm_bf16(const float *x, const uint16_t *d, const float *post_gamma,
+                                             const uint16_t *gate, size_t gate_ld, float residual_scale,
+                                             const float *gamma, size_t rows, size_t cols, float eps, float *h,
+                                             uint16_t *out, void *stream);
+
+/* reng_hip_residual_norm_bf16 with the normalised row as fp8 codes [rows, cols]
+ * and a scale for each 128 columns, scales [rows, ceil(cols / 128)]: what
+ * reng_hip_quantize_blocks (block_rows 1) gives for the f32 row before any
+ * rounding to bf16; the a operand of reng_hip_gemm_fp8_blocks. */
+RENG_HIP_API int reng_hip_residual_norm_fp8(const float *x, const uint16_t *d, const float *post_gamma,
+                                            const uint16_t *gate, size_t gate_ld, float residual_scale,
+                                            const float *gamma, size_t rows, size_t cols, float eps, int format,
+                                            float backoff, float *h, uint8_t *codes, float *scales, void *stream);
 
 /* out = bf16(silu(gate) * up), silu(g) = g / (1 + exp(-g)) (layer_cpu's
  * Activation::Silu, model.rs:3070-3080). */
