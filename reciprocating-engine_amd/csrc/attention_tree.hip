@@ -11,7 +11,11 @@
 // f32 inside. A row that a token does not see takes no part, whatever it holds
 // (NaN and infinities included); a token that sees nothing (len = 0 and an empty
 // mask row) gives zeros; a NaN score among the rows seen makes its output NaN.
+#include <type_traits>
+
 #include "common.h"
+#include "mfma_pipe.h"
+#include "tree_plan.h"
 
 namespace reng {
 namespace {
@@ -113,6 +117,486 @@ __global__ __launch_bounds__(ANY_T) void attention_tree_any(TreeArgs a) {
     }
 }
 
+// ------------------------------------------------------------ tiled form
+//
+// The query rows of a key/value head (row r: token r / per, query head r % per of
+// the per that share it) go 32 to a wave. A workgroup's RW waves of a key group
+// share its tiles of TK cache rows; KW key groups take tiles in turn and merge in
+// LDS; splits of the cache merge in a second kernel (tree_plan.h).
+//
+// Per tile a wave forms S^T = K Q^T on v_mfma_f32_32x32x16_bf16 (keys from LDS
+// as the first operand, the queries in registers as the second), so a lane holds
+// 16 scores of one query per 32 keys: the softmax needs one exchange, with the
+// lane that holds the query's other 16, and the weights, rounded to bf16, are the
+// second operand of O^T = V^T P^T as they lie. V^T comes from LDS by transposing
+// reads. Only tiles that reach past the context look at the mask.
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+__device__ uint32_t tree_zeros[4];   // what a copy reads past the head size
+
+struct TreeTiles {
+    TreeArgs a;
+    uint32_t row_blocks, units, splits, tiles, base, more;   // split s: base tiles, one more for the first `more`
+    float *part;                                             // null: one pass
+};
+
+// Chunk (16 bytes) slots of a tile row. Keys: 32 rows are read at one chunk, so
+// chunk c of row r sits in slot c ^ r. Values: 4 rows are read over 64 bytes, so
+// the 64-byte quarter is permuted by the row.
+template <int P2>
+__device__ __forceinline__ uint32_t key_slot(uint32_t r, uint32_t c) {
+    if constexpr (P2 == 8) return c ^ ((r ^ (r >> 3)) & 7);
+    else return c ^ (r & 15);
+}
+template <int P2>
+__device__ __forceinline__ uint32_t value_slot(uint32_t r, uint32_t c) {
+    if constexpr (P2 == 8) return c ^ (((r >> 1) & 1) << 2);
+    else return c ^ ((r & 3) << 2);
+}
+
+__device__ __forceinline__ u32x2 read_tr(const uint8_t *p) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                         (__attribute__((address_space(3))) s16x4 *)p));
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x, y}, bf16x2));
+}
+
+// The value of the lane 32 further, combined.
+__device__ __forceinline__ float both_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float both_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Bit b: whether token i sees cache row j0 + b.
+__device__ __forceinline__ uint32_t seen_bits(const TreeArgs &a, uint32_t i, uint32_t j0) {
+    const int d0 = (int)j0 - (int)a.len;
+    int n = (a.mask ? (int)a.tokens : (int)i + 1) - d0;   // rows j0 .. j0 + n - 1 may be seen
+    uint32_t w = 0xffffffffu;
+    if (a.mask) {
+        const uint32_t *m = a.mask + (size_t)i * a.words;
+        if (d0 >= 0) {
+            const uint32_t k = (uint32_t)d0 / 32, sh = (uint32_t)d0 % 32;
+            const uint32_t lo = k < a.words ? m[k] : 0u, hi = k + 1 < a.words ? m[k + 1] : 0u;
+            w = (uint32_t)((((uint64_t)hi << 32) | lo) >> sh);
+        } else if (d0 > -32) {
+            w = (m[0] << -d0) | ((1u << -d0) - 1u);
+        }
+    }
+    if (n < 32) w &= n <= 0 ? 0u : (1u << n) - 1u;
+    return w;
+}
+
+__device__ bool sees_any(const TreeArgs &a, uint32_t i) {
+    if (a.len || !a.mask) return true;
+    for (uint32_t d = 0; d < a.tokens; ++d)
+        if ((a.mask[(size_t)i * a.words + d / 32] >> (d % 32)) & 1) return true;
+    return false;
+}
+
+// o / l as two bf16 pairs; l = 0: nothing seen gives zeros, scores that are all -inf give NaN.
+__device__ __forceinline__ u32x2 finish(const f32x4 &o, float l, bool any) {
+    if (!any) return u32x2{0u, 0u};
+    const float r = 1.0f / l;   // one rounding more than a division, far below bf16's
+    return u32x2{pack_bf16(o.x * r, o.y * r), pack_bf16(o.z * r, o.w * r)};
+}
+
+template <int HD, int RW, int KW, int TK, int S>
+struct TreeShape {
+    static constexpr int W = RW * KW, P2 = HD <= 64 ? 8 : HD <= 128 ? 16 : 32, ROWB = 16 * P2;
+    static constexpr int RPC = 64 / P2;                       // rows per 1 KB copy
+    static constexpr int TILE = TK * ROWB, STAGE = 2 * TILE;  // keys then values
+    static constexpr int CPW = TK / RPC / RW, LOADS = 2 * CPW;   // copies per wave, of keys; of both
+    static constexpr int LDS = KW * S * STAGE;
+    static constexpr int DB = HD / 32, KB = TK / 32;
+    static_assert(TK % (RPC * RW) == 0, "copies split evenly");
+    static_assert((KW - 1) * RW * (DB * 16 + 2) * 256 <= LDS, "the key groups merge in the ring");
+    static_assert(LDS <= 160 * 1024, "LDS");
+};
+
+template <int HD, int RW, int KW, int TK, int S>
+__global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t) {
+    using T = TreeShape<HD, RW, KW, TK, S>;
+    constexpr int P2 = T::P2, ROWB = T::ROWB, DB = T::DB, KB = T::KB;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    const TreeArgs &a = t.a;
+    // Workgroups go to the XCDs in turn: the row blocks of one split and key/value head
+    // follow each other on one XCD, whose L2 gives them the rows after the first.
+    const uint32_t b = blockIdx.x / TREE_XCDS, rb = b % t.row_blocks;
+    const uint32_t unit = b / t.row_blocks * TREE_XCDS + blockIdx.x % TREE_XCDS;
+    if (unit >= t.units) return;
+    const uint32_t g = unit % a.nkv, split = unit / a.nkv;
+    const uint32_t lane = threadIdx.x & 63, h = lane >> 5, ql = lane & 31;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = wave % RW, kg = wave / RW;
+    const uint32_t per = a.nh / a.nkv, R = a.tokens * per, rows = a.len + a.tokens;
+
+    // This lane's query row (clamped: rows past the last are not stored).
+    const uint32_t r0 = (rb * RW + rw) * 32 + ql, r = min(r0, R - 1), tok = r / per;
+    const size_t qrow = (size_t)tok * a.nh + g * per + r % per;
+    // scale < 0 goes into the queries' signs, so that the largest product is the largest score.
+    const float c = fabsf(a.scale) * 1.44269504088896341f;
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+    bf16x8 qf[HD / 16];
+#pragma unroll
+    for (int s = 0; s < HD / 16; ++s) {
+        const uint32_t d = 16 * s + 8 * h;
+        u32x4 v{0u, 0u, 0u, 0u};
+        if (d < a.hd) v = *reinterpret_cast<const u32x4 *>(a.q + qrow * a.hd + d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] ^= flip;
+        qf[s] = __builtin_bit_cast(bf16x8, v);
+    }
+
+    // The split's tiles, cut for a chain at the last row its tokens see.
+    const uint32_t t0 = split * t.base + min(split, t.more);
+    uint32_t t1 = t0 + t.base + (split < t.more);
+    if (!a.mask) {
+        const uint32_t last = min((rb * RW + RW) * 32 - 1, R - 1) / per;
+        t1 = min(t1, (a.len + last) / TK + 1);
+    }
+    const uint32_t n = t1 > t0 ? t1 - t0 : 0, steps = (n + KW - 1) / KW;
+
+    const size_t pitch = (size_t)a.nkv * a.hd;
+    const uint16_t *kbase = a.k + (size_t)g * a.hd, *vbase = a.v + (size_t)g * a.hd;
+    const uint32_t lr = lane / P2, ls = lane % P2, chunks = a.hd / 8;
+    uint8_t *ring = lds + kg * (S * T::STAGE);
+    auto has = [&](uint32_t step) { return step * KW + kg < n; };
+    auto issue = [&](uint32_t step) {
+        uint8_t *slot = ring + (step % S) * T::STAGE;
+        const uint32_t j0 = (t0 + step * KW + kg) * TK;
+#pragma unroll
+        for (int q = 0; q < T::CPW; ++q) {
+            const uint32_t tr = (rw * T::CPW + q) * T::RPC, row = tr + lr;
+            // Rows behind the last are clamped: no token sees them.
+            const size_t off = (size_t)min(j0 + row, rows - 1) * pitch;
+            const uint32_t kc = key_slot<P2>(row, ls), vc = value_slot<P2>(row, ls);
+            const uint16_t *kp = kc < chunks ? kbase + off + 8 * kc : reinterpret_cast<const uint16_t *>(tree_zeros);
+            const uint16_t *vp = vc < chunks ? vbase + off + 8 * vc : reinterpret_cast<const uint16_t *>(tree_zeros);
+            pipe::copy16_to_lds(reinterpret_cast<const uint8_t *>(kp), slot + tr * ROWB);
+            pipe::copy16_to_lds(reinterpret_cast<const uint8_t *>(vp), slot + T::TILE + tr * ROWB);
+        }
+    };
+
+    f32x16 o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+    float m = -INFINITY, l = 0.0f;   // the running maximum of the products, this lane's share of the sum
+
+    auto tile = [&](auto masked_c, const uint8_t *ks, uint32_t j0) {
+        constexpr bool MASKED = decltype(masked_c)::value;
+        const uint8_t *vs = ks + T::TILE;
+        f32x16 s[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
+#pragma unroll
+            for (int st = 0; st < HD / 16; ++st) {
+                const uint32_t row = 32 * kb + ql;
+                const bf16x8 kf =
+                    *reinterpret_cast<const bf16x8 *>(ks + row * ROWB + key_slot<P2>(row, 2 * st + h) * 16);
+                s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[st], s[kb], 0, 0, 0);
+            }
+        }
+        uint32_t see[KB];   // bit 8 (i / 4) + i % 4: whether score i counts
+        if constexpr (MASKED) {
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                see[kb] = seen_bits(a, tok, j0 + 32 * kb) >> (4 * h);
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (!((see[kb] >> (8 * (i / 4) + i % 4)) & 1)) s[kb][i] = -INFINITY;
+            }
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
+        mx = both_max(mx);
+        // The maximum moves, and what is summed so far is scaled down, only where a
+        // score passes it by more than 2^8: weights up to 256 lose nothing in f32 or bf16.
+        const bool move = (mx - m) * c > 8.0f || (m == -INFINITY && mx > m);
+        if (__builtin_amdgcn_ballot_w64(move)) {
+            const float f = !move ? 1.0f : m == -INFINITY ? 0.0f : exp2f((m - mx) * c);
+            if (move) m = mx;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= f;
+        }
+        // With nothing above -inf so far, exponents are taken against 0: they are 0.
+        const float mc = m == -INFINITY ? 0.0f : m * c;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float p = __builtin_amdgcn_exp2f(fmaf(s[kb][i], c, -mc));
+                if constexpr (MASKED) p = (see[kb] >> (8 * (i / 4) + i % 4)) & 1 ? p : 0.0f;
+                s[kb][i] = p;
+                l += p;
+            }
+        }
+        bool odd = false;   // a value of the tile is no finite number
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                u32x4 pw;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) pw[i] = pack_bf16(s[kb][8 * u + 2 * i], s[kb][8 * u + 2 * i + 1]);
+                const bf16x8 pf = __builtin_bit_cast(bf16x8, pw);
+                const uint32_t row = 32 * kb + 16 * u + 4 * h + (lane & 15) / 4;
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    // Lane: dimensions 4 (l % 4) .. + 3 of a row, from the 16 at 32 d + 16 (l / 16 % 2).
+                    const uint32_t dim = 32 * d + (lane & 16) + 4 * (lane & 3);
+                    const uint32_t in = 2 * (dim & 7), ch = dim / 8;
+                    const u32x2 v0 = read_tr(vs + row * ROWB + value_slot<P2>(row, ch) * 16 + in);
+                    const u32x2 v1 = read_tr(vs + (row + 8) * ROWB + value_slot<P2>(row + 8, ch) * 16 + in);
+                    u32x4 v{v0.x, v0.y, v1.x, v1.y};
+                    if constexpr (MASKED) {
+                        // A weight of 0 has to take nothing from a row that is not seen.
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t e = v[i] & 0x7f807f80u;
+                            const uint32_t lo = (e & 0xffffu) == 0x7f80u ? 0xffffu : 0u;
+                            const uint32_t hi = (e >> 16) == 0x7f80u ? 0xffff0000u : 0u;
+                            odd |= (lo | hi) != 0;
+                            v[i] &= ~(lo | hi);
+                        }
+                    }
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v), pf, o[d], 0, 0, 0);
+                }
+            }
+        if constexpr (MASKED) {
+            if (__builtin_amdgcn_ballot_w64(odd)) {
+                // Seldom: per dimension and query, count the NaN, +inf and -inf values among the
+                // rows seen with the same products, and add what they come to.
+#pragma unroll 1
+                for (int kind = 0; kind < 3; ++kind) {
+                    const float what = kind == 0 ? __builtin_nanf("") : kind == 1 ? INFINITY : -INFINITY;
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) {
+                        f32x16 cnt;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) cnt[i] = 0.0f;
+#pragma unroll
+                        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                            for (int u = 0; u < 2; ++u) {
+                                const uint32_t row = 32 * kb + 16 * u + 4 * h + (lane & 15) / 4;
+                                const uint32_t dim = 32 * d + (lane & 16) + 4 * (lane & 3);
+                                const uint32_t in = 2 * (dim & 7), ch = dim / 8;
+                                const u32x2 v0 = read_tr(vs + row * ROWB + value_slot<P2>(row, ch) * 16 + in);
+                                const u32x2 v1 = read_tr(vs + (row + 8) * ROWB + value_slot<P2>(row + 8, ch) * 16 + in);
+                                const u32x4 v{v0.x, v0.y, v1.x, v1.y};
+                                u32x4 isv, isp;
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    uint32_t z = 0, y = 0;
+#pragma unroll
+                                    for (int e = 0; e < 2; ++e) {
+                                        const uint32_t x = (v[i] >> (16 * e)) & 0xffffu;
+                                        const bool hit = kind == 0   ? (x & 0x7fffu) > 0x7f80u
+                                                         : kind == 1 ? x == 0x7f80u
+                                                                     : x == 0xff80u;
+                                        const int k = 8 * u + 2 * i + e;
+                                        z |= hit ? 0x3f80u << (16 * e) : 0u;
+                                        y |= (see[kb] >> (8 * (k / 4) + k % 4)) & 1 ? 0x3f80u << (16 * e) : 0u;
+                                    }
+                                    isv[i] = z;
+                                    isp[i] = y;
+                                }
+                                cnt = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, isv),
+                                                                              __builtin_bit_cast(bf16x8, isp), cnt, 0,
+                                                                              0, 0);
+                            }
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (cnt[i] > 0.0f) o[d][i] += what;
+                    }
+                }
+            }
+        }
+    };
+
+#pragma unroll
+    for (int s = 0; s + 1 < S; ++s)
+        if (has(s)) issue(s);
+    for (uint32_t step = 0; step < steps; ++step) {
+        // This wave's copies of the step's tile have landed (with three slots the next step's
+        // may be in flight), then every wave's have, and every wave is done with the slot before.
+        if (S > 2 && has(step + 1)) pipe::wait_vmcnt<(S - 2) * T::LOADS>();
+        else pipe::wait_vmcnt<0>();
+        pipe::lds_barrier();
+        if (has(step + S - 1)) issue(step + S - 1);
+        if (has(step)) {
+            const uint8_t *ks = ring + (step % S) * T::STAGE;
+            const uint32_t j0 = (t0 + step * KW + kg) * TK;
+            if (j0 + TK > a.len) tile(std::true_type{}, ks, j0);
+            else tile(std::false_type{}, ks, j0);
+        }
+    }
+    l = both_sum(l);
+    float mc = m == -INFINITY ? -INFINITY : m * c;
+
+    if constexpr (KW > 1) {
+        // The other key groups' (o, m, l) through LDS, lane by lane.
+        __syncthreads();
+        float *buf = reinterpret_cast<float *>(lds);
+        constexpr int PW = (DB * 16 + 2) * 64;   // floats of a wave
+        if (kg > 0) {
+            float *w = buf + ((kg - 1) * RW + rw) * PW;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<f32x4 *>(w + (d * 4 + i) * 256 + lane * 4) =
+                        f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+            w[DB * 1024 + lane] = mc;
+            w[DB * 1024 + 64 + lane] = l;
+        }
+        __syncthreads();
+        if (kg > 0) return;
+        float top = mc;
+#pragma unroll
+        for (int k = 0; k < KW - 1; ++k) top = fmaxf(top, buf[(k * RW + rw) * PW + DB * 1024 + lane]);
+        const float at = top == -INFINITY ? 0.0f : top;
+        float f = exp2f(mc - at);
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] *= f;
+#pragma unroll
+        for (int k = 0; k < KW - 1; ++k) {
+            const float *w = buf + (k * RW + rw) * PW;
+            f = exp2f(w[DB * 1024 + lane] - at);
+            l += w[DB * 1024 + 64 + lane] * f;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 v = *reinterpret_cast<const f32x4 *>(w + (d * 4 + i) * 256 + lane * 4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[d][4 * i + e] += v[e] * f;
+                }
+        }
+        mc = top;
+    }
+    if (r0 >= R) return;
+    // A lane has dimensions 32 d + 8 i + 4 h .. + 3 of its row.
+    if (t.part) {
+        const size_t all = (size_t)a.tokens * a.nh;
+        float *po = t.part + ((size_t)split * all + qrow) * a.hd;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t dim = 32 * d + 8 * i + 4 * h;
+                if (dim < a.hd)
+                    *reinterpret_cast<f32x4 *>(po + dim) =
+                        f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+            }
+        if (h == 0) {
+            float *ml = t.part + (size_t)t.splits * all * a.hd + ((size_t)split * all + qrow) * 2;
+            ml[0] = mc;
+            ml[1] = l;
+        }
+        return;
+    }
+    const bool any = l != 0.0f || sees_any(a, tok);
+    uint16_t *out = a.out + qrow * a.hd;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t dim = 32 * d + 8 * i + 4 * h;
+            if (dim < a.hd)
+                *reinterpret_cast<u32x2 *>(out + dim) =
+                    finish(f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]}, l, any);
+        }
+}
+
+// Merges the splits' (o, m, l): a thread four dimensions of a row.
+__global__ __launch_bounds__(256) void attention_tree_merge(TreeArgs a, const float *__restrict__ part,
+                                                            uint32_t splits) {
+    const uint32_t quads = a.hd / 4;
+    const size_t all = (size_t)a.tokens * a.nh, i = (size_t)blockIdx.x * 256 + threadIdx.x, row = i / quads;
+    if (row >= all) return;
+    const uint32_t d = (uint32_t)(i % quads) * 4;
+    const float *ml = part + (size_t)splits * all * a.hd + row * 2;
+    float top = -INFINITY;
+    for (uint32_t s = 0; s < splits; ++s) top = fmaxf(top, ml[(size_t)s * all * 2]);
+    const float at = top == -INFINITY ? 0.0f : top;
+    float l = 0.0f;
+    f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t s = 0; s < splits; ++s) {
+        const float f = exp2f(ml[(size_t)s * all * 2] - at);
+        l += ml[(size_t)s * all * 2 + 1] * f;
+        const f32x4 v = *reinterpret_cast<const f32x4 *>(part + ((size_t)s * all + row) * a.hd + d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += v[e] * f;
+    }
+    const bool any = l != 0.0f || sees_any(a, (uint32_t)(row / a.nh));
+    *reinterpret_cast<u32x2 *>(a.out + row * a.hd + d) = finish(o, l, any);
+}
+
+template <int HD, int RW, int KW, int TK, int S>
+int launch_tiles(const TreeArgs &a, const TreePlan &p, float *part, hipStream_t st) {
+    using T = TreeShape<HD, RW, KW, TK, S>;
+    const uint32_t units = p.splits * a.nkv;
+    const TreeTiles t{a,       p.row_blocks,        units,
+                      p.splits, p.tiles,             p.tiles / p.splits,
+                      p.tiles % p.splits, p.splits > 1 ? part : nullptr};
+    const unsigned grid = (units + TREE_XCDS - 1) / TREE_XCDS * TREE_XCDS * p.row_blocks;
+    auto kern = attention_tree_tiles<HD, RW, KW, TK, S>;
+    hipLaunchKernelGGL(kern, dim3(grid), dim3(64 * T::W), T::LDS, st, t);
+    if (int rc = check_launch("attention_tree_tiles")) return rc;
+    if (p.splits < 2) return RENG_HIP_OK;
+    const size_t threads = (size_t)a.tokens * a.nh * (a.hd / 4);
+    hipLaunchKernelGGL(attention_tree_merge, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a, part,
+                       p.splits);
+    return check_launch("attention_tree_merge");
+}
+
+template <int HD>
+int launch_form(const TreeArgs &a, const TreePlan &p, float *part, hipStream_t st) {
+    if constexpr (HD == 256) {
+        if (p.form == 0) return launch_tiles<256, 1, 2, 32, 2>(a, p, part, st);
+        if (p.form == 1) return launch_tiles<256, 2, 2, 32, 2>(a, p, part, st);
+        return launch_tiles<256, 4, 1, 32, 3>(a, p, part, st);
+    } else {
+        if (p.form == 0) return launch_tiles<HD, 1, 4, 32, 2>(a, p, part, st);
+        if (p.form == 1) return launch_tiles<HD, 2, 4, 32, 2>(a, p, part, st);
+        if (p.form == 2) return launch_tiles<HD, 4, 2, 32, 3>(a, p, part, st);
+        return launch_tiles<HD, 8, 1, 64, 3>(a, p, part, st);
+    }
+}
+
+int launch_tree(const TreeArgs &a, const TreePlan &p, float *part, hipStream_t st) {
+    if (p.hdp == 64) return launch_form<64>(a, p, part, st);
+    if (p.hdp == 96) return launch_form<96>(a, p, part, st);
+    if (p.hdp == 128) return launch_form<128>(a, p, part, st);
+    return launch_form<256>(a, p, part, st);
+}
+
 }  // namespace
 }  // namespace reng
 
@@ -120,8 +604,10 @@ using namespace reng;
 
 RENG_HIP_API size_t reng_hip_attention_tree_workspace_bytes(size_t n_heads, size_t n_kv_heads, size_t head_dim,
                                                             size_t len, size_t tokens) {
-    (void)n_heads, (void)n_kv_heads, (void)head_dim, (void)len, (void)tokens;
-    return 0;
+    if (n_heads == 0 || n_kv_heads == 0 || n_heads % n_kv_heads || n_heads > 4096 || head_dim > 1024) return 0;
+    if (tokens > RENG_HIP_TREE_MAX_TOKENS) tokens = RENG_HIP_TREE_MAX_TOKENS;
+    if (len > RENG_HIP_ATTENTION_MAX_LEN) len = RENG_HIP_ATTENTION_MAX_LEN;
+    return tree_workspace(n_heads, n_kv_heads, head_dim, len, tokens, (size_t)device_props().cus);
 }
 
 RENG_HIP_API int reng_hip_attention_tree(const uint16_t *q, const uint16_t *k_cache, const uint16_t *v_cache,
@@ -143,13 +629,18 @@ RENG_HIP_API int reng_hip_attention_tree(const uint16_t *q, const uint16_t *k_ca
                    reinterpret_cast<uintptr_t>(v_cache) | reinterpret_cast<uintptr_t>(out) |
                    reinterpret_cast<uintptr_t>(mask)) & 3) == 0,
                  "q, k_cache, v_cache, mask and out must be 4-byte aligned");
-    const size_t need = reng_hip_attention_tree_workspace_bytes(n_heads, n_kv_heads, head_dim, len, tokens);
+    const bool aligned = ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) |
+                           reinterpret_cast<uintptr_t>(v_cache)) & 15) == 0 &&
+                         (reinterpret_cast<uintptr_t>(out) & 7) == 0;
+    const TreePlan p = tree_plan(n_heads, n_kv_heads, head_dim, len, tokens, aligned, (size_t)device_props().cus);
+    const size_t need = tree_part_bytes(p, n_heads, head_dim, tokens);
     RENG_REQUIRE(workspace_bytes >= need, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
     RENG_REQUIRE(need == 0 || workspace, "null workspace");
     RENG_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "workspace must be 16-byte aligned");
     hipStream_t st = static_cast<hipStream_t>(stream);
     const TreeArgs a{q, k_cache, v_cache, (uint32_t)n_heads, (uint32_t)n_kv_heads, (uint32_t)head_dim, (uint32_t)len,
                      (uint32_t)tokens, mask, (uint32_t)((tokens + 31) / 32), scale, out};
+    if (p.fast) return launch_tree(a, p, static_cast<float *>(workspace), st);
     hipLaunchKernelGGL(attention_tree_any, dim3((unsigned)(tokens * n_heads)), dim3(ANY_T), 0, st, a);
     return check_launch("attention_tree_any");
 }
