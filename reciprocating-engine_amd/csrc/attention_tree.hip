@@ -221,6 +221,8 @@ struct TreeShape {
     static constexpr int CPW = TK / RPC / RW, LOADS = 2 * CPW;   // copies per wave, of keys; of both
     static constexpr int LDS = KW * S * STAGE;
     static constexpr int DB = HD / 32, KB = TK / 32;
+    static constexpr bool TURNS = S == 4;                     // the waves' halves take turns
+    static_assert(!TURNS || (KW == 1 && W == 8), "one wave of each half on a SIMD");
     static_assert(TK % (RPC * RW) == 0, "copies split evenly");
     static_assert((KW - 1) * RW * (DB * 16 + 2) * 256 <= LDS, "the key groups merge in the ring");
     static_assert(LDS <= 160 * 1024, "LDS");
@@ -296,10 +298,11 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
         for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
     float m = -INFINITY, l = 0.0f;   // the running maximum of the products, this lane's share of the sum
 
-    auto tile = [&](auto masked_c, const uint8_t *ks, uint32_t j0) {
-        constexpr bool MASKED = decltype(masked_c)::value;
-        const uint8_t *vs = ks + T::TILE;
-        f32x16 s[KB];
+    f32x16 s[KB];       // a tile's scores, before the scale
+    u32x4 pw[2 * KB];   // its weights in bf16: the 16 rows 16 u .. of each 32 as PV takes them
+    uint32_t see[KB];   // of a tile past the context, bit 8 (i / 4) + i % 4: whether score i counts
+
+    auto scores = [&](const uint8_t *ks) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
@@ -312,7 +315,9 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
                 s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[st], s[kb], 0, 0, 0);
             }
         }
-        uint32_t see[KB];   // bit 8 (i / 4) + i % 4: whether score i counts
+    };
+    auto weights = [&](auto masked_c, uint32_t j0) {
+        constexpr bool MASKED = decltype(masked_c)::value;
         if constexpr (MASKED) {
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
@@ -343,33 +348,40 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
         // With nothing above -inf so far, exponents are taken against 0: they are 0.
         const float mc = m == -INFINITY ? 0.0f : m * c;
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float p = __builtin_amdgcn_exp2f(fmaf(s[kb][i], c, -mc));
-                if constexpr (MASKED) p = (see[kb] >> (8 * (i / 4) + i % 4)) & 1 ? p : 0.0f;
-                s[kb][i] = p;
-                l += p;
+            for (int u = 0; u < 2; ++u) {
+                float p[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int k = 8 * u + i;
+                    p[i] = __builtin_amdgcn_exp2f(fmaf(s[kb][k], c, -mc));
+                    if constexpr (MASKED) p[i] = (see[kb] >> (8 * (k / 4) + k % 4)) & 1 ? p[i] : 0.0f;
+                    l += p[i];
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) pw[2 * kb + u][i] = pack_bf16(p[2 * i], p[2 * i + 1]);
             }
-        }
+    };
+    // V^T of the 16 rows from 32 kb + 16 u as the matrix cores take it. Lane: dimensions
+    // 4 (l % 4) .. + 3 of a row, from the 16 at 32 d + 16 (l / 16 % 2).
+    auto value_frag = [&](const uint8_t *vs, int kb, int u, int d) {
+        const uint32_t row = 32 * kb + 16 * u + 4 * h + (lane & 15) / 4;
+        const uint32_t dim = 32 * d + (lane & 16) + 4 * (lane & 3), in = 2 * (dim & 7), ch = dim / 8;
+        const u32x2 v0 = read_tr(vs + row * ROWB + value_slot<P2>(row, ch) * 16 + in);
+        const u32x2 v1 = read_tr(vs + (row + 8) * ROWB + value_slot<P2>(row + 8, ch) * 16 + in);
+        return u32x4{v0.x, v0.y, v1.x, v1.y};
+    };
+    auto products = [&](auto masked_c, const uint8_t *vs) {
+        constexpr bool MASKED = decltype(masked_c)::value;
         bool odd = false;   // a value of the tile is no finite number
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                u32x4 pw;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) pw[i] = pack_bf16(s[kb][8 * u + 2 * i], s[kb][8 * u + 2 * i + 1]);
-                const bf16x8 pf = __builtin_bit_cast(bf16x8, pw);
-                const uint32_t row = 32 * kb + 16 * u + 4 * h + (lane & 15) / 4;
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
-                    // Lane: dimensions 4 (l % 4) .. + 3 of a row, from the 16 at 32 d + 16 (l / 16 % 2).
-                    const uint32_t dim = 32 * d + (lane & 16) + 4 * (lane & 3);
-                    const uint32_t in = 2 * (dim & 7), ch = dim / 8;
-                    const u32x2 v0 = read_tr(vs + row * ROWB + value_slot<P2>(row, ch) * 16 + in);
-                    const u32x2 v1 = read_tr(vs + (row + 8) * ROWB + value_slot<P2>(row + 8, ch) * 16 + in);
-                    u32x4 v{v0.x, v0.y, v1.x, v1.y};
+                    u32x4 v = value_frag(vs, kb, u, d);
                     if constexpr (MASKED) {
                         // A weight of 0 has to take nothing from a row that is not seen.
 #pragma unroll
@@ -381,9 +393,9 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
                             v[i] &= ~(lo | hi);
                         }
                     }
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v), pf, o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                        __builtin_bit_cast(bf16x8, v), __builtin_bit_cast(bf16x8, pw[2 * kb + u]), o[d], 0, 0, 0);
                 }
-            }
         if constexpr (MASKED) {
             if (__builtin_amdgcn_ballot_w64(odd)) {
                 // Seldom: per dimension and query, count the NaN, +inf and -inf values among the
@@ -400,12 +412,7 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
                         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                             for (int u = 0; u < 2; ++u) {
-                                const uint32_t row = 32 * kb + 16 * u + 4 * h + (lane & 15) / 4;
-                                const uint32_t dim = 32 * d + (lane & 16) + 4 * (lane & 3);
-                                const uint32_t in = 2 * (dim & 7), ch = dim / 8;
-                                const u32x2 v0 = read_tr(vs + row * ROWB + value_slot<P2>(row, ch) * 16 + in);
-                                const u32x2 v1 = read_tr(vs + (row + 8) * ROWB + value_slot<P2>(row + 8, ch) * 16 + in);
-                                const u32x4 v{v0.x, v0.y, v1.x, v1.y};
+                                const u32x4 v = value_frag(vs, kb, u, d);
                                 u32x4 isv, isp;
 #pragma unroll
                                 for (int i = 0; i < 4; ++i) {
@@ -435,22 +442,85 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
             }
         }
     };
+    const std::true_type past{};
+    const std::false_type within{};
+    auto tile_row = [&](uint32_t step) { return (t0 + step * KW + kg) * TK; };
+    auto keys = [&](uint32_t step) { return ring + (step % S) * T::STAGE; };
+    auto soften = [&](uint32_t step) {
+        if (tile_row(step) + TK > a.len) weights(past, tile_row(step));
+        else weights(within, 0);
+    };
+    auto gather = [&](uint32_t step) {
+        const uint8_t *vs = keys(step) + T::TILE;
+        if (tile_row(step) + TK > a.len) products(past, vs);
+        else products(within, vs);
+    };
 
-#pragma unroll
-    for (int s = 0; s + 1 < S; ++s)
-        if (has(s)) issue(s);
-    for (uint32_t step = 0; step < steps; ++step) {
-        // This wave's copies of the step's tile have landed (with three slots the next step's
-        // may be in flight), then every wave's have, and every wave is done with the slot before.
-        if (S > 2 && has(step + 1)) pipe::wait_vmcnt<(S - 2) * T::LOADS>();
-        else pipe::wait_vmcnt<0>();
+    // Every LDS read of this wave is done before another may overwrite what it read.
+    auto barrier = [&] {
+        pipe::wait_lgkm0();
         pipe::lds_barrier();
-        if (has(step + S - 1)) issue(step + S - 1);
-        if (has(step)) {
-            const uint8_t *ks = ring + (step % S) * T::STAGE;
-            const uint32_t j0 = (t0 + step * KW + kg) * TK;
-            if (j0 + TK > a.len) tile(std::true_type{}, ks, j0);
-            else tile(std::false_type{}, ks, j0);
+    };
+    if constexpr (T::TURNS) {
+        // The waves' two halves, one of each on a SIMD, take turns: while one half runs its
+        // matrix products (a tile's values, the next tile's scores), the other half's weights
+        // use the vector unit. A phase ends at a barrier; the second half runs one phase
+        // behind. Tile i's scores are formed in phases 2 i and 2 i + 1, its values used by
+        // phase 2 i + 3, its copies issued in phase 2 i - 4 and waited for before the barrier
+        // that ends phase 2 i - 1: four slots.
+        const bool second = wave >= T::W / 2;
+        if (steps) {
+            issue(0);
+            if (has(1)) issue(1);
+            if (has(1)) pipe::wait_vmcnt<T::LOADS>();
+            else pipe::wait_vmcnt<0>();
+            barrier();
+            auto landed = [&](uint32_t step) {   // this wave's copies of that tile
+                if (has(step + 1)) pipe::wait_vmcnt<T::LOADS>();
+                else pipe::wait_vmcnt<0>();
+            };
+            if (!second) {
+                for (uint32_t i = 0; i < steps; ++i) {
+                    if (has(i + 2)) issue(i + 2);
+                    if (i) gather(i - 1);
+                    scores(keys(i));
+                    barrier();
+                    soften(i);
+                    landed(i + 1);
+                    barrier();
+                }
+                gather(steps - 1);
+            } else {
+                if (has(2)) issue(2);
+                barrier();
+                for (uint32_t i = 0; i < steps; ++i) {
+                    if (i) gather(i - 1);
+                    scores(keys(i));
+                    landed(i + 1);
+                    barrier();
+                    if (has(i + 3)) issue(i + 3);
+                    soften(i);
+                    if (i + 1 < steps) barrier();
+                }
+                gather(steps - 1);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i + 1 < S; ++i)
+            if (has(i)) issue(i);
+        for (uint32_t step = 0; step < steps; ++step) {
+            // This wave's copies of the step's tile have landed (with three slots the next step's
+            // may be in flight), then every wave's have, and every wave is done with the slot before.
+            if (S > 2 && has(step + 1)) pipe::wait_vmcnt<(S - 2) * T::LOADS>();
+            else pipe::wait_vmcnt<0>();
+            barrier();
+            if (has(step + S - 1)) issue(step + S - 1);
+            if (has(step)) {
+                scores(keys(step));
+                soften(step);
+                gather(step);
+            }
         }
     }
     l = both_sum(l);
@@ -586,7 +656,7 @@ int launch_form(const TreeArgs &a, const TreePlan &p, float *part, hipStream_t s
         if (p.form == 0) return launch_tiles<HD, 1, 4, 32, 2>(a, p, part, st);
         if (p.form == 1) return launch_tiles<HD, 2, 4, 32, 2>(a, p, part, st);
         if (p.form == 2) return launch_tiles<HD, 4, 2, 32, 3>(a, p, part, st);
-        return launch_tiles<HD, 8, 1, 64, 3>(a, p, part, st);
+        return launch_tiles<HD, 8, 1, 64, 4>(a, p, part, st);
     }
 }
 
