@@ -213,6 +213,20 @@ __device__ __forceinline__ u32x2 finish(const f32x4 &o, float l, bool any) {
     return u32x2{pack_bf16(o.x * r, o.y * r), pack_bf16(o.z * r, o.w * r)};
 }
 
+// NM matrix products that take R LDS reads each, four products' reads ahead of them.
+template <int NM, int R>
+__device__ __forceinline__ void read_ahead() {
+    constexpr int A = NM < 4 ? NM : 4;
+    __builtin_amdgcn_sched_group_barrier(0x100, A * R, 0);
+#pragma unroll
+    for (int i = 0; i < NM - A; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, A, 0);
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 template <int HD, int RW, int KW, int TK, int S>
 struct TreeShape {
     static constexpr int W = RW * KW, P2 = HD <= 64 ? 8 : HD <= 128 ? 16 : 32, ROWB = 16 * P2;
@@ -315,6 +329,7 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
                 s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[st], s[kb], 0, 0, 0);
             }
         }
+        read_ahead<KB * (HD / 16), 1>();
     };
     auto weights = [&](auto masked_c, uint32_t j0) {
         constexpr bool MASKED = decltype(masked_c)::value;
@@ -396,6 +411,7 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
                         __builtin_bit_cast(bf16x8, v), __builtin_bit_cast(bf16x8, pw[2 * kb + u]), o[d], 0, 0, 0);
                 }
+        if constexpr (!MASKED) read_ahead<2 * KB * DB, 2>();
         if constexpr (MASKED) {
             if (__builtin_amdgcn_ballot_w64(odd)) {
                 // Seldom: per dimension and query, count the NaN, +inf and -inf values among the
@@ -465,45 +481,33 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
         // The waves' two halves, one of each on a SIMD, take turns: while one half runs its
         // matrix products (a tile's values, the next tile's scores), the other half's weights
         // use the vector unit. A phase ends at a barrier; the second half runs one phase
-        // behind. Tile i's scores are formed in phases 2 i and 2 i + 1, its values used by
-        // phase 2 i + 3, its copies issued in phase 2 i - 4 and waited for before the barrier
-        // that ends phase 2 i - 1: four slots.
+        // behind. Tile i's scores are formed in phases 2 i and 2 i + 1, its values used in
+        // phases 2 i + 2 and 2 i + 3. A half issues its copies of tile i + 2 after it has read
+        // the values of tile i - 1 (the transposing reads wait for every copy in flight) and
+        // while the other half may still read those: four slots. Its copies of tile i + 1 have
+        // landed before the barrier that ends phase 2 i + 1.
         const bool second = wave >= T::W / 2;
         if (steps) {
-            issue(0);
-            if (has(1)) issue(1);
-            if (has(1)) pipe::wait_vmcnt<T::LOADS>();
-            else pipe::wait_vmcnt<0>();
-            barrier();
-            auto landed = [&](uint32_t step) {   // this wave's copies of that tile
+            auto landed = [&](uint32_t step) {
                 if (has(step + 1)) pipe::wait_vmcnt<T::LOADS>();
                 else pipe::wait_vmcnt<0>();
             };
-            if (!second) {
-                for (uint32_t i = 0; i < steps; ++i) {
-                    if (has(i + 2)) issue(i + 2);
-                    if (i) gather(i - 1);
-                    scores(keys(i));
-                    barrier();
-                    soften(i);
-                    landed(i + 1);
-                    barrier();
-                }
-                gather(steps - 1);
-            } else {
-                if (has(2)) issue(2);
+            issue(0);
+            if (has(1)) issue(1);
+            landed(0);
+            barrier();
+            if (second) barrier();
+            for (uint32_t i = 0; i < steps; ++i) {
+                if (i) gather(i - 1);
+                if (has(i + 2)) issue(i + 2);
+                scores(keys(i));
+                if (second) landed(i + 1);
                 barrier();
-                for (uint32_t i = 0; i < steps; ++i) {
-                    if (i) gather(i - 1);
-                    scores(keys(i));
-                    landed(i + 1);
-                    barrier();
-                    if (has(i + 3)) issue(i + 3);
-                    soften(i);
-                    if (i + 1 < steps) barrier();
-                }
-                gather(steps - 1);
+                soften(i);
+                if (!second) landed(i + 1);
+                if (!second || i + 1 < steps) barrier();
             }
+            gather(steps - 1);
         }
     } else {
 #pragma unroll
