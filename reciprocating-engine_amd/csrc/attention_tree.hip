@@ -139,8 +139,6 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-__device__ uint32_t tree_zeros[4];   // what a copy reads past the head size
-
 struct TreeTiles {
     TreeArgs a;
     uint32_t row_blocks, units, splits, tiles, base, more;   // split s: base tiles, one more for the first `more`
@@ -213,20 +211,6 @@ __device__ __forceinline__ u32x2 finish(const f32x4 &o, float l, bool any) {
     return u32x2{pack_bf16(o.x * r, o.y * r), pack_bf16(o.z * r, o.w * r)};
 }
 
-// NM matrix products that take R LDS reads each, four products' reads ahead of them.
-template <int NM, int R>
-__device__ __forceinline__ void read_ahead() {
-    constexpr int A = NM < 4 ? NM : 4;
-    __builtin_amdgcn_sched_group_barrier(0x100, A * R, 0);
-#pragma unroll
-    for (int i = 0; i < NM - A; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(0x008, A, 0);
-    __builtin_amdgcn_sched_barrier(0);
-}
-
 template <int HD, int RW, int KW, int TK, int S>
 struct TreeShape {
     static constexpr int W = RW * KW, P2 = HD <= 64 ? 8 : HD <= 128 ? 16 : 32, ROWB = 16 * P2;
@@ -235,6 +219,7 @@ struct TreeShape {
     static constexpr int CPW = TK / RPC / RW, LOADS = 2 * CPW;   // copies per wave, of keys; of both
     static constexpr int LDS = KW * S * STAGE;
     static constexpr int DB = HD / 32, KB = TK / 32;
+    static constexpr int AHEAD = 6;                           // products whose operands are read ahead
     static constexpr bool TURNS = S == 4;                     // the waves' halves take turns
     static_assert(!TURNS || (KW == 1 && W == 8), "one wave of each half on a SIMD");
     static_assert(TK % (RPC * RW) == 0, "copies split evenly");
@@ -245,7 +230,7 @@ struct TreeShape {
 template <int HD, int RW, int KW, int TK, int S>
 __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t) {
     using T = TreeShape<HD, RW, KW, TK, S>;
-    constexpr int P2 = T::P2, ROWB = T::ROWB, DB = T::DB, KB = T::KB;
+    constexpr int P2 = T::P2, ROWB = T::ROWB, DB = T::DB, KB = T::KB, AHEAD = T::AHEAD;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const TreeArgs &a = t.a;
     // Workgroups go to the XCDs in turn: the row blocks of one split and key/value head
@@ -284,26 +269,33 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
     }
     const uint32_t n = t1 > t0 ? t1 - t0 : 0, steps = (n + KW - 1) / KW;
 
-    const size_t pitch = (size_t)a.nkv * a.hd;
-    const uint16_t *kbase = a.k + (size_t)g * a.hd, *vbase = a.v + (size_t)g * a.hd;
-    const uint32_t lr = lane / P2, ls = lane % P2, chunks = a.hd / 8;
+    // A tile's copies go through a buffer resource of its rows of this head: rows behind the
+    // last cache row, and the chunks behind a head smaller than HD, lie outside and are not
+    // read. Nothing sees those rows; those chunks stay zero.
+    const uint32_t pitch = a.nkv * a.hd * 2, lr = lane / P2, ls = lane % P2, lrow = lr * pitch;
     uint8_t *ring = lds + kg * (S * T::STAGE);
     auto has = [&](uint32_t step) { return step * KW + kg < n; };
-    auto issue = [&](uint32_t step) {
+    auto issue = [&](uint32_t step) __attribute__((always_inline)) {
         uint8_t *slot = ring + (step % S) * T::STAGE;
-        const uint32_t j0 = (t0 + step * KW + kg) * TK;
+        const uint32_t j0 = (t0 + step * KW + kg) * TK, left = min((uint32_t)TK, rows - j0);
+        const size_t at = ((size_t)j0 * a.nkv + g) * a.hd;
+        const uint32_t bytes = (left - 1) * pitch + a.hd * 2;
+        const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void *)(a.k + at), 0, bytes, 0x00020000);
+        const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void *)(a.v + at), 0, bytes, 0x00020000);
 #pragma unroll
         for (int q = 0; q < T::CPW; ++q) {
             const uint32_t tr = (rw * T::CPW + q) * T::RPC, row = tr + lr;
-            // Rows behind the last are clamped: no token sees them.
-            const size_t off = (size_t)min(j0 + row, rows - 1) * pitch;
-            const uint32_t kc = key_slot<P2>(row, ls), vc = value_slot<P2>(row, ls);
-            const uint16_t *kp = kc < chunks ? kbase + off + 8 * kc : reinterpret_cast<const uint16_t *>(tree_zeros);
-            const uint16_t *vp = vc < chunks ? vbase + off + 8 * vc : reinterpret_cast<const uint16_t *>(tree_zeros);
-            pipe::copy16_to_lds(reinterpret_cast<const uint8_t *>(kp), slot + tr * ROWB);
-            pipe::copy16_to_lds(reinterpret_cast<const uint8_t *>(vp), slot + T::TILE + tr * ROWB);
+            const uint32_t kc = key_slot<P2>(row, ls), vc = value_slot<P2>(row, ls), off = lrow + tr * pitch;
+            const uint32_t none = 0x7fffffffu;   // past every resource
+            pipe::copy16_buf_asm(rk, slot + tr * ROWB, kc * 8 < a.hd ? off + 16 * kc : none);
+            pipe::copy16_buf_asm(rv, slot + T::TILE + tr * ROWB, vc * 8 < a.hd ? off + 16 * vc : none);
         }
     };
+    if (a.hd < HD) {
+        for (uint32_t i = threadIdx.x * 16; i < (uint32_t)T::LDS; i += 64 * T::W * 16)
+            *reinterpret_cast<u32x4 *>(lds + i) = u32x4{0u, 0u, 0u, 0u};
+        __syncthreads();
+    }
 
     f32x16 o[DB];
 #pragma unroll
@@ -316,22 +308,14 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
     u32x4 pw[2 * KB];   // its weights in bf16: the 16 rows 16 u .. of each 32 as PV takes them
     uint32_t see[KB];   // of a tile past the context, bit 8 (i / 4) + i % 4: whether score i counts
 
-    auto scores = [&](const uint8_t *ks) {
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[kb][i] = 0.0f;
-#pragma unroll
-            for (int st = 0; st < HD / 16; ++st) {
-                const uint32_t row = 32 * kb + ql;
-                const bf16x8 kf =
-                    *reinterpret_cast<const bf16x8 *>(ks + row * ROWB + key_slot<P2>(row, 2 * st + h) * 16);
-                s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[st], s[kb], 0, 0, 0);
-            }
-        }
-        read_ahead<KB * (HD / 16), 1>();
+    // 16 dimensions of 32 of a tile's keys as the matrix cores take them.
+    auto key_frag = [&](const uint8_t *ks, int kb, int st) __attribute__((always_inline)) {
+        const uint32_t row = 32 * kb + ql;
+        return *reinterpret_cast<const u32x4 *>(ks + row * ROWB + key_slot<P2>(row, 2 * st + h) * 16);
     };
-    auto weights = [&](auto masked_c, uint32_t j0) {
+    const f32x16 zero = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f,
+                         0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    auto weights = [&](auto masked_c, uint32_t j0) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(masked_c)::value;
         if constexpr (MASKED) {
 #pragma unroll
@@ -342,12 +326,18 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
                     if (!((see[kb] >> (8 * (i / 4) + i % 4)) & 1)) s[kb][i] = -INFINITY;
             }
         }
-        float mx = s[0][0];
+        // Four chains each for the maximum and the sum: one would wait for every step's result.
+        float mx4[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx4[i] = s[0][i];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
-        mx = both_max(mx);
+            for (int i = kb ? 0 : 4; i < 16; i += 8)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    mx4[e] = i + 4 < 16 ? fmaxf(fmaxf(mx4[e], s[kb][i + e]), s[kb][i + 4 + e]) : fmaxf(mx4[e], s[kb][i + e]);
+        const float mx = both_max(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])));
         // The maximum moves, and what is summed so far is scaled down, only where a
         // score passes it by more than 2^8: weights up to 256 lose nothing in f32 or bf16.
         const bool move = (mx - m) * c > 8.0f || (m == -INFINITY && mx > m);
@@ -362,6 +352,7 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
         }
         // With nothing above -inf so far, exponents are taken against 0: they are 0.
         const float mc = m == -INFINITY ? 0.0f : m * c;
+        float l4[4] = {l, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -372,23 +363,27 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
                     const int k = 8 * u + i;
                     p[i] = __builtin_amdgcn_exp2f(fmaf(s[kb][k], c, -mc));
                     if constexpr (MASKED) p[i] = (see[kb] >> (8 * (k / 4) + k % 4)) & 1 ? p[i] : 0.0f;
-                    l += p[i];
+                    l4[i % 4] += p[i];
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) pw[2 * kb + u][i] = pack_bf16(p[2 * i], p[2 * i + 1]);
             }
+        l = (l4[0] + l4[1]) + (l4[2] + l4[3]);
+        // Formed here, not where they are used: that may be behind a barrier.
+#pragma unroll
+        for (int i = 0; i < 2 * KB; ++i) asm volatile("" : "+v"(pw[i]));
     };
     // V^T of the 16 rows from 32 kb + 16 u as the matrix cores take it. Lane: dimensions
     // 4 (l % 4) .. + 3 of a row, from the 16 at 32 d + 16 (l / 16 % 2).
-    auto value_frag = [&](const uint8_t *vs, int kb, int u, int d) {
+    auto value_frag = [&](const uint8_t *vs, int kb, int u, int d) __attribute__((always_inline)) {
         const uint32_t row = 32 * kb + 16 * u + 4 * h + (lane & 15) / 4;
         const uint32_t dim = 32 * d + (lane & 16) + 4 * (lane & 3), in = 2 * (dim & 7), ch = dim / 8;
         const u32x2 v0 = read_tr(vs + row * ROWB + value_slot<P2>(row, ch) * 16 + in);
         const u32x2 v1 = read_tr(vs + (row + 8) * ROWB + value_slot<P2>(row + 8, ch) * 16 + in);
         return u32x4{v0.x, v0.y, v1.x, v1.y};
     };
-    auto products = [&](auto masked_c, const uint8_t *vs) {
-        constexpr bool MASKED = decltype(masked_c)::value;
+    auto masked_products = [&](const uint8_t *vs) __attribute__((always_inline)) {
+        constexpr bool MASKED = true;
         bool odd = false;   // a value of the tile is no finite number
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
@@ -411,7 +406,6 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
                         __builtin_bit_cast(bf16x8, v), __builtin_bit_cast(bf16x8, pw[2 * kb + u]), o[d], 0, 0, 0);
                 }
-        if constexpr (!MASKED) read_ahead<2 * KB * DB, 2>();
         if constexpr (MASKED) {
             if (__builtin_amdgcn_ballot_w64(odd)) {
                 // Seldom: per dimension and query, count the NaN, +inf and -inf values among the
@@ -458,73 +452,109 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
             }
         }
     };
-    const std::true_type past{};
-    const std::false_type within{};
     auto tile_row = [&](uint32_t step) { return (t0 + step * KW + kg) * TK; };
     auto keys = [&](uint32_t step) { return ring + (step % S) * T::STAGE; };
-    auto soften = [&](uint32_t step) {
-        if (tile_row(step) + TK > a.len) weights(past, tile_row(step));
-        else weights(within, 0);
+    // A run of matrix products in the order written, each one's operand read from LDS AHEAD
+    // products before it is used: the values of a tile (VALUES) and the scores of another.
+    auto run = [&](auto values_c, auto scores_c, const uint8_t *vs, const uint8_t *ks) __attribute__((always_inline)) {
+        constexpr int NV = decltype(values_c)::value ? 2 * KB * DB : 0, NK = decltype(scores_c)::value ? KB * HD / 16 : 0;
+        constexpr int N = NV + NK;
+        auto read = [&](int p) __attribute__((always_inline)) {
+            return p < NV ? value_frag(vs, p / DB / 2, p / DB % 2, p % DB) : key_frag(ks, (p - NV) % KB, (p - NV) / KB);
+        };
+        u32x4 f[AHEAD];
+#pragma unroll
+        for (int p = 0; p < AHEAD; ++p) f[p] = read(p);
+#pragma unroll
+        for (int p = 0; p < N; ++p) {
+            const bf16x8 x = __builtin_bit_cast(bf16x8, f[p % AHEAD]);
+            if (p < NV) {
+                o[p % DB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, __builtin_bit_cast(bf16x8, pw[p / DB]), o[p % DB],
+                                                                    0, 0, 0);
+            } else {
+                const int kb = (p - NV) % KB, st = (p - NV) / KB;
+                s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, qf[st], st ? s[kb] : zero, 0, 0, 0);
+            }
+            if (p + AHEAD < N) f[p % AHEAD] = read(p + AHEAD);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
-    auto gather = [&](uint32_t step) {
-        const uint8_t *vs = keys(step) + T::TILE;
-        if (tile_row(step) + TK > a.len) products(past, vs);
-        else products(within, vs);
-    };
+    const std::true_type yes{};
+    const std::false_type no{};
+    auto score = [&](uint32_t step) __attribute__((always_inline)) { run(no, yes, nullptr, keys(step)); };
 
     // Every LDS read of this wave is done before another may overwrite what it read.
     auto barrier = [&] {
         pipe::wait_lgkm0();
         pipe::lds_barrier();
     };
+    // The first `whole` steps' tiles lie within the context; the others look at the mask, in
+    // a loop of their own, whose registers the first does not pay for.
+    const uint32_t in = min(n, max(a.len / TK, t0) - t0), whole = in / KW;
+    // This wave's copies of a step's tile have landed (one step's may be in flight behind it).
+    auto landed = [&](uint32_t step) {
+        if (S > 2 && has(step + 1)) pipe::wait_vmcnt<T::LOADS>();
+        else pipe::wait_vmcnt<0>();
+    };
+    auto masked_tile = [&](uint32_t step) __attribute__((always_inline)) {
+        score(step);
+        weights(yes, tile_row(step));
+        masked_products(keys(step) + T::TILE);
+    };
     if constexpr (T::TURNS) {
         // The waves' two halves, one of each on a SIMD, take turns: while one half runs its
-        // matrix products (a tile's values, the next tile's scores), the other half's weights
-        // use the vector unit. A phase ends at a barrier; the second half runs one phase
-        // behind. Tile i's scores are formed in phases 2 i and 2 i + 1, its values used in
-        // phases 2 i + 2 and 2 i + 3. A half issues its copies of tile i + 2 after it has read
-        // the values of tile i - 1 (the transposing reads wait for every copy in flight) and
-        // while the other half may still read those: four slots. Its copies of tile i + 1 have
-        // landed before the barrier that ends phase 2 i + 1.
+        // matrix products (a tile's values, the next tile's scores), the other half's
+        // weights use the vector unit and its copies the memory pipe. A phase ends at a
+        // barrier; the second half runs one phase behind. Tile i's scores are formed in phases
+        // 2 i and 2 i + 1 and its values used in phases 2 i + 2 and 2 i + 3, so with four slots
+        // the first half may issue tile i + 2 in phase 2 i + 1, the second tile i + 3 in phase
+        // 2 i + 2. Tile i + 1 has landed before the barrier that ends phase 2 i + 1.
         const bool second = wave >= T::W / 2;
-        if (steps) {
-            auto landed = [&](uint32_t step) {
-                if (has(step + 1)) pipe::wait_vmcnt<T::LOADS>();
-                else pipe::wait_vmcnt<0>();
-            };
-            issue(0);
-            if (has(1)) issue(1);
-            landed(0);
+        const uint32_t far = second ? 3 : 2;
+#pragma unroll
+        for (uint32_t i = 0; i < 3; ++i)
+            if (i < far && has(i)) issue(i);
+        if (whole) {
+            pipe::wait_vmcnt<0>();
             barrier();
             if (second) barrier();
-            for (uint32_t i = 0; i < steps; ++i) {
-                if (i) gather(i - 1);
-                if (has(i + 2)) issue(i + 2);
-                scores(keys(i));
+            score(0);
+            for (uint32_t i = 0; i < whole; ++i) {
                 if (second) landed(i + 1);
                 barrier();
-                soften(i);
+                if (has(i + far)) issue(i + far);
+                weights(no, 0);
                 if (!second) landed(i + 1);
-                if (!second || i + 1 < steps) barrier();
+                barrier();
+                // Behind the last tile these scores are not used.
+                run(yes, yes, keys(i) + T::TILE, keys(i + 1));
             }
-            gather(steps - 1);
+            if (!second) barrier();
+        }
+        for (uint32_t i = whole; i < steps; ++i) {
+            landed(i);
+            barrier();
+            if (has(i + far)) issue(i + far);
+            masked_tile(i);
         }
     } else {
 #pragma unroll
         for (int i = 0; i + 1 < S; ++i)
             if (has(i)) issue(i);
-        for (uint32_t step = 0; step < steps; ++step) {
-            // This wave's copies of the step's tile have landed (with three slots the next step's
-            // may be in flight), then every wave's have, and every wave is done with the slot before.
-            if (S > 2 && has(step + 1)) pipe::wait_vmcnt<(S - 2) * T::LOADS>();
-            else pipe::wait_vmcnt<0>();
+        uint32_t step = 0;
+        for (; step < whole; ++step) {
+            landed(step);
+            barrier();   // every wave's copies have landed, and every wave is done with the slot before
+            if (has(step + S - 1)) issue(step + S - 1);
+            score(step);
+            weights(no, 0);
+            run(yes, no, keys(step) + T::TILE, nullptr);
+        }
+        for (; step < steps; ++step) {
+            landed(step);
             barrier();
             if (has(step + S - 1)) issue(step + S - 1);
-            if (has(step)) {
-                scores(keys(step));
-                soften(step);
-                gather(step);
-            }
+            if (has(step)) masked_tile(step);
         }
     }
     l = both_sum(l);

@@ -299,10 +299,6 @@ int launch_fp8_cfg(const Fp8Args &g, hipStream_t st) {
 // fragment reads or the stage barrier; the 256 x 256 tile halves the operand
 // bytes each output needs against 128 x 128.
 
-__device__ __forceinline__ void copy16_buf(__amdgpu_buffer_rsrc_t r, uint8_t *l, uint32_t voff, uint32_t soff) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)l, 16, voff, soff, 0, 0);
-}
-
 // WGM x WGN waves (default 2 x 4), each owning WM x WN MFMA tiles of 32 x 32.
 template <int WM, int WN, int BK_ = 128, int WGM_ = 2, int WGN_ = 4>
 struct WideTile {

@@ -52,6 +52,25 @@ __device__ __forceinline__ void copy16_to_lds(const uint8_t *g, uint8_t *l) {
     __builtin_amdgcn_global_load_lds(g, (__attribute__((address_space(3))) void *)l, 16, 0, 0);
 }
 
+// The same through a buffer resource: the lane's part of the address in voff, the
+// copy's in the scalar soff; bytes past the resource's size are not read.
+__device__ __forceinline__ void copy16_buf(__amdgpu_buffer_rsrc_t r, uint8_t *l, uint32_t voff, uint32_t soff) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)l, 16, voff, soff, 0, 0);
+}
+
+// copy16_buf as inline asm, which the compiler does not know to write LDS: it puts
+// a wait for every copy in flight before a transposing LDS read (ds_read_tr), and
+// none after these. The caller's own waits (wait_vmcnt, then a barrier) have to
+// order every read of the bytes. No output registers; m0 holds the LDS address,
+// one wait state before its use (a kernel that uses these has no other use of m0).
+__device__ __forceinline__ void copy16_buf_asm(__amdgpu_buffer_rsrc_t r, uint8_t *l, uint32_t voff) {
+    const uint32_t at = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void *)l);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(at), "v"(voff), "s"(r)
+                 : "memory");
+}
+
 // A workgroup barrier that orders LDS traffic for the compiler (the memory
 // clobbers) without the vmcnt(0) that __syncthreads' fence would add.
 __device__ __forceinline__ void lds_barrier() {
