@@ -220,8 +220,8 @@ struct TreeShape {
     static constexpr int LDS = KW * S * STAGE;
     static constexpr int DB = HD / 32, KB = TK / 32;
     static constexpr int AHEAD = 6;                           // products whose operands are read ahead
-    static constexpr bool TURNS = S == 4;                     // the waves' halves take turns
-    static_assert(!TURNS || (KW == 1 && W == 8), "one wave of each half on a SIMD");
+    static constexpr bool TURNS = RW == 8;                    // the waves' halves take turns
+    static_assert(!TURNS || (KW == 1 && S == 4), "one wave of each half on a SIMD, four slots");
     static_assert(TK % (RPC * RW) == 0, "copies split evenly");
     static_assert((KW - 1) * RW * (DB * 16 + 2) * 256 <= LDS, "the key groups merge in the ring");
     static_assert(LDS <= 160 * 1024, "LDS");
@@ -232,6 +232,7 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
     using T = TreeShape<HD, RW, KW, TK, S>;
     constexpr int P2 = T::P2, ROWB = T::ROWB, DB = T::DB, KB = T::KB, AHEAD = T::AHEAD;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    __shared__ uint32_t odd[2];   // step + 1 where a step's tiles hold a value that is no finite number
     const TreeArgs &a = t.a;
     // Workgroups go to the XCDs in turn: the row blocks of one split and key/value head
     // follow each other on one XCD, whose L2 gives them the rows after the first.
@@ -294,8 +295,10 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
     if (a.hd < HD) {
         for (uint32_t i = threadIdx.x * 16; i < (uint32_t)T::LDS; i += 64 * T::W * 16)
             *reinterpret_cast<u32x4 *>(lds + i) = u32x4{0u, 0u, 0u, 0u};
-        __syncthreads();
     }
+
+    if (threadIdx.x < 2) odd[threadIdx.x] = 0;
+    __syncthreads();
 
     f32x16 o[DB];
 #pragma unroll
@@ -382,73 +385,45 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
         const u32x2 v1 = read_tr(vs + (row + 8) * ROWB + value_slot<P2>(row + 8, ch) * 16 + in);
         return u32x4{v0.x, v0.y, v1.x, v1.y};
     };
-    auto masked_products = [&](const uint8_t *vs) __attribute__((always_inline)) {
-        constexpr bool MASKED = true;
-        bool odd = false;   // a value of the tile is no finite number
+    // What the values of a tile that are no finite numbers add: per dimension and query, the
+    // NaN, +inf and -inf among the rows seen are counted on the matrix cores.
+    auto specials = [&](const uint8_t *vs) __attribute__((always_inline)) {
+#pragma unroll 1
+        for (int kind = 0; kind < 3; ++kind) {
+            const float what = kind == 0 ? __builtin_nanf("") : kind == 1 ? INFINITY : -INFINITY;
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
+            for (int d = 0; d < DB; ++d) {
+                f32x16 cnt = zero;
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+                for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-                for (int d = 0; d < DB; ++d) {
-                    u32x4 v = value_frag(vs, kb, u, d);
-                    if constexpr (MASKED) {
-                        // A weight of 0 has to take nothing from a row that is not seen.
+                    for (int u = 0; u < 2; ++u) {
+                        const u32x4 v = value_frag(vs, kb, u, d);
+                        u32x4 isv, isp;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const uint32_t e = v[i] & 0x7f807f80u;
-                            const uint32_t lo = (e & 0xffffu) == 0x7f80u ? 0xffffu : 0u;
-                            const uint32_t hi = (e >> 16) == 0x7f80u ? 0xffff0000u : 0u;
-                            odd |= (lo | hi) != 0;
-                            v[i] &= ~(lo | hi);
-                        }
-                    }
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                        __builtin_bit_cast(bf16x8, v), __builtin_bit_cast(bf16x8, pw[2 * kb + u]), o[d], 0, 0, 0);
-                }
-        if constexpr (MASKED) {
-            if (__builtin_amdgcn_ballot_w64(odd)) {
-                // Seldom: per dimension and query, count the NaN, +inf and -inf values among the
-                // rows seen with the same products, and add what they come to.
-#pragma unroll 1
-                for (int kind = 0; kind < 3; ++kind) {
-                    const float what = kind == 0 ? __builtin_nanf("") : kind == 1 ? INFINITY : -INFINITY;
+                            uint32_t z = 0, y = 0;
 #pragma unroll
-                    for (int d = 0; d < DB; ++d) {
-                        f32x16 cnt;
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) cnt[i] = 0.0f;
-#pragma unroll
-                        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                            for (int u = 0; u < 2; ++u) {
-                                const u32x4 v = value_frag(vs, kb, u, d);
-                                u32x4 isv, isp;
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    uint32_t z = 0, y = 0;
-#pragma unroll
-                                    for (int e = 0; e < 2; ++e) {
-                                        const uint32_t x = (v[i] >> (16 * e)) & 0xffffu;
-                                        const bool hit = kind == 0   ? (x & 0x7fffu) > 0x7f80u
-                                                         : kind == 1 ? x == 0x7f80u
-                                                                     : x == 0xff80u;
-                                        const int k = 8 * u + 2 * i + e;
-                                        z |= hit ? 0x3f80u << (16 * e) : 0u;
-                                        y |= (see[kb] >> (8 * (k / 4) + k % 4)) & 1 ? 0x3f80u << (16 * e) : 0u;
-                                    }
-                                    isv[i] = z;
-                                    isp[i] = y;
-                                }
-                                cnt = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, isv),
-                                                                              __builtin_bit_cast(bf16x8, isp), cnt, 0,
-                                                                              0, 0);
+                            for (int e = 0; e < 2; ++e) {
+                                const uint32_t x = (v[i] >> (16 * e)) & 0xffffu;
+                                const bool hit = kind == 0   ? (x & 0x7fffu) > 0x7f80u
+                                                 : kind == 1 ? x == 0x7f80u
+                                                             : x == 0xff80u;
+                                const int k = 8 * u + 2 * i + e;
+                                z |= hit ? 0x3f80u << (16 * e) : 0u;
+                                y |= (see[kb] >> (8 * (k / 4) + k % 4)) & 1 ? 0x3f80u << (16 * e) : 0u;
                             }
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (cnt[i] > 0.0f) o[d][i] += what;
+                            isv[i] = z;
+                            isp[i] = y;
+                        }
+                        cnt = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, isv),
+                                                                      __builtin_bit_cast(bf16x8, isp), cnt, 0, 0, 0);
+                        __builtin_amdgcn_sched_barrier(0);
                     }
-                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (cnt[i] > 0.0f) o[d][i] += what;
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     };
@@ -491,15 +466,64 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
     // The first `whole` steps' tiles lie within the context; the others look at the mask, in
     // a loop of their own, whose registers the first does not pay for.
     const uint32_t in = min(n, max(a.len / TK, t0) - t0), whole = in / KW;
-    // This wave's copies of a step's tile have landed (one step's may be in flight behind it).
+    // This wave's copies of a step's tile have landed (those of up to BEHIND steps after it may
+    // be in flight).
+    constexpr int BEHIND = T::TURNS ? 1 : S - 2;
     auto landed = [&](uint32_t step) {
-        if (S > 2 && has(step + 1)) pipe::wait_vmcnt<T::LOADS>();
+        if (BEHIND > 1 && has(step + 2)) pipe::wait_vmcnt<BEHIND * T::LOADS>();
+        else if (BEHIND > 0 && has(step + 1)) pipe::wait_vmcnt<T::LOADS>();
         else pipe::wait_vmcnt<0>();
     };
-    auto masked_tile = [&](uint32_t step) __attribute__((always_inline)) {
-        score(step);
-        weights(yes, tile_row(step));
-        masked_products(keys(step) + T::TILE);
+    static_assert(BEHIND <= 2 && BEHIND * T::LOADS < 64, "vmcnt range");
+    // A weight of 0 must take nothing from a row that is not seen. So the waves look through the
+    // values of a tile that may hold such rows for anything that is no finite number, each at
+    // the part it copied, and where a step's tiles held some (seldom) it is added by itself and
+    // replaced by 0. `odd` is told apart by step: a wave may be one step ahead of another that
+    // has not read it yet.
+    auto each_copied = [&](uint32_t step, auto f) __attribute__((always_inline)) {
+#pragma unroll
+        for (int q = 0; q < T::CPW; ++q)
+            f(reinterpret_cast<u32x4 *>(ring + (step % S) * T::STAGE + T::TILE + (rw * T::CPW + q) * 1024 + lane * 16));
+    };
+    auto look = [&](uint32_t step) __attribute__((always_inline)) {
+        bool found = false;
+        each_copied(step, [&](const u32x4 *p) {
+            const u32x4 v = *p;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                found |= (v[i] & 0x7f80u) == 0x7f80u || (v[i] & 0x7f800000u) == 0x7f800000u;
+        });
+        if (__builtin_amdgcn_ballot_w64(found) && lane == 0) odd[step & 1] = step + 1;
+    };
+    auto clean = [&](uint32_t step) __attribute__((always_inline)) {
+        each_copied(step, [&](u32x4 *p) {
+            u32x4 v = *p;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if ((v[i] & 0x7f80u) == 0x7f80u) v[i] &= 0xffff0000u;
+                if ((v[i] & 0x7f800000u) == 0x7f800000u) v[i] &= 0xffffu;
+            }
+            *p = v;
+        });
+    };
+    auto masked_step = [&](uint32_t step, uint32_t next) __attribute__((always_inline)) {
+        const bool on = has(step);
+        const uint8_t *vs = keys(step) + T::TILE;
+        landed(step);
+        if (on) look(step);
+        barrier();   // every wave's copies have landed, and every wave is done with the slot before
+        if (has(next)) issue(next);
+        if (on) {
+            score(step);
+            weights(yes, tile_row(step));
+        }
+        if (odd[step & 1] == step + 1) {
+            if (on) specials(vs);
+            barrier();
+            if (on) clean(step);
+            barrier();
+        }
+        if (on) run(yes, no, vs, nullptr);
     };
     if constexpr (T::TURNS) {
         // The waves' two halves, one of each on a SIMD, take turns: while one half runs its
@@ -531,12 +555,7 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
             }
             if (!second) barrier();
         }
-        for (uint32_t i = whole; i < steps; ++i) {
-            landed(i);
-            barrier();
-            if (has(i + far)) issue(i + far);
-            masked_tile(i);
-        }
+        for (uint32_t i = whole; i < steps; ++i) masked_step(i, i + far);
     } else {
 #pragma unroll
         for (int i = 0; i + 1 < S; ++i)
@@ -550,12 +569,7 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
             weights(no, 0);
             run(yes, no, keys(step) + T::TILE, nullptr);
         }
-        for (; step < steps; ++step) {
-            landed(step);
-            barrier();
-            if (has(step + S - 1)) issue(step + S - 1);
-            if (has(step)) masked_tile(step);
-        }
+        for (; step < steps; ++step) masked_step(step, step + S - 1);
     }
     l = both_sum(l);
     float mc = m == -INFINITY ? -INFINITY : m * c;
@@ -564,7 +578,7 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
         // The other key groups' (o, m, l) through LDS, lane by lane.
         __syncthreads();
         float *buf = reinterpret_cast<float *>(lds);
-        constexpr int PW = (DB * 16 + 2) * 64;   // floats of a wave
+        constexpr int PW = tree_wave_floats(HD);
         if (kg > 0) {
             float *w = buf + ((kg - 1) * RW + rw) * PW;
 #pragma unroll
@@ -607,22 +621,15 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
     if (r0 >= R) return;
     // A lane has dimensions 32 d + 8 i + 4 h .. + 3 of its row.
     if (t.part) {
-        const size_t all = (size_t)a.tokens * a.nh;
-        float *po = t.part + ((size_t)split * all + qrow) * a.hd;
+        float *w = t.part + ((size_t)unit * (t.row_blocks * RW) + rb * RW + rw) * tree_wave_floats(HD);
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t dim = 32 * d + 8 * i + 4 * h;
-                if (dim < a.hd)
-                    *reinterpret_cast<f32x4 *>(po + dim) =
-                        f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-            }
-        if (h == 0) {
-            float *ml = t.part + (size_t)t.splits * all * a.hd + ((size_t)split * all + qrow) * 2;
-            ml[0] = mc;
-            ml[1] = l;
-        }
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<f32x4 *>(w + (d * 4 + i) * 256 + lane * 4) =
+                    f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+        w[DB * 1024 + lane] = mc;
+        w[DB * 1024 + 64 + lane] = l;
         return;
     }
     const bool any = l != 0.0f || sees_any(a, tok);
@@ -638,28 +645,65 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
         }
 }
 
-// Merges the splits' (o, m, l): a thread four dimensions of a row.
+// Merges the splits' (o, m, l), which lie as a wave of attention_tree_tiles held them: a wave
+// here takes one quad of dimensions of each of its lanes (32 rows, two quads each). With SW = 4
+// the four waves of a workgroup take a quarter of the splits each and meet in LDS: few rows over
+// many splits otherwise wait for one wave's chain of loads (one token after 4096 rows 20.5 ->
+// 15.3 us for the call).
+template <int HD, int SW>
 __global__ __launch_bounds__(256) void attention_tree_merge(TreeArgs a, const float *__restrict__ part,
-                                                            uint32_t splits) {
-    const uint32_t quads = a.hd / 4;
-    const size_t all = (size_t)a.tokens * a.nh, i = (size_t)blockIdx.x * 256 + threadIdx.x, row = i / quads;
-    if (row >= all) return;
-    const uint32_t d = (uint32_t)(i % quads) * 4;
-    const float *ml = part + (size_t)splits * all * a.hd + row * 2;
-    float top = -INFINITY;
-    for (uint32_t s = 0; s < splits; ++s) top = fmaxf(top, ml[(size_t)s * all * 2]);
-    const float at = top == -INFINITY ? 0.0f : top;
-    float l = 0.0f;
+                                                            uint32_t splits, uint32_t waves) {
+    constexpr uint32_t Q = HD / 8;   // quads a lane
+    __shared__ float lds[SW > 1 ? 4 * 6 * 64 : 1];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t w = SW > 1 ? blockIdx.x : blockIdx.x * 4 + wave, quad = w % Q, tile = w / Q;
+    const uint32_t per = a.nh / a.nkv, R = a.tokens * per, g = tile / waves, r = tile % waves * 32 + (lane & 31);
+    const uint32_t dim = 8 * quad + 4 * (lane >> 5);
+    const bool on = g < a.nkv && r < R && dim < a.hd;
+    const size_t step = (size_t)a.nkv * waves * tree_wave_floats(HD);   // from a split to the next
+    const float *p = part + (size_t)tile * tree_wave_floats(HD), *ml = p + HD * 32 + lane;
+    float top = -INFINITY, l = 0.0f;
     f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t s = 0; s < splits; ++s) {
-        const float f = exp2f(ml[(size_t)s * all * 2] - at);
-        l += ml[(size_t)s * all * 2 + 1] * f;
-        const f32x4 v = *reinterpret_cast<const f32x4 *>(part + ((size_t)s * all + row) * a.hd + d);
+    if (on) {
+        const uint32_t s0 = SW > 1 ? wave : 0;
+#pragma unroll 8
+        for (uint32_t s = s0; s < splits; s += SW) top = fmaxf(top, ml[s * step]);
+        const float at = top == -INFINITY ? 0.0f : top;
+#pragma unroll 8
+        for (uint32_t s = s0; s < splits; s += SW) {
+            const f32x4 v = *reinterpret_cast<const f32x4 *>(p + s * step + quad * 256 + lane * 4);
+            const float f = exp2f(ml[s * step] - at);
+            l += ml[s * step + 64] * f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] += v[e] * f;
+            for (int e = 0; e < 4; ++e) o[e] += v[e] * f;
+        }
     }
-    const bool any = l != 0.0f || sees_any(a, (uint32_t)(row / a.nh));
-    *reinterpret_cast<u32x2 *>(a.out + row * a.hd + d) = finish(o, l, any);
+    if constexpr (SW > 1) {
+        float *mine = lds + wave * 384 + lane;
+        mine[0] = top;
+        mine[64] = l;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mine[128 + 64 * e] = o[e];
+        __syncthreads();
+        if (wave > 0) return;
+        const float *all = lds + lane;
+        top = fmaxf(fmaxf(all[0], all[384]), fmaxf(all[768], all[1152]));
+        const float at = top == -INFINITY ? 0.0f : top;
+        l = 0.0f;
+        o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float f = exp2f(all[384 * k] - at);
+            l += all[384 * k + 64] * f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] += all[384 * k + 128 + 64 * e] * f;
+        }
+    }
+    if (!on) return;
+    const uint32_t tok = r / per;
+    const bool any = l != 0.0f || sees_any(a, tok);
+    uint16_t *out = a.out + ((size_t)tok * a.nh + g * per + r % per) * a.hd + dim;
+    *reinterpret_cast<u32x2 *>(out) = finish(o, l, any);
 }
 
 template <int HD, int RW, int KW, int TK, int S>
@@ -674,9 +718,13 @@ int launch_tiles(const TreeArgs &a, const TreePlan &p, float *part, hipStream_t 
     hipLaunchKernelGGL(kern, dim3(grid), dim3(64 * T::W), T::LDS, st, t);
     if (int rc = check_launch("attention_tree_tiles")) return rc;
     if (p.splits < 2) return RENG_HIP_OK;
-    const size_t threads = (size_t)a.tokens * a.nh * (a.hd / 4);
-    hipLaunchKernelGGL(attention_tree_merge, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a, part,
-                       p.splits);
+    const uint32_t waves = p.row_blocks * RW;
+    const uint32_t pieces = a.nkv * waves * (HD / 8);
+    if (p.splits >= 8 && pieces <= 4096)   // at most a few workgroups a CU
+        hipLaunchKernelGGL((attention_tree_merge<HD, 4>), dim3(pieces), dim3(256), 0, st, a, part, p.splits, waves);
+    else
+        hipLaunchKernelGGL((attention_tree_merge<HD, 1>), dim3((pieces + 3) / 4), dim3(256), 0, st, a, part, p.splits,
+                           waves);
     return check_launch("attention_tree_merge");
 }
 
@@ -687,7 +735,7 @@ int launch_form(const TreeArgs &a, const TreePlan &p, float *part, hipStream_t s
         if (p.form == 1) return launch_tiles<256, 2, 2, 32, 2>(a, p, part, st);
         return launch_tiles<256, 4, 1, 32, 3>(a, p, part, st);
     } else {
-        if (p.form == 0) return launch_tiles<HD, 1, 4, 32, 2>(a, p, part, st);
+        if (p.form == 0) return launch_tiles<HD, 1, 2, 32, 4>(a, p, part, st);
         if (p.form == 1) return launch_tiles<HD, 2, 4, 32, 2>(a, p, part, st);
         if (p.form == 2) return launch_tiles<HD, 4, 2, 32, 3>(a, p, part, st);
         return launch_tiles<HD, 8, 1, 64, 4>(a, p, part, st);
@@ -737,7 +785,7 @@ RENG_HIP_API int reng_hip_attention_tree(const uint16_t *q, const uint16_t *k_ca
                            reinterpret_cast<uintptr_t>(v_cache)) & 15) == 0 &&
                          (reinterpret_cast<uintptr_t>(out) & 7) == 0;
     const TreePlan p = tree_plan(n_heads, n_kv_heads, head_dim, len, tokens, aligned, (size_t)device_props().cus);
-    const size_t need = tree_part_bytes(p, n_heads, head_dim, tokens);
+    const size_t need = tree_part_bytes(p, n_kv_heads);
     RENG_REQUIRE(workspace_bytes >= need, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
     RENG_REQUIRE(need == 0 || workspace, "null workspace");
     RENG_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "workspace must be 16-byte aligned");

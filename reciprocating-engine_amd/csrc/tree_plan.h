@@ -24,7 +24,7 @@ struct TreePlan {
     uint32_t splits, tiles; // of the cache, and all its tiles
 };
 
-constexpr TreeForm TREE_FORMS[4] = {{1, 4, 32}, {2, 4, 32}, {4, 2, 32}, {8, 1, 64}};
+constexpr TreeForm TREE_FORMS[4] = {{1, 2, 32}, {2, 4, 32}, {4, 2, 32}, {8, 1, 64}};
 constexpr TreeForm TREE_FORMS_256[3] = {{1, 2, 32}, {2, 2, 32}, {4, 1, 32}};
 
 inline TreeForm tree_form(uint32_t hdp, int form) { return hdp == 256 ? TREE_FORMS_256[form] : TREE_FORMS[form]; }
@@ -39,6 +39,7 @@ inline TreePlan tree_plan(size_t nh, size_t nkv, size_t hd, size_t len, size_t t
     const size_t rows = tokens * (nh / nkv), cache = len + tokens;
     const int forms = p.hdp == 256 ? 3 : 4;
     while (p.form + 1 < forms && rows > 32 * tree_form(p.hdp, p.form).rw) ++p.form;
+    // FORM CHOSEN
     const TreeForm f = tree_form(p.hdp, p.form);
     p.row_blocks = (uint32_t)((rows + 32 * f.rw - 1) / (32 * f.rw));
     p.tiles = (uint32_t)((cache + f.tk - 1) / f.tk);
@@ -49,11 +50,21 @@ inline TreePlan tree_plan(size_t nh, size_t nkv, size_t hd, size_t len, size_t t
     if (s > most) s = most;
     if (s > TREE_SPLIT_MAX) s = TREE_SPLIT_MAX;
     p.splits = s < 1 ? 1 : (uint32_t)s;
+    // SPLITS CHOSEN
     return p;
 }
 
-inline size_t tree_part_bytes(const TreePlan &p, size_t nh, size_t hd, size_t tokens) {
-    return p.splits < 2 ? 0 : (size_t)p.splits * tokens * nh * (hd + 2) * sizeof(float);
+// What a wave leaves of a split: for 32 rows the unnormalised outputs, as its 64 lanes hold
+// them, and each lane's maximum and sum.
+#if defined(__HIPCC__)
+__host__ __device__
+#endif
+constexpr uint32_t tree_wave_floats(uint32_t hdp) { return hdp * 32 + 128; }
+
+inline size_t tree_part_bytes(const TreePlan &p, size_t nkv) {
+    return p.splits < 2 ? 0
+                        : (size_t)p.splits * nkv * p.row_blocks * tree_form(p.hdp, p.form).rw *
+                              tree_wave_floats(p.hdp) * sizeof(float);
 }
 
 // The most tree_part_bytes asks for over 1 .. tokens tokens and 0 .. len context
@@ -65,7 +76,7 @@ inline size_t tree_workspace(size_t nh, size_t nkv, size_t hd, size_t len, size_
     auto at = [&](size_t t) {
         if (t > tokens) t = tokens;
         const TreePlan p = tree_plan(nh, nkv, hd, len, t, true, cus);
-        const size_t b = tree_part_bytes(p, nh, hd, t);
+        const size_t b = tree_part_bytes(p, nkv);
         if (b > most) most = b;
         return p;
     };
