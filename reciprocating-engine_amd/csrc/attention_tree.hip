@@ -386,46 +386,48 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
         return u32x4{v0.x, v0.y, v1.x, v1.y};
     };
     // What the values of a tile that are no finite numbers add: per dimension and query, the
-    // NaN, +inf and -inf among the rows seen are counted on the matrix cores.
+    // NaN, +inf and -inf among the rows seen are counted on the matrix cores. The sums go
+    // through memory, so that this seldom path asks for no registers the others would miss.
     auto specials = [&](const uint8_t *vs) __attribute__((always_inline)) {
+        volatile float sums[DB * 16];
+#pragma unroll
+        for (int i = 0; i < DB * 16; ++i) sums[i] = o[i / 16][i % 16];
 #pragma unroll 1
-        for (int kind = 0; kind < 3; ++kind) {
+        for (int kd = 0; kd < 3 * DB; ++kd) {
+            const int kind = kd % 3, d = kd / 3;
             const float what = kind == 0 ? __builtin_nanf("") : kind == 1 ? INFINITY : -INFINITY;
+            f32x16 cnt = zero;
 #pragma unroll
-            for (int d = 0; d < DB; ++d) {
-                f32x16 cnt = zero;
+            for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-                for (int kb = 0; kb < KB; ++kb)
+                for (int u = 0; u < 2; ++u) {
+                    const u32x4 v = value_frag(vs, kb, u, d);
+                    u32x4 isv, isp;
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const u32x4 v = value_frag(vs, kb, u, d);
-                        u32x4 isv, isp;
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t z = 0, y = 0;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            uint32_t z = 0, y = 0;
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const uint32_t x = (v[i] >> (16 * e)) & 0xffffu;
-                                const bool hit = kind == 0   ? (x & 0x7fffu) > 0x7f80u
-                                                 : kind == 1 ? x == 0x7f80u
-                                                             : x == 0xff80u;
-                                const int k = 8 * u + 2 * i + e;
-                                z |= hit ? 0x3f80u << (16 * e) : 0u;
-                                y |= (see[kb] >> (8 * (k / 4) + k % 4)) & 1 ? 0x3f80u << (16 * e) : 0u;
-                            }
-                            isv[i] = z;
-                            isp[i] = y;
+                        for (int e = 0; e < 2; ++e) {
+                            const uint32_t x = (v[i] >> (16 * e)) & 0xffffu;
+                            const bool hit = kind == 0   ? (x & 0x7fffu) > 0x7f80u
+                                             : kind == 1 ? x == 0x7f80u
+                                                         : x == 0xff80u;
+                            const int k = 8 * u + 2 * i + e;
+                            z |= hit ? 0x3f80u << (16 * e) : 0u;
+                            y |= (see[kb] >> (8 * (k / 4) + k % 4)) & 1 ? 0x3f80u << (16 * e) : 0u;
                         }
-                        cnt = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, isv),
-                                                                      __builtin_bit_cast(bf16x8, isp), cnt, 0, 0, 0);
-                        __builtin_amdgcn_sched_barrier(0);
+                        isv[i] = z;
+                        isp[i] = y;
                     }
+                    cnt = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, isv),
+                                                                  __builtin_bit_cast(bf16x8, isp), cnt, 0, 0, 0);
+                }
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (cnt[i] > 0.0f) o[d][i] += what;
-                __builtin_amdgcn_sched_barrier(0);
-            }
+            for (int i = 0; i < 16; ++i)
+                if (cnt[i] > 0.0f) sums[16 * d + i] = sums[16 * d + i] + what;
         }
+#pragma unroll
+        for (int i = 0; i < DB * 16; ++i) o[i / 16][i % 16] = sums[i];
     };
     auto tile_row = [&](uint32_t step) { return (t0 + step * KW + kg) * TK; };
     auto keys = [&](uint32_t step) { return ring + (step % S) * T::STAGE; };
@@ -759,7 +761,7 @@ RENG_HIP_API size_t reng_hip_attention_tree_workspace_bytes(size_t n_heads, size
     if (n_heads == 0 || n_kv_heads == 0 || n_heads % n_kv_heads || n_heads > 4096 || head_dim > 1024) return 0;
     if (tokens > RENG_HIP_TREE_MAX_TOKENS) tokens = RENG_HIP_TREE_MAX_TOKENS;
     if (len > RENG_HIP_ATTENTION_MAX_LEN) len = RENG_HIP_ATTENTION_MAX_LEN;
-    return tree_workspace(n_heads, n_kv_heads, head_dim, len, tokens, (size_t)device_props().cus);
+    return tree_workspace(n_heads, n_kv_heads, head_dim, len, tokens);
 }
 
 RENG_HIP_API int reng_hip_attention_tree(const uint16_t *q, const uint16_t *k_cache, const uint16_t *v_cache,
@@ -785,7 +787,7 @@ RENG_HIP_API int reng_hip_attention_tree(const uint16_t *q, const uint16_t *k_ca
                            reinterpret_cast<uintptr_t>(v_cache)) & 15) == 0 &&
                          (reinterpret_cast<uintptr_t>(out) & 7) == 0;
     const TreePlan p = tree_plan(n_heads, n_kv_heads, head_dim, len, tokens, aligned, (size_t)device_props().cus);
-    const size_t need = tree_part_bytes(p, n_kv_heads);
+    const size_t need = p.fast ? tree_workspace(n_heads, n_kv_heads, head_dim, len, tokens) : 0;
     RENG_REQUIRE(workspace_bytes >= need, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
     RENG_REQUIRE(need == 0 || workspace, "null workspace");
     RENG_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "workspace must be 16-byte aligned");

@@ -29,31 +29,6 @@ constexpr TreeForm TREE_FORMS_256[3] = {{1, 2, 32}, {2, 2, 32}, {4, 1, 32}};
 
 inline TreeForm tree_form(uint32_t hdp, int form) { return hdp == 256 ? TREE_FORMS_256[form] : TREE_FORMS[form]; }
 
-// rows: query rows of a key/value head, tokens x heads that share it.
-inline TreePlan tree_plan(size_t nh, size_t nkv, size_t hd, size_t len, size_t tokens, bool aligned, size_t cus) {
-    TreePlan p{};
-    p.fast = hd % 8 == 0 && hd <= 256 && aligned;
-    p.splits = 1;
-    if (!p.fast) return p;
-    p.hdp = hd <= 64 ? 64 : hd <= 96 ? 96 : hd <= 128 ? 128 : 256;
-    const size_t rows = tokens * (nh / nkv), cache = len + tokens;
-    const int forms = p.hdp == 256 ? 3 : 4;
-    while (p.form + 1 < forms && rows > 32 * tree_form(p.hdp, p.form).rw) ++p.form;
-    // FORM CHOSEN
-    const TreeForm f = tree_form(p.hdp, p.form);
-    p.row_blocks = (uint32_t)((rows + 32 * f.rw - 1) / (32 * f.rw));
-    p.tiles = (uint32_t)((cache + f.tk - 1) / f.tk);
-    // Workgroups for every CU, but two steps of tiles a workgroup at least.
-    const size_t wgs = nkv * p.row_blocks;
-    size_t s = (cus + wgs - 1) / wgs;
-    const size_t most = p.tiles / (2 * f.kw);
-    if (s > most) s = most;
-    if (s > TREE_SPLIT_MAX) s = TREE_SPLIT_MAX;
-    p.splits = s < 1 ? 1 : (uint32_t)s;
-    // SPLITS CHOSEN
-    return p;
-}
-
 // What a wave leaves of a split: for 32 rows the unnormalised outputs, as its 64 lanes hold
 // them, and each lane's maximum and sum.
 #if defined(__HIPCC__)
@@ -61,33 +36,75 @@ __host__ __device__
 #endif
 constexpr uint32_t tree_wave_floats(uint32_t hdp) { return hdp * 32 + 128; }
 
+// At most 64 splits of 64 rows or more, and 4096 waves' partials (68 MB at 128 dimensions).
+constexpr size_t TREE_SPLIT_ROWS = 64, TREE_PART_WAVES = 4096;
+
+inline size_t tree_most_splits(size_t cache) {
+    const size_t s = cache / TREE_SPLIT_ROWS;
+    return s < 1 ? 1 : s > TREE_SPLIT_MAX ? TREE_SPLIT_MAX : s;
+}
+
+// A step's microseconds by form and head size, 64, 96, 128 and 256; the start of a round of
+// workgroups, the merge's launch, and its share of a megabyte of partials. Fitted to
+// graph-replayed timings of forms and splits on calls of 1 to 1024 tokens over 500 to 131000
+// rows (32 heads on 8 of 128 dimensions, 16 tokens after 500: 11.6 us by the model, 11.8
+// measured, where one split a workgroup a CU took 13.2; 28 on 4, 255 after 8191: 50 and 50, 72;
+// 40 on 8, 1024 after 16384: 293 and 360, 475).
+constexpr float TREE_STEP_US[4][4] = {
+    {0.70f, 0.90f, 1.05f, 1.30f}, {0.80f, 1.10f, 1.40f, 1.35f}, {0.70f, 0.95f, 1.10f, 1.50f}, {0.80f, 1.10f, 1.30f, 0.0f}};
+constexpr float TREE_ROUND_US = 4.0f, TREE_MERGE_US = 4.0f, TREE_MERGE_US_MB = 0.7f;
+
+// The cheapest form and number of splits. Rounds go by XCD: the row blocks of a split and
+// key/value head run on one, and those units go to the XCDs in turn. A form may leave less than
+// half of its row blocks' rows without a query.
+inline TreePlan tree_plan(size_t nh, size_t nkv, size_t hd, size_t len, size_t tokens, bool aligned, size_t cus) {
+    TreePlan p{};
+    p.fast = hd % 8 == 0 && hd <= 256 && aligned;
+    p.splits = 1;
+    if (!p.fast) return p;
+    p.hdp = hd <= 64 ? 64 : hd <= 96 ? 96 : hd <= 128 ? 128 : 256;
+    const int col = p.hdp == 64 ? 0 : p.hdp == 96 ? 1 : p.hdp == 128 ? 2 : 3;
+    const size_t cache = len + tokens, most = tree_most_splits(cache);
+    const size_t tiles32 = (tokens * (nh / nkv) + 31) / 32;   // 32-row tiles of a key/value head
+    const size_t xcd = cus < TREE_XCDS ? 1 : cus / TREE_XCDS;
+    float best = 0.0f;
+    for (int f = 0; f < (p.hdp == 256 ? 3 : 4); ++f) {
+        const TreeForm form = tree_form(p.hdp, f);
+        if (f > 0 && form.rw >= 2 * tiles32) break;
+        const size_t blocks = (tiles32 + form.rw - 1) / form.rw, tiles = (cache + form.tk - 1) / form.tk;
+        for (size_t s = 1; s <= most; ++s) {
+            const size_t waves = s * nkv * blocks * form.rw;
+            if (s > 1 && waves > TREE_PART_WAVES) break;
+            const size_t rounds = ((s * nkv + TREE_XCDS - 1) / TREE_XCDS * blocks + xcd - 1) / xcd;
+            const size_t steps = ((tiles + s - 1) / s + form.kw - 1) / form.kw;
+            float us = (float)rounds * (TREE_ROUND_US + TREE_STEP_US[f][col] * (float)steps);
+            if (s > 1) us += TREE_MERGE_US + TREE_MERGE_US_MB * 4e-6f * (float)(waves * tree_wave_floats(p.hdp));
+            if (best == 0.0f || us < best) {
+                best = us;
+                p.form = f;
+                p.row_blocks = (uint32_t)blocks;
+                p.tiles = (uint32_t)tiles;
+                p.splits = (uint32_t)s;
+            }
+        }
+    }
+    return p;
+}
+
 inline size_t tree_part_bytes(const TreePlan &p, size_t nkv) {
     return p.splits < 2 ? 0
                         : (size_t)p.splits * nkv * p.row_blocks * tree_form(p.hdp, p.form).rw *
                               tree_wave_floats(p.hdp) * sizeof(float);
 }
 
-// The most tree_part_bytes asks for over 1 .. tokens tokens and 0 .. len context
-// rows: with the form and the row blocks given the splits only grow with the rows,
-// so the most tokens of each (form, row blocks) are looked at.
-inline size_t tree_workspace(size_t nh, size_t nkv, size_t hd, size_t len, size_t tokens, size_t cus) {
-    size_t most = 0;
-    const size_t per = nh / nkv;
-    auto at = [&](size_t t) {
-        if (t > tokens) t = tokens;
-        const TreePlan p = tree_plan(nh, nkv, hd, len, t, true, cus);
-        const size_t b = tree_part_bytes(p, nkv);
-        if (b > most) most = b;
-        return p;
-    };
-    const TreePlan last = at(tokens);
-    if (!last.fast) return 0;
-    for (int f = 0; f < last.form; ++f)
-        if (const size_t t = 32 * tree_form(last.hdp, f).rw / per) at(t);
-    const size_t block = 32 * tree_form(last.hdp, last.form).rw;
-    for (uint32_t rb = 1; rb < last.row_blocks && nkv * rb < cus; ++rb)
-        if (const size_t t = rb * block / per) at(t);
-    return most;
+// No less than tree_part_bytes asks for over 1 .. tokens tokens and 0 .. len context rows.
+inline size_t tree_workspace(size_t nh, size_t nkv, size_t hd, size_t len, size_t tokens) {
+    const size_t most = tree_most_splits(len + tokens);
+    if (hd % 8 || hd > 256 || most < 2) return 0;
+    const size_t tiles32 = (tokens * (nh / nkv) + 31) / 32;
+    size_t waves = most * nkv * 2 * tiles32;
+    if (waves > TREE_PART_WAVES) waves = TREE_PART_WAVES;
+    return waves * tree_wave_floats(hd <= 64 ? 64 : hd <= 96 ? 96 : hd <= 128 ? 128 : 256) * sizeof(float);
 }
 
 }  // namespace reng
