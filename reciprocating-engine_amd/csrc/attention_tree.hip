@@ -271,8 +271,8 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
     const uint32_t n = t1 > t0 ? t1 - t0 : 0, steps = (n + KW - 1) / KW;
 
     // A tile's copies go through a buffer resource of its rows of this head: rows behind the
-    // last cache row, and the chunks behind a head smaller than HD, lie outside and are not
-    // read. Nothing sees those rows; those chunks stay zero.
+    // last cache row, and the chunks behind a head smaller than HD, lie outside it and arrive
+    // as zeros.
     const uint32_t pitch = a.nkv * a.hd * 2, lr = lane / P2, ls = lane % P2, lrow = lr * pitch;
     uint8_t *ring = lds + kg * (S * T::STAGE);
     auto has = [&](uint32_t step) { return step * KW + kg < n; };
@@ -292,11 +292,6 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
             pipe::copy16_buf_asm(rv, slot + T::TILE + tr * ROWB, vc * 8 < a.hd ? off + 16 * vc : none);
         }
     };
-    if (a.hd < HD) {
-        for (uint32_t i = threadIdx.x * 16; i < (uint32_t)T::LDS; i += 64 * T::W * 16)
-            *reinterpret_cast<u32x4 *>(lds + i) = u32x4{0u, 0u, 0u, 0u};
-    }
-
     if (threadIdx.x < 2) odd[threadIdx.x] = 0;
     __syncthreads();
 

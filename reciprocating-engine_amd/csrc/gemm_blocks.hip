@@ -6,7 +6,11 @@
 // The matrix cores sum a block's products; the block's sum times its scale is
 // added to an f32 accumulator, so the scales cost one multiply-add per output and
 // block beside 128 multiply-adds on the matrix cores.
+#include <type_traits>
+
 #include "common.h"
+#include "mfma_pipe.h"
+#include "tile_order.h"
 
 namespace reng {
 namespace {
@@ -16,6 +20,7 @@ constexpr uint32_t KBLK = 128;
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 struct BlockArgs {
     const uint8_t *a;
@@ -93,8 +98,221 @@ __global__ __launch_bounds__(64 * W) void gemm_blocks_rows(BlockArgs g, uint32_t
     }
 }
 
+// ------------------------------------------------------------ output tiles
+//
+// BM x BN outputs a workgroup, WGM x WGN waves of 16 TM x 16 TN, K in stages of one
+// scale block. A stage's operand rows and its BM + BN / 128 scales are copied to an
+// S-slot LDS ring (16-byte chunks of a row permuted by swz, so that fragment reads
+// are free of bank conflicts). A wave keeps its TN weight fragments of a stage in
+// registers and goes through the TM activation fragments; the 16 x 16 product of a
+// stage (one v_mfma_f32_16x16x128) is scaled and added to the accumulator PART
+// products later, so that the vector unit works while the matrix cores do. The next
+// stage's first fragments are read behind the barrier before this stage's last two
+// rows of products. Rows past M and N and codes past K lie outside the tile's buffer
+// resources and arrive as zeros.
+template <int TM_, int TN_, int WGM_, int WGN_, int S_>
+struct BlockTile {
+    static constexpr int TM = TM_, TN = TN_, WGM = WGM_, WGN = WGN_, S = S_, NW = WGM * WGN;
+    static constexpr int BM = 16 * TM * WGM, BN = 16 * TN * WGN;
+    static constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128, SC = 4 * (BM + 64);   // the weight's scales in the last 64
+    static constexpr int STAGE = A_BYTES + B_BYTES, RING = S * (STAGE + SC);
+    static constexpr int LA = BM / 8 / NW, LB = BN / 8 / NW, LS = (BM / 64 + 1 + NW - 1) / NW, LOADS = LA + LB + LS;
+    static constexpr int OUT = BM * (BN * 2 + 16);   // the epilogue's rows, padded by a chunk
+    static constexpr int LDS = RING > OUT ? RING : OUT;
+    static constexpr int PART = 3;
+    static_assert(LA * 8 * NW == BM && LB * 8 * NW == BN, "copies split evenly");
+    static_assert((TM == 2 || TM % 4 == 0) && 16 * TN <= 128 && 128 % (16 * TN) == 0, "a wave's columns share a scale");
+    static_assert((S - 2) * LOADS < 64 && S >= 2 && LDS <= 160 * 1024, "vmcnt range, LDS");
+};
+
+template <int FA, int FB, typename T>
+__global__ __launch_bounds__(64 * T::NW) void gemm_blocks_tiles(BlockArgs g, uint32_t tiles_m, uint32_t tiles,
+                                                                uint32_t mapm) {
+    constexpr int TM = T::TM, TN = T::TN, S = T::S, PART = T::PART;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, row = lane & 15, q = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / T::WGN, wn = wave % T::WGN;
+    uint32_t mt, nt;
+    wide_tile_of(blockIdx.x, tiles_m, tiles, mapm, mt, nt);
+    const uint32_t m0 = mt * T::BM, n0 = nt * T::BN;
+    const uint32_t KB = (g.K + KBLK - 1) / KBLK, NB = (g.N + KBLK - 1) / KBLK;
+
+    auto rsrc = [](const void *p, size_t bytes) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, (uint32_t)bytes, 0x00020000);
+    };
+    const uint32_t rows_a = min((uint32_t)T::BM, g.M - m0), rows_b = min((uint32_t)T::BN, g.N - n0);
+    const uint32_t nb0 = n0 / KBLK, nbs = min((uint32_t)((T::BN + KBLK - 1) / KBLK), NB - nb0);
+    const __amdgpu_buffer_rsrc_t ra = rsrc(g.a + (size_t)m0 * g.K, (size_t)rows_a * g.K);
+    const __amdgpu_buffer_rsrc_t rb = rsrc(g.b + (size_t)n0 * g.K, (size_t)rows_b * g.K);
+    const __amdgpu_buffer_rsrc_t rsa = rsrc(g.sa + (size_t)m0 * KB, (size_t)rows_a * KB * 4);
+    const __amdgpu_buffer_rsrc_t rsb = rsrc(g.sb + (size_t)nb0 * KB, (size_t)nbs * KB * 4);
+    // Lane part of a copy of 8 rows: row lane / 8, the chunk that lands in slot lane % 8; the
+    // permutation repeats every four copies.
+    uint32_t voff[4], chunk[4];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+        chunk[v] = (lane % 8) ^ pipe::swz<8>(8 * v + lane / 8);
+        voff[v] = lane / 8 * g.K + 16 * chunk[v];
+    }
+    const uint32_t none = 0x7fffffffu;   // past every resource
+    auto issue = [&](uint32_t step) __attribute__((always_inline)) {
+        uint8_t *base = lds + (step % S) * T::STAGE;
+        const uint32_t ko = step * KBLK, left = g.K - ko;   // codes of k left: fewer than a block in the last stage
+        uint32_t vo[4];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) vo[v] = left < KBLK && 16 * chunk[v] >= left ? none : voff[v] + ko;
+#pragma unroll
+        for (int c = 0; c < T::LA; ++c) {
+            const uint32_t r = (wave * T::LA + c) * 8;
+            pipe::copy16_buf(ra, base + r * 128, vo[(T::LA % 4 ? r / 8 : c) % 4], r * g.K);
+        }
+#pragma unroll
+        for (int c = 0; c < T::LB; ++c) {
+            const uint32_t r = (wave * T::LB + c) * 8;
+            pipe::copy16_buf(rb, base + T::A_BYTES + r * 128, vo[(T::LB % 4 ? r / 8 : c) % 4], r * g.K);
+        }
+        // Scales: 64 rows of a a copy, then the blocks of b.
+        uint8_t *sc = lds + S * T::STAGE + (step % S) * T::SC;
+#pragma unroll
+        for (int c = 0; c < T::LS; ++c) {
+            const uint32_t w = min(wave + c * T::NW, (uint32_t)T::BM / 64);
+            const bool of_b = w == T::BM / 64;
+            pipe::copy4_buf(of_b ? rsb : rsa, sc + w * 256, ((of_b ? 0 : w * 64) + lane) * KB * 4 + step * 4);
+        }
+    };
+
+    const uint32_t sw = pipe::swz<8>(row), o0 = (q ^ sw) * 16, o1 = ((q + 4) ^ sw) * 16;
+    // Rows 16 i .. of a wave's operand: the permutation's second half differs by 16 rows.
+    auto frag = [&](const uint8_t *base, int i) __attribute__((always_inline)) {
+        const uint32_t flip = (i & 1) ? 2 * 16 : 0;   // swz<8>(r + 16) = swz<8>(r) ^ 2
+        const uint8_t *p = base + (16 * i + row) * 128;
+        return join(*reinterpret_cast<const u32x4 *>(p + (o0 ^ flip)), *reinterpret_cast<const u32x4 *>(p + (o1 ^ flip)));
+    };
+    auto a_of = [&](uint32_t step) { return lds + (step % S) * T::STAGE + wm * (16 * TM * 128); };
+    auto b_of = [&](uint32_t step) { return lds + (step % S) * T::STAGE + T::A_BYTES + wn * (16 * TN * 128); };
+
+    f32x4 acc[TM][TN], part[PART + 1];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i <= PART; ++i) part[i] = f32x4{0, 0, 0, 0};
+    constexpr int R = TM % 4 == 0 ? 4 : 2;   // activation fragments held: two rows are read ahead, or the row after next
+    static_assert(TM % R == 0, "the ring of fragments keeps its place from stage to stage");
+    i32x8 fa[R], fb[TN];
+    float sa[TM], last = 0.0f;   // this stage's scales; the last row's of the stage before
+
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+        if (s < (int)KB) issue(s);
+    auto landed = [&](uint32_t step) {   // this wave's copies of a stage; later ones may be in flight
+        if (S > 2 && step + S - 2 < KB) pipe::wait_vmcnt<(S - 2) * T::LOADS>();
+        else pipe::wait_vmcnt<0>();
+    };
+    pipe::wait_vmcnt<0>();
+    pipe::lds_barrier();
+    fa[0] = frag(a_of(0), 0);
+    fa[1] = frag(a_of(0), 1);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) fb[j] = frag(b_of(0), j);
+
+    for (uint32_t t = 0; t < KB; ++t) {
+        const uint8_t *sc = lds + S * T::STAGE + (t % S) * T::SC;
+        const float sb = *reinterpret_cast<const float *>(sc + 4 * T::BM + 4 * (wn * (16 * TN) / KBLK));
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+            sa[i] = *reinterpret_cast<const float *>(sc + 4 * (wm * (16 * TM) + 16 * i + row)) * sb;
+        const bool more = t + 1 < KB;
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            if (R == 4 && i + 2 < TM) fa[(i + 2) % R] = frag(a_of(t), i + 2);
+            if (i == TM - 2 && more) {
+                // Every fragment and scale of this stage is in registers, and the next stage has
+                // landed: behind the barrier its slot is read and this stage's is written.
+                pipe::wait_lgkm0();
+                landed(t + 1);
+                pipe::lds_barrier();
+                if (t + S < KB) issue(t + S);
+            }
+            if (R == 4 && i >= TM - 2 && more) fa[(i + 2) % R] = frag(a_of(t + 1), i + 2 - TM);
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                const int p = i * TN + j, d = p - PART, e = d < 0 ? TM * TN + d : d;   // e: the product that is added now
+                part[p % (PART + 1)] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                    fb[j], fa[i % R], f32x4{0, 0, 0, 0}, FB, FA, 0, 0, 0, 0);
+                const float s = d < 0 ? last : sa[e / TN];
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    acc[e / TN][e % TN][x] = fmaf(part[(p + 1) % (PART + 1)][x], s, acc[e / TN][e % TN][x]);
+                if (i == TM - 1 && more) fb[j] = frag(b_of(t + 1), j);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (R == 2 && more) fa[i % R] = frag(a_of(t + 1), i);
+        }
+        last = sa[TM - 1];
+    }
+
+    // The products still to be added.
+#pragma unroll
+    for (int e = TM * TN - PART; e < TM * TN; ++e)
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            acc[e / TN][e % TN][x] = fmaf(part[e % (PART + 1)][x], last, acc[e / TN][e % TN][x]);
+    static_assert((TM * TN) % (PART + 1) == 0 && PART <= TN, "the parts' ring keeps its place from stage to stage");
+
+    // Epilogue through LDS: a lane holds four consecutive columns of a row; the workgroup
+    // stores whole row segments.
+    __syncthreads();
+    constexpr uint32_t RB = T::BN * 2 + 16;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            const f32x4 v = acc[i][j];
+            *reinterpret_cast<u32x2 *>(lds + (wm * (16 * TM) + 16 * i + row) * RB + 2 * (wn * (16 * TN) + 16 * j + 4 * q)) =
+                u32x2{f32_to_bf16_bits(v.x) | (f32_to_bf16_bits(v.y) << 16),
+                      f32_to_bf16_bits(v.z) | (f32_to_bf16_bits(v.w) << 16)};
+        }
+    __syncthreads();
+    constexpr uint32_t CC = T::BN / 8;
+    const bool vec = g.N % 8 == 0 && reinterpret_cast<uintptr_t>(g.out) % 16 == 0;
+    for (uint32_t i = tid; i < T::BM * CC; i += 64 * T::NW) {
+        const uint32_t r = i / CC, c = i % CC, m = m0 + r, n = n0 + 8 * c;
+        if (m >= g.M || n >= g.N) continue;
+        const u32x4 v = *reinterpret_cast<const u32x4 *>(lds + r * RB + 16 * c);
+        uint16_t *out = g.out + (size_t)m * g.N + n;
+        if (vec) {
+            __builtin_nontemporal_store(v, reinterpret_cast<u32x4 *>(out));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (n + e < g.N) out[e] = (uint16_t)(v[e / 2] >> (16 * (e % 2)));
+        }
+    }
+}
+
+template <int FA, int FB, typename T>
+int launch_tiles(const BlockArgs &g, hipStream_t st) {
+    const uint32_t tiles_m = (g.M + T::BM - 1) / T::BM, tiles_n = (g.N + T::BN - 1) / T::BN, tiles = tiles_m * tiles_n;
+    hipLaunchKernelGGL((gemm_blocks_tiles<FA, FB, T>), dim3(tiles), dim3(64 * T::NW), T::LDS, st, g, tiles_m, tiles,
+                       wide_mapm(tiles_m, tiles_n, T::BM, T::BN));
+    return check_launch("gemm_blocks_tiles");
+}
+
+using Tile256 = BlockTile<8, 4, 2, 4, 2>;
+using Tile128 = BlockTile<4, 4, 2, 2, 2>;
+using Tile64 = BlockTile<2, 4, 2, 1, 3>;
+
 template <int FA, int FB>
 int launch_blocks(const BlockArgs &g, hipStream_t st) {
+    if (g.M > 64) {
+        const uint64_t cus = (uint64_t)device_props().cus;
+        auto tiles = [&](uint64_t b) { return ((g.M + b - 1) / b) * ((g.N + b - 1) / b); };
+        if (tiles(256) >= cus) return launch_tiles<FA, FB, Tile256>(g, st);
+        if (tiles(128) >= cus) return launch_tiles<FA, FB, Tile128>(g, st);
+        return launch_tiles<FA, FB, Tile64>(g, st);
+    }
     constexpr int W = 8;
     const uint64_t tiles_n = (g.N + 15) / 16;
     auto go = [&](auto mt_c) {

@@ -53,9 +53,14 @@ __device__ __forceinline__ void copy16_to_lds(const uint8_t *g, uint8_t *l) {
 }
 
 // The same through a buffer resource: the lane's part of the address in voff, the
-// copy's in the scalar soff; bytes past the resource's size are not read.
+// copy's in the scalar soff; a lane past the resource's size leaves zeros.
 __device__ __forceinline__ void copy16_buf(__amdgpu_buffer_rsrc_t r, uint8_t *l, uint32_t voff, uint32_t soff) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)l, 16, voff, soff, 0, 0);
+}
+
+// Four bytes a lane.
+__device__ __forceinline__ void copy4_buf(__amdgpu_buffer_rsrc_t r, uint8_t *l, uint32_t voff) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)l, 4, voff, 0, 0, 0);
 }
 
 // copy16_buf as inline asm, which the compiler does not know to write LDS: it puts
