@@ -121,8 +121,8 @@ struct BlockTile {
     static constexpr int LDS = RING > OUT ? RING : OUT;
     static constexpr int PART = 3;
     static_assert(LA * 8 * NW == BM && LB * 8 * NW == BN, "copies split evenly");
-    static_assert((TM == 2 || TM % 4 == 0) && 16 * TN <= 128 && 128 % (16 * TN) == 0, "a wave's columns share a scale");
-    static_assert((S - 2) * LOADS < 64 && S >= 2 && LDS <= 160 * 1024, "vmcnt range, LDS");
+    static_assert(TM % 2 == 0 && 16 * TN <= 128 && 128 % (16 * TN) == 0, "a wave's columns share a scale");
+    static_assert((S - 1) * LOADS < 64 && S >= 2 && LDS <= 160 * 1024, "vmcnt range, LDS");
 };
 
 template <int FA, int FB, typename T>
@@ -146,38 +146,37 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_blocks_tiles(BlockArgs g, uin
     const __amdgpu_buffer_rsrc_t rb = rsrc(g.b + (size_t)n0 * g.K, (size_t)rows_b * g.K);
     const __amdgpu_buffer_rsrc_t rsa = rsrc(g.sa + (size_t)m0 * KB, (size_t)rows_a * KB * 4);
     const __amdgpu_buffer_rsrc_t rsb = rsrc(g.sb + (size_t)nb0 * KB, (size_t)nbs * KB * 4);
-    // Lane part of a copy of 8 rows: row lane / 8, the chunk that lands in slot lane % 8; the
-    // permutation repeats every four copies.
-    uint32_t voff[4], chunk[4];
+    // A copy brings 8 rows: lane l the chunk of row l / 8 that lands in slot l % 8. The whole
+    // offset is the lane's (the scalar one would not count in the range check).
+    auto chunk_at = [&](uint32_t r) { return 16 * ((lane % 8) ^ pipe::swz<8>((r + lane / 8) & 31)); };
+    uint32_t va[T::LA], vb[T::LB];
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
-        chunk[v] = (lane % 8) ^ pipe::swz<8>(8 * v + lane / 8);
-        voff[v] = lane / 8 * g.K + 16 * chunk[v];
-    }
-    const uint32_t none = 0x7fffffffu;   // past every resource
+    for (int c = 0; c < T::LA; ++c) va[c] = ((wave * T::LA + c) * 8 + lane / 8) * g.K;
+#pragma unroll
+    for (int c = 0; c < T::LB; ++c) vb[c] = ((wave * T::LB + c) * 8 + lane / 8) * g.K;
+    // Straight-line code, like all of the loop below: products wait in registers for their
+    // addition, and the compiler would move the additions behind a branch.
     auto issue = [&](uint32_t step) __attribute__((always_inline)) {
-        uint8_t *base = lds + (step % S) * T::STAGE;
-        const uint32_t ko = step * KBLK, left = g.K - ko;   // codes of k left: fewer than a block in the last stage
-        uint32_t vo[4];
-#pragma unroll
-        for (int v = 0; v < 4; ++v) vo[v] = left < KBLK && 16 * chunk[v] >= left ? none : voff[v] + ko;
+        uint8_t *base = lds + (step % S) * T::STAGE, *scales = lds + S * T::STAGE + (step % S) * T::SC;
+        step = min(step, KB - 1);   // past the last stage: that one again, into a slot that is not read
+        const uint32_t ko = step * KBLK, left = g.K - ko;   // codes of k left
+        const uint32_t none = 0x7fffffffu;   // past every resource
 #pragma unroll
         for (int c = 0; c < T::LA; ++c) {
-            const uint32_t r = (wave * T::LA + c) * 8;
-            pipe::copy16_buf(ra, base + r * 128, vo[(T::LA % 4 ? r / 8 : c) % 4], r * g.K);
+            const uint32_t r = (wave * T::LA + c) * 8, ch = chunk_at(r);
+            pipe::copy16_buf(ra, base + r * 128, ch < left ? va[c] + (ko + ch) : none, 0);
         }
 #pragma unroll
         for (int c = 0; c < T::LB; ++c) {
-            const uint32_t r = (wave * T::LB + c) * 8;
-            pipe::copy16_buf(rb, base + T::A_BYTES + r * 128, vo[(T::LB % 4 ? r / 8 : c) % 4], r * g.K);
+            const uint32_t r = (wave * T::LB + c) * 8, ch = chunk_at(r);
+            pipe::copy16_buf(rb, base + T::A_BYTES + r * 128, ch < left ? vb[c] + (ko + ch) : none, 0);
         }
         // Scales: 64 rows of a a copy, then the blocks of b.
-        uint8_t *sc = lds + S * T::STAGE + (step % S) * T::SC;
 #pragma unroll
         for (int c = 0; c < T::LS; ++c) {
             const uint32_t w = min(wave + c * T::NW, (uint32_t)T::BM / 64);
             const bool of_b = w == T::BM / 64;
-            pipe::copy4_buf(of_b ? rsb : rsa, sc + w * 256, ((of_b ? 0 : w * 64) + lane) * KB * 4 + step * 4);
+            pipe::copy4_buf(of_b ? rsb : rsa, scales + w * 256, ((of_b ? 0 : w * 64) + lane) * KB * 4 + step * 4);
         }
     };
 
@@ -198,19 +197,14 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_blocks_tiles(BlockArgs g, uin
         for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i <= PART; ++i) part[i] = f32x4{0, 0, 0, 0};
-    constexpr int R = TM % 4 == 0 ? 4 : 2;   // activation fragments held: two rows are read ahead, or the row after next
+    constexpr int R = TM == 4 ? 4 : 2;   // activation fragments held: two rows are read ahead, or the row after next
     static_assert(TM % R == 0, "the ring of fragments keeps its place from stage to stage");
     i32x8 fa[R], fb[TN];
     float sa[TM], last = 0.0f;   // this stage's scales; the last row's of the stage before
 
 #pragma unroll
-    for (int s = 0; s < S; ++s)
-        if (s < (int)KB) issue(s);
-    auto landed = [&](uint32_t step) {   // this wave's copies of a stage; later ones may be in flight
-        if (S > 2 && step + S - 2 < KB) pipe::wait_vmcnt<(S - 2) * T::LOADS>();
-        else pipe::wait_vmcnt<0>();
-    };
-    pipe::wait_vmcnt<0>();
+    for (int s = 0; s < S; ++s) issue(s);
+    pipe::wait_vmcnt<(S - 1) * T::LOADS>();
     pipe::lds_barrier();
     fa[0] = frag(a_of(0), 0);
     fa[1] = frag(a_of(0), 1);
@@ -223,19 +217,18 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_blocks_tiles(BlockArgs g, uin
 #pragma unroll
         for (int i = 0; i < TM; ++i)
             sa[i] = *reinterpret_cast<const float *>(sc + 4 * (wm * (16 * TM) + 16 * i + row)) * sb;
-        const bool more = t + 1 < KB;
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
             if (R == 4 && i + 2 < TM) fa[(i + 2) % R] = frag(a_of(t), i + 2);
-            if (i == TM - 2 && more) {
+            if (i == TM - 2) {
                 // Every fragment and scale of this stage is in registers, and the next stage has
                 // landed: behind the barrier its slot is read and this stage's is written.
                 pipe::wait_lgkm0();
-                landed(t + 1);
+                pipe::wait_vmcnt<(S - 2) * T::LOADS>();
                 pipe::lds_barrier();
-                if (t + S < KB) issue(t + S);
+                issue(t + S);
             }
-            if (R == 4 && i >= TM - 2 && more) fa[(i + 2) % R] = frag(a_of(t + 1), i + 2 - TM);
+            if (R == 4 && i >= TM - 2) fa[(i + 2) % R] = frag(a_of(t + 1), i + 2 - TM);
 #pragma unroll
             for (int j = 0; j < TN; ++j) {
                 const int p = i * TN + j, d = p - PART, e = d < 0 ? TM * TN + d : d;   // e: the product that is added now
@@ -245,10 +238,10 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_blocks_tiles(BlockArgs g, uin
 #pragma unroll
                 for (int x = 0; x < 4; ++x)
                     acc[e / TN][e % TN][x] = fmaf(part[(p + 1) % (PART + 1)][x], s, acc[e / TN][e % TN][x]);
-                if (i == TM - 1 && more) fb[j] = frag(b_of(t + 1), j);
+                if (i == TM - 1) fb[j] = frag(b_of(t + 1), j);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if (R == 2 && more) fa[i % R] = frag(a_of(t + 1), i);
+            if (R == 2) fa[i % R] = i + 2 < TM ? frag(a_of(t), i + 2) : frag(a_of(t + 1), i + 2 - TM);
         }
         last = sa[TM - 1];
     }
@@ -260,6 +253,8 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_blocks_tiles(BlockArgs g, uin
         for (int x = 0; x < 4; ++x)
             acc[e / TN][e % TN][x] = fmaf(part[e % (PART + 1)][x], last, acc[e / TN][e % TN][x]);
     static_assert((TM * TN) % (PART + 1) == 0 && PART <= TN, "the parts' ring keeps its place from stage to stage");
+
+    pipe::wait_vmcnt<0>();   // the copies past the last stage, before LDS holds outputs
 
     // Epilogue through LDS: a lane holds four consecutive columns of a row; the workgroup
     // stores whole row segments.
@@ -301,6 +296,8 @@ int launch_tiles(const BlockArgs &g, hipStream_t st) {
 }
 
 using Tile256 = BlockTile<8, 4, 2, 4, 2>;
+using Tile256x128 = BlockTile<4, 4, 4, 2, 3>;
+using Tile192 = BlockTile<6, 4, 2, 4, 2>;
 using Tile128 = BlockTile<4, 4, 2, 2, 2>;
 using Tile64 = BlockTile<2, 4, 2, 1, 3>;
 
