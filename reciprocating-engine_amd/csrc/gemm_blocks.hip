@@ -180,7 +180,7 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_blocks_tiles(BlockArgs g, uin
         }
     };
 
-    const uint32_t sw = pipe::swz<8>(row), o0 = (q ^ sw) * 16, o1 = ((q + 4) ^ sw) * 16;
+    const uint32_t sw = pipe::swz<8>(row), o0 = (2 * q ^ sw) * 16, o1 = ((2 * q + 1) ^ sw) * 16;
     // Rows 16 i .. of a wave's operand: the permutation's second half differs by 16 rows.
     auto frag = [&](const uint8_t *base, int i) __attribute__((always_inline)) {
         const uint32_t flip = (i & 1) ? 2 * 16 : 0;   // swz<8>(r + 16) = swz<8>(r) ^ 2
