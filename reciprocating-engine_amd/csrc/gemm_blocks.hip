@@ -101,9 +101,11 @@ __global__ __launch_bounds__(64 * W) void gemm_blocks_rows(BlockArgs g, uint32_t
 // ------------------------------------------------------------ output tiles
 //
 // BM x BN outputs a workgroup, WGM x WGN waves of 16 TM x 16 TN, K in stages of one
-// scale block. A stage's operand rows and its BM + BN / 128 scales are copied to an
+// scale block. A stage's operand rows are copied to an
 // S-slot LDS ring (16-byte chunks of a row permuted by swz, so that fragment reads
-// are free of bank conflicts). A wave keeps its TN weight fragments of a stage in
+// are free of bank conflicts; the scales four stages at a time, 16 bytes of a row:
+// one stage's are 4 bytes of BM different lines, which cost the copies of the codes
+// 10-40%). A wave keeps its TN weight fragments of a stage in
 // registers and goes through the TM activation fragments; the 16 x 16 product of a
 // stage (one v_mfma_f32_16x16x128) is scaled and added to the accumulator PART
 // products later, so that the vector unit works while the matrix cores do. The next
@@ -114,15 +116,17 @@ template <int TM_, int TN_, int WGM_, int WGN_, int S_>
 struct BlockTile {
     static constexpr int TM = TM_, TN = TN_, WGM = WGM_, WGN = WGN_, S = S_, NW = WGM * WGN;
     static constexpr int BM = 16 * TM * WGM, BN = 16 * TN * WGN;
-    static constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128, SC = 4 * (BM + 64);   // the weight's scales in the last 64
-    static constexpr int STAGE = A_BYTES + B_BYTES, RING = S * (STAGE + SC);
-    static constexpr int LA = BM / 8 / NW, LB = BN / 8 / NW, LS = (BM / 64 + 1 + NW - 1) / NW, LOADS = LA + LB + LS;
+    static constexpr int A_BYTES = BM * 128, B_BYTES = BN * 128, STAGE = A_BYTES + B_BYTES;
+    static constexpr int G = 4, SC = 4 * G * (BM + 64);   // scales of G stages: BM rows', then the weight's blocks'
+    static constexpr int RING = S * STAGE + 2 * SC;
+    static constexpr int LA = BM / 8 / NW, LB = BN / 8 / NW, LOADS = LA + LB;
+    static constexpr int LS = (BM / 64 + 1 + NW - 1) / NW;   // scale copies a wave, every G stages
     static constexpr int OUT = BM * (BN * 2 + 16);   // the epilogue's rows, padded by a chunk
     static constexpr int LDS = RING > OUT ? RING : OUT;
     static constexpr int PART = 3;
     static_assert(LA * 8 * NW == BM && LB * 8 * NW == BN, "copies split evenly");
     static_assert(TM % 2 == 0 && 16 * TN <= 128 && 128 % (16 * TN) == 0, "a wave's columns share a scale");
-    static_assert((S - 1) * LOADS < 64 && S >= 2 && LDS <= 160 * 1024, "vmcnt range, LDS");
+    static_assert((S - 1) * LOADS < 64 && S >= 2 && S <= 3 && LDS <= 160 * 1024, "vmcnt range, LDS");
 };
 
 template <int FA, int FB, typename T>
@@ -157,7 +161,7 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_blocks_tiles(BlockArgs g, uin
     // Straight-line code, like all of the loop below: products wait in registers for their
     // addition, and the compiler would move the additions behind a branch.
     auto issue = [&](uint32_t step) __attribute__((always_inline)) {
-        uint8_t *base = lds + (step % S) * T::STAGE, *scales = lds + S * T::STAGE + (step % S) * T::SC;
+        uint8_t *base = lds + (step % S) * T::STAGE;
         step = min(step, KB - 1);   // past the last stage: that one again, into a slot that is not read
         const uint32_t ko = step * KBLK, left = g.K - ko;   // codes of k left
         const uint32_t none = 0x7fffffffu;   // past every resource
@@ -171,12 +175,17 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_blocks_tiles(BlockArgs g, uin
             const uint32_t r = (wave * T::LB + c) * 8, ch = chunk_at(r);
             pipe::copy16_buf(rb, base + T::A_BYTES + r * 128, ch < left ? vb[c] + (ko + ch) : none, 0);
         }
-        // Scales: 64 rows of a a copy, then the blocks of b.
+    };
+    // The scales of stages G grp .. G grp + 3: 64 rows of a a copy, then the blocks of b.
+    // (Those behind a row's last are the next row's and are not used.)
+    auto issue_scales = [&](uint32_t grp) __attribute__((always_inline)) {
+        uint8_t *to = lds + S * T::STAGE + (grp & 1) * T::SC;
 #pragma unroll
         for (int c = 0; c < T::LS; ++c) {
             const uint32_t w = min(wave + c * T::NW, (uint32_t)T::BM / 64);
             const bool of_b = w == T::BM / 64;
-            pipe::copy4_buf(of_b ? rsb : rsa, scales + w * 256, ((of_b ? 0 : w * 64) + lane) * KB * 4 + step * 4);
+            pipe::copy16_buf(of_b ? rsb : rsa, to + w * (64 * 4 * T::G),
+                             (((of_b ? 0 : w * 64) + lane) * KB + grp * T::G) * 4, 0);
         }
     };
 
@@ -203,7 +212,10 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_blocks_tiles(BlockArgs g, uin
     float sa[TM], last = 0.0f;   // this stage's scales; the last row's of the stage before
 
 #pragma unroll
-    for (int s = 0; s < S; ++s) issue(s);
+    for (int s = 0; s < S; ++s) {
+        if (s == 0) issue_scales(0);
+        issue(s);
+    }
     pipe::wait_vmcnt<(S - 1) * T::LOADS>();
     pipe::lds_barrier();
     fa[0] = frag(a_of(0), 0);
@@ -212,11 +224,11 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_blocks_tiles(BlockArgs g, uin
     for (int j = 0; j < TN; ++j) fb[j] = frag(b_of(0), j);
 
     for (uint32_t t = 0; t < KB; ++t) {
-        const uint8_t *sc = lds + S * T::STAGE + (t % S) * T::SC;
-        const float sb = *reinterpret_cast<const float *>(sc + 4 * T::BM + 4 * (wn * (16 * TN) / KBLK));
+        const uint8_t *sc = lds + S * T::STAGE + (t / T::G & 1) * T::SC + t % T::G * 4;
+        const float sb = *reinterpret_cast<const float *>(sc + 4 * T::G * (T::BM + wn * (16 * TN) / KBLK));
 #pragma unroll
         for (int i = 0; i < TM; ++i)
-            sa[i] = *reinterpret_cast<const float *>(sc + 4 * (wm * (16 * TM) + 16 * i + row)) * sb;
+            sa[i] = *reinterpret_cast<const float *>(sc + 4 * T::G * (wm * (16 * TM) + 16 * i + row)) * sb;
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
             if (R == 4 && i + 2 < TM) fa[(i + 2) % R] = frag(a_of(t), i + 2);
@@ -227,6 +239,13 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_blocks_tiles(BlockArgs g, uin
                 pipe::wait_vmcnt<(S - 2) * T::LOADS>();
                 pipe::lds_barrier();
                 issue(t + S);
+                // Every fourth stage the next four's scales. The sums are held here: the compiler
+                // would move additions behind the branch.
+#pragma unroll
+                for (int x = 0; x < TM; ++x)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) asm volatile("" : "+v"(acc[x][j]));
+                if (t % T::G == 0 && t + T::G < KB) issue_scales(t / T::G + 1);
             }
             if (R == 4 && i >= TM - 2) fa[(i + 2) % R] = frag(a_of(t + 1), i + 2 - TM);
 #pragma unroll
