@@ -124,6 +124,8 @@ struct BlockTile {
     static constexpr int OUT = BM * (BN * 2 + 16);   // the epilogue's rows, padded by a chunk
     static constexpr int LDS = RING > OUT ? RING : OUT;
     static constexpr int PART = 3;
+    static constexpr bool TURNS = TM == 8;   // the halves of the rows take turns
+    static_assert(!TURNS || (WGM == 2 && WGN == 4 && S == 2), "a wave of each half on a SIMD");
     static_assert(LA * 8 * NW == BM && LB * 8 * NW == BN, "copies split evenly");
     static_assert(TM % 2 == 0 && 16 * TN <= 128 && 128 % (16 * TN) == 0, "a wave's columns share a scale");
     static_assert((S - 1) * LOADS < 64 && S >= 2 && S <= 3 && LDS <= 160 * 1024, "vmcnt range, LDS");
@@ -160,21 +162,31 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_blocks_tiles(BlockArgs g, uin
     for (int c = 0; c < T::LB; ++c) vb[c] = ((wave * T::LB + c) * 8 + lane / 8) * g.K;
     // Straight-line code, like all of the loop below: products wait in registers for their
     // addition, and the compiler would move the additions behind a branch.
-    auto issue = [&](uint32_t step) __attribute__((always_inline)) {
+    const uint32_t none = 0x7fffffffu;   // past every resource
+    auto issue_a = [&](uint32_t step) __attribute__((always_inline)) {
         uint8_t *base = lds + (step % S) * T::STAGE;
         step = min(step, KB - 1);   // past the last stage: that one again, into a slot that is not read
         const uint32_t ko = step * KBLK, left = g.K - ko;   // codes of k left
-        const uint32_t none = 0x7fffffffu;   // past every resource
 #pragma unroll
         for (int c = 0; c < T::LA; ++c) {
             const uint32_t r = (wave * T::LA + c) * 8, ch = chunk_at(r);
-            pipe::copy16_buf(ra, base + r * 128, ch < left ? va[c] + (ko + ch) : none, 0);
+            pipe::copy16_buf_asm(ra, base + r * 128, ch < left ? va[c] + (ko + ch) : none);
         }
+    };
+    auto issue_b = [&](uint32_t step, int from, int to) __attribute__((always_inline)) {
+        uint8_t *base = lds + (step % S) * T::STAGE + T::A_BYTES;
+        step = min(step, KB - 1);
+        const uint32_t ko = step * KBLK, left = g.K - ko;
 #pragma unroll
         for (int c = 0; c < T::LB; ++c) {
+            if (c < from || c >= to) continue;
             const uint32_t r = (wave * T::LB + c) * 8, ch = chunk_at(r);
-            pipe::copy16_buf(rb, base + T::A_BYTES + r * 128, ch < left ? vb[c] + (ko + ch) : none, 0);
+            pipe::copy16_buf_asm(rb, base + r * 128, ch < left ? vb[c] + (ko + ch) : none);
         }
+    };
+    auto issue = [&](uint32_t step) __attribute__((always_inline)) {
+        issue_a(step);
+        issue_b(step, 0, T::LB);
     };
     // The scales of stages G grp .. G grp + 3: 64 rows of a a copy, then the blocks of b.
     // (Those behind a row's last are the next row's and are not used.)
@@ -184,8 +196,8 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_blocks_tiles(BlockArgs g, uin
         for (int c = 0; c < T::LS; ++c) {
             const uint32_t w = min(wave + c * T::NW, (uint32_t)T::BM / 64);
             const bool of_b = w == T::BM / 64;
-            pipe::copy16_buf(of_b ? rsb : rsa, to + w * (64 * 4 * T::G),
-                             (((of_b ? 0 : w * 64) + lane) * KB + grp * T::G) * 4, 0);
+            pipe::copy16_buf_asm(of_b ? rsb : rsa, to + w * (64 * 4 * T::G),
+                                 (((of_b ? 0 : w * 64) + lane) * KB + grp * T::G) * 4);
         }
     };
 
@@ -206,11 +218,108 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_blocks_tiles(BlockArgs g, uin
         for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i <= PART; ++i) part[i] = f32x4{0, 0, 0, 0};
-    constexpr int R = TM == 4 ? 4 : 2;   // activation fragments held: two rows are read ahead, or the row after next
+    constexpr int R = TM % 4 == 0 ? 4 : 2;   // activation fragments held: two rows are read ahead, or the row after next
     static_assert(TM % R == 0, "the ring of fragments keeps its place from stage to stage");
     i32x8 fa[R], fb[TN];
     float sa[TM], last = 0.0f;   // this stage's scales; the last row's of the stage before
 
+    // The sums are held here: the compiler would move additions behind a branch.
+    auto hold = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < TM; ++x)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) asm volatile("" : "+v"(acc[x][j]));
+    };
+    auto read_scales = [&](uint32_t t) __attribute__((always_inline)) {
+        const uint8_t *sc = lds + S * T::STAGE + (t / T::G & 1) * T::SC + t % T::G * 4;
+        const float sb = *reinterpret_cast<const float *>(sc + 4 * T::G * (T::BM + wn * (16 * TN) / KBLK));
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+            sa[i] = *reinterpret_cast<const float *>(sc + 4 * T::G * (wm * (16 * TM) + 16 * i + row)) * sb;
+    };
+    // Product (i, j) of a stage is begun, and the one PART before it scaled and added.
+    auto product = [&](int i, int j, const i32x8 &f) __attribute__((always_inline)) {
+        const int p = i * TN + j, d = p - PART, e = d < 0 ? TM * TN + d : d;
+        part[p % (PART + 1)] =
+            __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], f, f32x4{0, 0, 0, 0}, FB, FA, 0, 0, 0, 0);
+        const float s = d < 0 ? last : sa[e / TN];
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            acc[e / TN][e % TN][x] = fmaf(part[(p + 1) % (PART + 1)][x], s, acc[e / TN][e % TN][x]);
+    };
+
+    if constexpr (T::TURNS) {
+        // The two halves of the tile's rows take turns, a wave of each on a SIMD: while one half's
+        // products run, the other copies its rows of a later stage and reads the first fragments
+        // of its next one, which together take as long. A phase ends at a barrier; the second
+        // half runs one behind. The first half's products of stage t are phase 2 t, its turnover
+        // 2 t + 1, the second's 2 t + 1 and 2 t + 2. Both halves have stage t's weight fragments
+        // in registers by the end of phase 2 t, so its slot takes the weight codes of stage t + 2
+        // in phase 2 t + 1 (a share of each half), the first half's rows in 2 t + 1, the second's
+        // in 2 t + 2; each has landed two phases later.
+        auto turnover = [&](uint32_t t) __attribute__((always_inline)) {
+            last = sa[TM - 1];
+            fa[0] = frag(a_of(t), 0);
+            fa[1] = frag(a_of(t), 1);
+#pragma unroll
+            for (int j = 0; j < TN; ++j) fb[j] = frag(b_of(t), j);
+            read_scales(t);
+        };
+        auto barrier = [&]() __attribute__((always_inline)) {
+            pipe::wait_lgkm0();
+            pipe::lds_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        auto products = [&](uint32_t t, auto copy_c) __attribute__((always_inline)) {
+            constexpr bool COPY = decltype(copy_c)::value;
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                if (i + 2 < TM) fa[(i + 2) % R] = frag(a_of(t), i + 2);
+                if (COPY && i < T::LB) issue_b(t + 2, i, i + 1);
+#pragma unroll
+                for (int j = 0; j < TN; ++j) {
+                    product(i, j, fa[i % R]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            hold();
+        };
+#pragma unroll
+        for (int i = 0; i < TM; ++i) sa[i] = 0.0f;
+        issue_scales(0);
+        issue(0);
+        issue(1);
+        pipe::wait_vmcnt<0>();
+        barrier();
+        if (wm == 0) {
+            turnover(0);
+            barrier();
+            for (uint32_t t = 0; t < KB; ++t) {
+                products(t, std::false_type{});
+                pipe::wait_vmcnt<0>();
+                barrier();
+                if (t % T::G == 0 && t + T::G < KB) issue_scales(t / T::G + 1);
+                issue(t + 2);
+                turnover(t + 1);
+                barrier();
+            }
+            barrier();
+        } else {
+            barrier();
+            turnover(0);
+            barrier();
+            for (uint32_t t = 0; t < KB; ++t) {
+                products(t, std::true_type{});
+                pipe::wait_vmcnt<T::LB>();
+                barrier();
+                if (t % T::G == 0 && t + T::G < KB) issue_scales(t / T::G + 1);
+                issue_a(t + 2);
+                turnover(t + 1);
+                pipe::wait_vmcnt<T::LA>();
+                barrier();
+            }
+        }
+    } else {
 #pragma unroll
     for (int s = 0; s < S; ++s) {
         if (s == 0) issue_scales(0);
@@ -224,11 +333,7 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_blocks_tiles(BlockArgs g, uin
     for (int j = 0; j < TN; ++j) fb[j] = frag(b_of(0), j);
 
     for (uint32_t t = 0; t < KB; ++t) {
-        const uint8_t *sc = lds + S * T::STAGE + (t / T::G & 1) * T::SC + t % T::G * 4;
-        const float sb = *reinterpret_cast<const float *>(sc + 4 * T::G * (T::BM + wn * (16 * TN) / KBLK));
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-            sa[i] = *reinterpret_cast<const float *>(sc + 4 * T::G * (wm * (16 * TM) + 16 * i + row)) * sb;
+        read_scales(t);
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
             if (R == 4 && i + 2 < TM) fa[(i + 2) % R] = frag(a_of(t), i + 2);
@@ -241,22 +346,13 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_blocks_tiles(BlockArgs g, uin
                 issue(t + S);
                 // Every fourth stage the next four's scales. The sums are held here: the compiler
                 // would move additions behind the branch.
-#pragma unroll
-                for (int x = 0; x < TM; ++x)
-#pragma unroll
-                    for (int j = 0; j < TN; ++j) asm volatile("" : "+v"(acc[x][j]));
+                hold();
                 if (t % T::G == 0 && t + T::G < KB) issue_scales(t / T::G + 1);
             }
             if (R == 4 && i >= TM - 2) fa[(i + 2) % R] = frag(a_of(t + 1), i + 2 - TM);
 #pragma unroll
             for (int j = 0; j < TN; ++j) {
-                const int p = i * TN + j, d = p - PART, e = d < 0 ? TM * TN + d : d;   // e: the product that is added now
-                part[p % (PART + 1)] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                    fb[j], fa[i % R], f32x4{0, 0, 0, 0}, FB, FA, 0, 0, 0, 0);
-                const float s = d < 0 ? last : sa[e / TN];
-#pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    acc[e / TN][e % TN][x] = fmaf(part[(p + 1) % (PART + 1)][x], s, acc[e / TN][e % TN][x]);
+                product(i, j, fa[i % R]);
                 if (i == TM - 1) fb[j] = frag(b_of(t + 1), j);
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -264,7 +360,7 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_blocks_tiles(BlockArgs g, uin
         }
         last = sa[TM - 1];
     }
-
+    }
     // The products still to be added.
 #pragma unroll
     for (int e = TM * TN - PART; e < TM * TN; ++e)
