@@ -153,40 +153,28 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_blocks_tiles(BlockArgs g, uin
     const __amdgpu_buffer_rsrc_t rsa = rsrc(g.sa + (size_t)m0 * KB, (size_t)rows_a * KB * 4);
     const __amdgpu_buffer_rsrc_t rsb = rsrc(g.sb + (size_t)nb0 * KB, (size_t)nbs * KB * 4);
     // A copy brings 8 rows: lane l the chunk of row l / 8 that lands in slot l % 8. The whole
-    // offset is the lane's (the scalar one would not count in the range check).
-    auto chunk_at = [&](uint32_t r) { return 16 * ((lane % 8) ^ pipe::swz<8>((r + lane / 8) & 31)); };
-    uint32_t va[T::LA], vb[T::LB];
-#pragma unroll
-    for (int c = 0; c < T::LA; ++c) va[c] = ((wave * T::LA + c) * 8 + lane / 8) * g.K;
-#pragma unroll
-    for (int c = 0; c < T::LB; ++c) vb[c] = ((wave * T::LB + c) * 8 + lane / 8) * g.K;
-    // Straight-line code, like all of the loop below: products wait in registers for their
-    // addition, and the compiler would move the additions behind a branch.
-    const uint32_t none = 0x7fffffffu;   // past every resource
-    auto issue_a = [&](uint32_t step) __attribute__((always_inline)) {
-        uint8_t *base = lds + (step % S) * T::STAGE;
+    // offset is the lane's (a scalar one would not count in the range check).
+    auto copy_rows = [&](const __amdgpu_buffer_rsrc_t &rs, uint8_t *to, uint32_t r, uint32_t step) __attribute__((always_inline)) {
         step = min(step, KB - 1);   // past the last stage: that one again, into a slot that is not read
         const uint32_t ko = step * KBLK, left = g.K - ko;   // codes of k left
-#pragma unroll
-        for (int c = 0; c < T::LA; ++c) {
-            const uint32_t r = (wave * T::LA + c) * 8, ch = chunk_at(r);
-            pipe::copy16_buf_asm(ra, base + r * 128, ch < left ? va[c] + (ko + ch) : none);
-        }
+        const uint32_t ch = 16 * ((lane % 8) ^ pipe::swz<8>((r + lane / 8) & 31));
+        pipe::copy16_buf_asm(rs, to + r * 128, ch < left ? lane / 8 * g.K + ch + (r * g.K + ko) : 0x7fffffffu);
     };
-    auto issue_b = [&](uint32_t step, int from, int to) __attribute__((always_inline)) {
-        uint8_t *base = lds + (step % S) * T::STAGE + T::A_BYTES;
-        step = min(step, KB - 1);
-        const uint32_t ko = step * KBLK, left = g.K - ko;
+    // N copies of a, or of b, from row 8 first on.
+    auto issue_a = [&](uint32_t step, uint32_t first, auto n_c) __attribute__((always_inline)) {
 #pragma unroll
-        for (int c = 0; c < T::LB; ++c) {
-            if (c < from || c >= to) continue;
-            const uint32_t r = (wave * T::LB + c) * 8, ch = chunk_at(r);
-            pipe::copy16_buf_asm(rb, base + r * 128, ch < left ? vb[c] + (ko + ch) : none);
-        }
+        for (int c = 0; c < decltype(n_c)::value; ++c) copy_rows(ra, lds + step % S * T::STAGE, (first + c) * 8, step);
     };
-    auto issue = [&](uint32_t step) __attribute__((always_inline)) {
-        issue_a(step);
-        issue_b(step, 0, T::LB);
+    auto issue_b = [&](uint32_t step, uint32_t first, auto n_c) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < decltype(n_c)::value; ++c)
+            copy_rows(rb, lds + step % S * T::STAGE + T::A_BYTES, (first + c) * 8, step);
+    };
+    const std::integral_constant<int, T::LA> la{};
+    const std::integral_constant<int, T::LB> lb{};
+    auto issue = [&](uint32_t step) __attribute__((always_inline)) {   // a wave's share of a stage
+        issue_a(step, wave * T::LA, la);
+        issue_b(step, wave * T::LB, lb);
     };
     // The scales of stages G grp .. G grp + 3: 64 rows of a a copy, then the blocks of b.
     // (Those behind a row's last are the next row's and are not used.)
@@ -254,9 +242,9 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_blocks_tiles(BlockArgs g, uin
         // of its next one, which together take as long. A phase ends at a barrier; the second
         // half runs one behind. The first half's products of stage t are phase 2 t, its turnover
         // 2 t + 1, the second's 2 t + 1 and 2 t + 2. Both halves have stage t's weight fragments
-        // in registers by the end of phase 2 t, so its slot takes the weight codes of stage t + 2
-        // in phase 2 t + 1 (a share of each half), the first half's rows in 2 t + 1, the second's
-        // in 2 t + 2; each has landed two phases later.
+        // in registers by the end of phase 2 t, so in phase 2 t + 1 the first half puts its rows
+        // and the weight codes of stage t + 2 into the slot, in phase 2 t + 2 the second its rows;
+        // each has landed before its next products' phase ends.
         auto turnover = [&](uint32_t t) __attribute__((always_inline)) {
             last = sa[TM - 1];
             fa[0] = frag(a_of(t), 0);
@@ -270,12 +258,10 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_blocks_tiles(BlockArgs g, uin
             pipe::lds_barrier();
             __builtin_amdgcn_sched_barrier(0);
         };
-        auto products = [&](uint32_t t, auto copy_c) __attribute__((always_inline)) {
-            constexpr bool COPY = decltype(copy_c)::value;
+        auto products = [&](uint32_t t) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < TM; ++i) {
                 if (i + 2 < TM) fa[(i + 2) % R] = frag(a_of(t), i + 2);
-                if (COPY && i < T::LB) issue_b(t + 2, i, i + 1);
 #pragma unroll
                 for (int j = 0; j < TN; ++j) {
                     product(i, j, fa[i % R]);
@@ -295,11 +281,12 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_blocks_tiles(BlockArgs g, uin
             turnover(0);
             barrier();
             for (uint32_t t = 0; t < KB; ++t) {
-                products(t, std::false_type{});
+                products(t);
                 pipe::wait_vmcnt<0>();
                 barrier();
                 if (t % T::G == 0 && t + T::G < KB) issue_scales(t / T::G + 1);
-                issue(t + 2);
+                issue_a(t + 2, wave * T::LA, la);
+                issue_b(t + 2, wave * 2 * T::LB, std::integral_constant<int, 2 * T::LB>{});
                 turnover(t + 1);
                 barrier();
             }
@@ -309,13 +296,12 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_blocks_tiles(BlockArgs g, uin
             turnover(0);
             barrier();
             for (uint32_t t = 0; t < KB; ++t) {
-                products(t, std::true_type{});
-                pipe::wait_vmcnt<T::LB>();
+                products(t);
+                pipe::wait_vmcnt<0>();
                 barrier();
                 if (t % T::G == 0 && t + T::G < KB) issue_scales(t / T::G + 1);
-                issue_a(t + 2);
+                issue_a(t + 2, wave * T::LA, la);
                 turnover(t + 1);
-                pipe::wait_vmcnt<T::LA>();
                 barrier();
             }
         }
