@@ -160,15 +160,6 @@ def _opt(t, what, nbytes=None):
     return None if t is None else _dev(t, what, nbytes)
 
 
-def _same_device(**tensors):
-    """Refuse tensors that are not on the device whose current stream the call runs on."""
-    import torch
-
-    for what, t in tensors.items():
-        if t is not None and t.device.type == "cuda" and t.device.index != torch.cuda.current_device():
-            raise ValueError(f"{what} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
-
-
 def _span(rows, cols, ld):
     """Elements a [rows, cols] window of row pitch ld spans."""
     return 0 if rows == 0 or cols == 0 else (rows - 1) * ld + cols
@@ -380,59 +371,87 @@ def gemm_fp8_scaled(a, a_fmt, scale_a, b, b_fmt, scale_b, M, N, K, out=None):
 
 SCALE_BLOCK = 128
 
+# What these calls ask of torch on every call, looked up once: the module, its types by what a
+# call accepts, whether tensors can be on another device than the current one, and the current
+# stream's handle (torch.cuda.current_stream() builds an object around it, 2.8 us of a call's 13).
+_T = None
+
+
+class _Torch:
+    def __init__(self):
+        import torch
+
+        self.empty, self.u8, self.f32, self.bf16 = torch.empty, torch.uint8, torch.float32, torch.bfloat16
+        self.is16 = frozenset((torch.bfloat16, torch.int16, torch.uint16))
+        self.is32 = frozenset((torch.int32, torch.uint32))
+        self.several = torch.cuda.device_count() > 1
+        self.current_device = torch.cuda.current_device
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        self.raw_stream = raw or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+    def stream(self):
+        return self.raw_stream(self.current_device())
+
+
+def _torch():
+    global _T
+    if _T is None:
+        _T = _Torch()
+    return _T
+
 
 def _nblocks(n, of=SCALE_BLOCK):
     return -(-n // of)
 
 
+def _at(t, what, n, size):
+    """The device address of a contiguous tensor of at least n elements of `size` bytes on the
+    current device (whose current stream the call runs on)."""
+    if not (t.is_cuda and t.is_contiguous() and t.numel() * t.element_size() >= n * size):
+        return _dev(t, what, n * size).value   # raises
+    if _T.several and t.get_device() != _T.current_device():
+        raise ValueError(f"{what} is on cuda:{t.get_device()}, the current device is cuda:{_T.current_device()}")
+    return t.data_ptr()
+
+
 def _f32(t, what, n):
-    import torch
-
-    if t.dtype != torch.float32:
+    if t.dtype != _T.f32:
         raise ValueError(f"{what} must be f32, not {t.dtype}")
-    return _dev(t, what, 4 * n)
-
-
-def _f32_opt(t, what, n):
-    return None if t is None else _f32(t, what, n)
+    return _at(t, what, n, 4)
 
 
 def _16bit(t, what, n):
-    import torch
-
-    if t.dtype not in (torch.bfloat16, torch.int16, torch.uint16):
+    if t.dtype not in _T.is16:
         raise ValueError(f"{what} must be bf16 (or its bits as int16/uint16), not {t.dtype}")
-    return _dev(t, what, 2 * n)
+    return _at(t, what, n, 2)
 
 
 def _8bit(t, what, n):
     if t.element_size() != 1:
         raise ValueError(f"{what} must hold one code per byte, not {t.dtype}")
-    return _dev(t, what, n)
+    return _at(t, what, n, 1)
 
 
 def quantize_blocks_into(w, rows, cols, fmt, block_rows, backoff, codes, scales, ld=None):
     """quantize_blocks into caller-owned tensors (no allocation)."""
+    T = _torch()
     ld = cols if ld is None else ld
-    dt = _dtype_code(w)
-    _same_device(w=w, codes=codes, scales=scales)
     if block_rows not in (1, SCALE_BLOCK):
         raise ValueError(f"blocks of {block_rows} rows; expected 1 or {SCALE_BLOCK}")
-    _check(lib().reng_hip_quantize_blocks(_dev(w, "weight", _span(rows, cols, ld) * (2 if dt == BF16 else 4)), dt, rows,
-                                          cols, ld, _fmt(fmt), block_rows, float(backoff),
-                                          _8bit(codes, "codes", rows * cols),
+    dt = _dtype_code(w)
+    _check(lib().reng_hip_quantize_blocks(_at(w, "weight", _span(rows, cols, ld), 2 if dt == BF16 else 4), dt, rows, cols,
+                                          ld, _fmt(fmt), block_rows, backoff, _8bit(codes, "codes", rows * cols),
                                           _f32(scales, "scales", _nblocks(rows, block_rows) * _nblocks(cols)),
-                                          _stream()))
+                                          T.stream()))
 
 
 def quantize_blocks(w, rows, cols, fmt, block_rows=SCALE_BLOCK, backoff=DEFAULT_BACKOFF, ld=None):
     """(codes [rows * cols], scales [blocks]) of a device tensor of bf16 (or its
     int16 bits) or f32, [rows, ld] row-major: one scale per block of block_rows x
     128 values, block_rows 128 for weights or 1 for activation rows."""
-    import torch
-
-    codes = torch.empty(rows * cols, dtype=torch.uint8, device=w.device)
-    scales = torch.empty(_nblocks(rows, max(1, block_rows)) * _nblocks(cols), dtype=torch.float32, device=w.device)
+    T, dev = _torch(), w.device
+    codes = T.empty(rows * cols, dtype=T.u8, device=dev)
+    scales = T.empty(_nblocks(rows, max(1, block_rows)) * _nblocks(cols), dtype=T.f32, device=dev)
     quantize_blocks_into(w, rows, cols, fmt, block_rows, backoff, codes, scales, ld)
     return codes, scales
 
@@ -440,33 +459,27 @@ def quantize_blocks(w, rows, cols, fmt, block_rows=SCALE_BLOCK, backoff=DEFAULT_
 def gemm_fp8_blocks(a, a_fmt, scale_a, b, b_fmt, scale_b, M, N, K, out=None):
     """bf16 out[M, N] of codes a [M, K] with scale_a [M, ceil(K / 128)] and codes
     b [N, K] with scale_b [ceil(N / 128), ceil(K / 128)]."""
-    import torch
-
+    T = _torch()
     if out is None:
-        out = torch.empty(M * N, dtype=torch.bfloat16, device=a.device)
-    _same_device(a=a, scale_a=scale_a, b=b, scale_b=scale_b, out=out)
+        out = T.empty(M * N, dtype=T.bf16, device=a.device)
     kb = _nblocks(K)
     _check(lib().reng_hip_gemm_fp8_blocks(_8bit(a, "a", M * K), _fmt(a_fmt), _f32(scale_a, "scale_a", M * kb),
                                           _8bit(b, "b", N * K), _fmt(b_fmt), _f32(scale_b, "scale_b", _nblocks(N) * kb),
-                                          M, N, K, _16bit(out, "out", M * N), _stream()))
+                                          M, N, K, _16bit(out, "out", M * N), T.stream()))
     return out
 
 
-def _residual_norm_args(x, d, gamma, rows, cols, post_gamma, gate, residual_scale, h):
-    """The arguments both output forms share, and h (allocated where a branch needs it)."""
-    import torch
-
+def _residual_norm_args(T, x, d, gamma, rows, cols, post_gamma, gate, residual_scale, h):
+    """The arguments both output forms share, h (allocated where a branch needs it) and its address."""
     n = rows * cols
     if h is None and d is not None:
-        h = torch.empty(n, dtype=torch.float32, device=x.device)
-    _same_device(x=x, d=d, gamma=gamma, post_gamma=post_gamma, gate=gate, h=h)
-    gate_ld = 0
-    if gate is not None and gate.numel() != cols:
-        gate_ld = cols
-    args = [_f32(x, "x", n), None if d is None else _16bit(d, "d", n), _f32_opt(post_gamma, "post_gamma", cols),
-            None if gate is None else _16bit(gate, "gate", rows * cols if gate_ld else cols), gate_ld,
-            float(residual_scale), _f32(gamma, "gamma", cols), rows, cols]
-    return args, h, _f32_opt(h, "h", n)
+        h = T.empty(n, dtype=T.f32, device=x.device)
+    gate_ld = 0 if gate is None or gate.numel() == cols else cols
+    args = (_f32(x, "x", n), None if d is None else _16bit(d, "d", n),
+            None if post_gamma is None else _f32(post_gamma, "post_gamma", cols),
+            None if gate is None else _16bit(gate, "gate", n if gate_ld else cols), gate_ld, residual_scale,
+            _f32(gamma, "gamma", cols), rows, cols)
+    return args, h, None if h is None else _f32(h, "h", n)
 
 
 def residual_norm_bf16(x, d, gamma, rows, cols, eps, post_gamma=None, gate=None, residual_scale=1.0, h=None, out=None):
@@ -474,13 +487,11 @@ def residual_norm_bf16(x, d, gamma, rows, cols, eps, post_gamma=None, gate=None,
     post-norm where post_gamma is given, the gate of [cols] or [rows, cols] bf16
     values where it is) and bf16 out = rms_norm(h) * gamma. h may be x. With d None
     there is no branch: h = x, returned as given."""
-    import torch
-
+    T = _torch()
     if out is None:
-        out = torch.empty(rows * cols, dtype=torch.bfloat16, device=x.device)
-    args, h, hp = _residual_norm_args(x, d, gamma, rows, cols, post_gamma, gate, residual_scale, h)
-    _same_device(out=out)
-    _check(lib().reng_hip_residual_norm_bf16(*args, eps, hp, _16bit(out, "out", rows * cols), _stream()))
+        out = T.empty(rows * cols, dtype=T.bf16, device=x.device)
+    args, h, hp = _residual_norm_args(T, x, d, gamma, rows, cols, post_gamma, gate, residual_scale, h)
+    _check(lib().reng_hip_residual_norm_bf16(*args, eps, hp, _16bit(out, "out", rows * cols), T.stream()))
     return h, out
 
 
@@ -488,17 +499,15 @@ def residual_norm_fp8(x, d, gamma, rows, cols, eps, fmt, post_gamma=None, gate=N
                       backoff=DEFAULT_BACKOFF, h=None, codes=None, scales=None):
     """(h, codes, scales): residual_norm_bf16 with the normalised rows as fp8 codes
     and one scale per 128 columns, gemm_fp8_blocks' a operand."""
-    import torch
-
+    T = _torch()
+    kb = _nblocks(cols)
     if codes is None:
-        codes = torch.empty(rows * cols, dtype=torch.uint8, device=x.device)
+        codes = T.empty(rows * cols, dtype=T.u8, device=x.device)
     if scales is None:
-        scales = torch.empty(rows * _nblocks(cols), dtype=torch.float32, device=x.device)
-    args, h, hp = _residual_norm_args(x, d, gamma, rows, cols, post_gamma, gate, residual_scale, h)
-    _same_device(codes=codes, scales=scales)
-    _check(lib().reng_hip_residual_norm_fp8(*args, eps, _fmt(fmt), float(backoff), hp,
-                                            _8bit(codes, "codes", rows * cols),
-                                            _f32(scales, "scales", rows * _nblocks(cols)), _stream()))
+        scales = T.empty(rows * kb, dtype=T.f32, device=x.device)
+    args, h, hp = _residual_norm_args(T, x, d, gamma, rows, cols, post_gamma, gate, residual_scale, h)
+    _check(lib().reng_hip_residual_norm_fp8(*args, eps, _fmt(fmt), backoff, hp, _8bit(codes, "codes", rows * cols),
+                                            _f32(scales, "scales", rows * kb), T.stream()))
     return h, codes, scales
 
 
@@ -514,22 +523,21 @@ def attention_tree(q, k_cache, v_cache, n_heads, n_kv_heads, head_dim, length, t
     whose bit is set in mask (int32 or uint32 words [tokens, ceil(tokens / 32)]; None:
     a chain, token i sees drafted rows 0 .. i). workspace: a device tensor of at least
     attention_tree_workspace_bytes(...) bytes (allocated here when None)."""
-    import torch
-
+    T = _torch()
     if out is None:
-        out = torch.empty(tokens * n_heads * head_dim, dtype=torch.bfloat16, device=q.device)
+        out = T.empty(tokens * n_heads * head_dim, dtype=T.bf16, device=q.device)
     if workspace is None:
-        n = attention_tree_workspace_bytes(n_heads, n_kv_heads, head_dim, length, tokens)
-        workspace = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-    _same_device(q=q, k_cache=k_cache, v_cache=v_cache, mask=mask, workspace=workspace, out=out)
+        wb = attention_tree_workspace_bytes(n_heads, n_kv_heads, head_dim, length, tokens)
+        workspace = T.empty(wb, dtype=T.u8, device=q.device) if wb else None
+    else:
+        wb = workspace.numel() * workspace.element_size()
     nq, nc = tokens * n_heads * head_dim, (length + tokens) * n_kv_heads * head_dim
-    if mask is not None and mask.element_size() != 4:
+    if mask is not None and mask.dtype not in T.is32:
         raise ValueError(f"mask must hold 32-bit words, not {mask.dtype}")
     _check(lib().reng_hip_attention_tree(
         _16bit(q, "q", nq), _16bit(k_cache, "k_cache", nc), _16bit(v_cache, "v_cache", nc), n_heads, n_kv_heads,
-        head_dim, length, tokens, _opt(mask, "mask", 4 * tokens * _nblocks(tokens, 32)), scale,
-        _opt(workspace, "workspace"), 0 if workspace is None else workspace.numel() * workspace.element_size(),
-        _16bit(out, "out", nq), _stream()))
+        head_dim, length, tokens, None if mask is None else _at(mask, "mask", tokens * _nblocks(tokens, 32), 4), scale,
+        None if workspace is None else _at(workspace, "workspace", 0, 1), wb, _16bit(out, "out", nq), T.stream()))
     return out
 
 
