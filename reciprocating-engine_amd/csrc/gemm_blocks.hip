@@ -8,6 +8,7 @@
 // block beside 128 multiply-adds on the matrix cores.
 #include <type_traits>
 
+#include "block_forms.h"
 #include "common.h"
 #include "mfma_pipe.h"
 #include "tile_order.h"
@@ -35,67 +36,137 @@ __device__ __forceinline__ i32x8 join(const u32x4 &x, const u32x4 &y) {
     return i32x8{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
 }
 
-// A workgroup computes 16 MT rows of a by 16 rows of b; its waves take the
-// blocks of k in turn and their sums meet in LDS. v_mfma_f32_16x16x128 with the
-// weight as the first operand: lane l holds row l % 16 of either operand, and of
-// the 128 codes the chunks of 16 at 16 (l / 16) and 64 + 16 (l / 16) (the same
-// places for both, so the order of k within the block is free); the result's lane
-// has activation row l % 16 and the four weight rows from 4 (l / 16).
-template <int FA, int FB, int MT, int W>
-__global__ __launch_bounds__(64 * W) void gemm_blocks_rows(BlockArgs g, uint32_t tiles_m, uint64_t tiles) {
-    __shared__ f32x4 part[W][MT][64];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, q = lane >> 4;
+// ------------------------------------------------------------ few rows
+//
+// Up to 64 activation rows: the weight's bytes are the time. A workgroup computes 16 MT
+// rows of a by 16 NT rows of b; its KW waves split the blocks of k evenly and their sums
+// meet in LDS, in the waves' order. A wave copies its own stages (one scale block of its
+// rows) through a ring of its own, S - 1 of them in flight, and waits for nobody until
+// the end. The copies are 8 rows x 128 bytes an instruction: read straight into
+// registers in the matrix operand's layout the codes come in 64-byte pieces. Scales are
+// copied four stages at a time.
+// v_mfma_f32_16x16x128 with the weight as the first operand: lane l holds row l % 16 of
+// either operand and the chunks 2 (l / 16) and 2 (l / 16) + 1 of its 128 codes; the
+// result's lane has activation row l % 16 and the four weight rows from 4 (l / 16).
+template <int MT, int NT, int S>
+struct RingShape {
+    static constexpr int ROWS = 16 * (MT + NT), STAGE = ROWS * 128, COPIES = ROWS / 8, G = 4;
+    static constexpr int SC = 2 * 1024;   // a group's scales: 64 activation rows', then the weight block's
+    static constexpr int WAVE = S * STAGE + 2 * SC;
+    static_assert(MT * NT * 1024 <= WAVE && (S - 1) * COPIES + 2 < 64 && 16 * NT <= 128, "the sums fit the ring; vmcnt range");
+};
+
+template <int FA, int FB, int MT, int NT, int KW, int S>
+__global__ __launch_bounds__(64 * KW) void gemm_blocks_ring(BlockArgs g, uint32_t tiles_m) {
+    using T = RingShape<MT, NT, S>;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    const uint32_t lane = threadIdx.x & 63, row = lane & 15, q = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t m0 = blockIdx.x % tiles_m * (16 * MT), n0 = blockIdx.x / tiles_m * (16 * NT);
     const uint32_t KB = (g.K + KBLK - 1) / KBLK;
-    for (uint64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-        const uint32_t m0 = (uint32_t)(t % tiles_m) * (16 * MT), n0 = (uint32_t)(t / tiles_m) * 16;
-        // Rows past the edges are clamped and not stored.
-        const uint8_t *pb = g.b + (size_t)min(n0 + row, g.N - 1) * g.K + 16 * q;
-        const float *ps = g.sb + (size_t)(n0 / KBLK) * KB;
-        const uint8_t *pa[MT];
-        const float *psa[MT];
-        f32x4 acc[MT];
+    const uint32_t k0 = wave * KB / KW, n = (wave + 1) * KB / KW - k0;   // this wave's blocks
+    auto rsrc = [](const void *p, size_t bytes) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, (uint32_t)bytes, 0x00020000);
+    };
+    // Rows past M and N and codes past K lie outside and arrive as zeros.
+    const uint32_t rows_a = min((uint32_t)(16 * MT), g.M - m0), rows_b = min((uint32_t)(16 * NT), g.N - n0);
+    const __amdgpu_buffer_rsrc_t ra = rsrc(g.a + (size_t)m0 * g.K, (size_t)rows_a * g.K);
+    const __amdgpu_buffer_rsrc_t rb = rsrc(g.b + (size_t)n0 * g.K, (size_t)rows_b * g.K);
+    const __amdgpu_buffer_rsrc_t rsa = rsrc(g.sa + (size_t)m0 * KB, (size_t)rows_a * KB * 4);
+    const __amdgpu_buffer_rsrc_t rsb = rsrc(g.sb + (size_t)(n0 / KBLK) * KB, (size_t)KB * 4);
+    const uint32_t none = 0x7fffffffu;
+    uint8_t *ring = lds + wave * T::WAVE;
+    auto issue = [&](uint32_t i) __attribute__((always_inline)) {   // stage i of this wave; past the last, nothing
+        uint8_t *to = ring + i % S * T::STAGE;
+        const uint32_t ko = (k0 + i) * KBLK, left = i < n ? g.K - ko : 0;
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            const size_t m = min(m0 + 16 * i + row, g.M - 1);
-            pa[i] = g.a + m * g.K + 16 * q;
-            psa[i] = g.sa + m * KB;
-            acc[i] = f32x4{0, 0, 0, 0};
+        for (int c = 0; c < T::COPIES; ++c) {
+            const bool of_b = c >= 2 * MT;
+            const uint32_t r = (of_b ? c - 2 * MT : c) * 8 + lane / 8;
+            const uint32_t ch = 16 * ((lane % 8) ^ pipe::swz<8>((c * 8 + lane / 8) & 31));
+            pipe::copy16_buf_asm(of_b ? rb : ra, to + c * 1024, ch < left ? r * g.K + (ko + ch) : none);
         }
-        for (uint32_t kb = wave; kb < KB; kb += W) {
-            const uint32_t k = kb * KBLK + 16 * q;
-            const bool lo = k < g.K, hi = k + 64 < g.K;   // K is a multiple of 16
-            const size_t ko = (size_t)kb * KBLK;
-            const u32x4 z{0, 0, 0, 0};
-            const i32x8 fb = join(lo ? *reinterpret_cast<const u32x4 *>(pb + ko) : z,
-                                  hi ? *reinterpret_cast<const u32x4 *>(pb + ko + 64) : z);
-            const float s = ps[kb];
+    };
+    auto issue_scales = [&](uint32_t grp) __attribute__((always_inline)) {
+        uint8_t *to = ring + S * T::STAGE + (grp & 1) * T::SC;
+        const uint32_t k = (k0 + grp * T::G) * 4;
+        pipe::copy16_buf_asm(rsa, to, lane * KB * 4 + k);
+        pipe::copy16_buf_asm(rsb, to + 1024, lane == 0 ? k : none);
+    };
+    auto frag = [&](const uint8_t *p, int tile) __attribute__((always_inline)) {
+        const uint32_t r = 16 * tile + row, w = pipe::swz<8>(r & 31);
+        p += r * 128;
+        return join(*reinterpret_cast<const u32x4 *>(p + (2 * q ^ w) * 16),
+                    *reinterpret_cast<const u32x4 *>(p + ((2 * q + 1) ^ w) * 16));
+    };
+    f32x4 acc[MT][NT];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const i32x8 fa = join(lo ? *reinterpret_cast<const u32x4 *>(pa[i] + ko) : z,
-                                      hi ? *reinterpret_cast<const u32x4 *>(pa[i] + ko + 64) : z);
-                const f32x4 d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb, fa, f32x4{0, 0, 0, 0}, FB, FA, 0,
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+    issue_scales(0);
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) issue(i);
+    for (uint32_t i = 0; i < n; ++i) {
+        // The slot of stage i + S - 1 was read by the stage before: those reads are done.
+        pipe::wait_lgkm0();
+        issue(i + S - 1);
+        if (i % T::G == 0) issue_scales(i / T::G + 1);
+        pipe::wait_vmcnt<(S - 1) * T::COPIES>();
+        asm volatile("" ::: "memory");
+        const uint8_t *st = ring + i % S * T::STAGE;
+        const uint8_t *sc = ring + S * T::STAGE + (i / T::G & 1) * T::SC + i % T::G * 4;
+        const float sb = *reinterpret_cast<const float *>(sc + 1024);
+        i32x8 fb[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) fb[j] = frag(st, MT + j);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const i32x8 fa = frag(st, m);
+            const float s = *reinterpret_cast<const float *>(sc + 16 * (16 * m + row)) * sb;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const f32x4 d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa, f32x4{0, 0, 0, 0}, FB, FA, 0,
                                                                                 0, 0, 0);
-                const float sc = psa[i][kb] * s;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][e] = fmaf(d[e], sc, acc[i][e]);
+                for (int e = 0; e < 4; ++e) acc[m][j][e] = fmaf(d[e], s, acc[m][j][e]);
             }
         }
-#pragma unroll
-        for (int i = 0; i < MT; ++i) part[wave][i][lane] = acc[i];
-        __syncthreads();
-        for (uint32_t i = wave; i < MT; i += W) {
-            f32x4 v = part[0][i][lane];
-#pragma unroll
-            for (int w = 1; w < W; ++w) v += part[w][i][lane];
-            const uint32_t m = m0 + 16 * i + row;
-            if (m < g.M)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (n0 + 4 * q + e < g.N)
-                        g.out[(size_t)m * g.N + n0 + 4 * q + e] = (uint16_t)f32_to_bf16_bits(v[e]);
-        }
-        __syncthreads();   // part is written again for the next tile
     }
+    pipe::wait_vmcnt<0>();
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) *reinterpret_cast<f32x4 *>(ring + (m * NT + j) * 1024 + lane * 16) = acc[m][j];
+    __syncthreads();
+    const bool vec = g.N % 4 == 0 && reinterpret_cast<uintptr_t>(g.out) % 8 == 0;
+    for (uint32_t t = wave; t < MT * NT; t += KW) {
+        f32x4 v = *reinterpret_cast<const f32x4 *>(lds + t * 1024 + lane * 16);
+#pragma unroll
+        for (int w = 1; w < KW; ++w) v += *reinterpret_cast<const f32x4 *>(lds + w * T::WAVE + t * 1024 + lane * 16);
+        const uint32_t m = m0 + 16 * (t / NT) + row, nn = n0 + 16 * (t % NT) + 4 * q;
+        if (m >= g.M || nn >= g.N) continue;
+        uint16_t *out = g.out + (size_t)m * g.N + nn;
+        if (vec) {
+            *reinterpret_cast<u32x2 *>(out) = u32x2{f32_to_bf16_bits(v.x) | (f32_to_bf16_bits(v.y) << 16),
+                                                    f32_to_bf16_bits(v.z) | (f32_to_bf16_bits(v.w) << 16)};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (nn + e < g.N) out[e] = (uint16_t)f32_to_bf16_bits(v[e]);
+        }
+    }
+}
+
+template <int FA, int FB, int MT, int NT, int KW, int S>
+int launch_ring(const BlockArgs &g, hipStream_t st) {
+    constexpr int LDS = KW * RingShape<MT, NT, S>::WAVE;
+    static_assert(LDS <= 160 * 1024, "LDS");
+    const uint32_t tiles_m = (g.M + 16 * MT - 1) / (16 * MT), tiles_n = (g.N + 16 * NT - 1) / (16 * NT);
+    RENG_REQUIRE((uint64_t)tiles_m * tiles_n * (64 * KW) < (1ull << 32), "%u x %u outputs are too many for a launch", g.M, g.N);
+    hipLaunchKernelGGL((gemm_blocks_ring<FA, FB, MT, NT, KW, S>), dim3(tiles_m * tiles_n), dim3(64 * KW), LDS, st, g,
+                       tiles_m);
+    return check_launch("gemm_blocks_ring");
 }
 
 // ------------------------------------------------------------ output tiles
@@ -391,39 +462,34 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_blocks_tiles(BlockArgs g, uin
 template <int FA, int FB, typename T>
 int launch_tiles(const BlockArgs &g, hipStream_t st) {
     const uint32_t tiles_m = (g.M + T::BM - 1) / T::BM, tiles_n = (g.N + T::BN - 1) / T::BN, tiles = tiles_m * tiles_n;
+    RENG_REQUIRE((uint64_t)tiles_m * tiles_n * (64 * T::NW) < (1ull << 32), "%u x %u outputs are too many for a launch", g.M,
+                 g.N);
     hipLaunchKernelGGL((gemm_blocks_tiles<FA, FB, T>), dim3(tiles), dim3(64 * T::NW), T::LDS, st, g, tiles_m, tiles,
                        wide_mapm(tiles_m, tiles_n, T::BM, T::BN));
     return check_launch("gemm_blocks_tiles");
 }
 
 using Tile256 = BlockTile<8, 4, 2, 4, 2>;
-using Tile256x128 = BlockTile<4, 4, 4, 2, 3>;
-using Tile192 = BlockTile<6, 4, 2, 4, 2>;
 using Tile128 = BlockTile<4, 4, 2, 2, 2>;
 using Tile64 = BlockTile<2, 4, 2, 1, 3>;
+static_assert(Tile256::BM == 256 && Tile256::BN == 256 && Tile128::BM == 128 && Tile128::BN == 128 &&
+                  Tile64::BM == 64 && Tile64::BN == 64,
+              "BLOCK_COST's tiles");
 
 template <int FA, int FB>
 int launch_blocks(const BlockArgs &g, hipStream_t st) {
-    if (g.M > 64) {
-        const uint64_t cus = (uint64_t)device_props().cus;
-        auto tiles = [&](uint64_t b) { return ((g.M + b - 1) / b) * ((g.N + b - 1) / b); };
-        if (tiles(256) >= cus) return launch_tiles<FA, FB, Tile256>(g, st);
-        if (tiles(128) >= cus) return launch_tiles<FA, FB, Tile128>(g, st);
-        return launch_tiles<FA, FB, Tile64>(g, st);
+    switch (block_pick(g.M, g.N, g.K, (uint64_t)device_props().cus)) {
+    case BLK_RING_1x1: return launch_ring<FA, FB, 1, 1, 4, 4>(g, st);
+    case BLK_RING_1x4: return launch_ring<FA, FB, 1, 4, 4, 2>(g, st);
+    case BLK_RING_2x1: return launch_ring<FA, FB, 2, 1, 4, 3>(g, st);
+    case BLK_RING_2x2: return launch_ring<FA, FB, 2, 2, 4, 2>(g, st);
+    case BLK_RING_4x1: return launch_ring<FA, FB, 4, 1, 4, 2>(g, st);
+    case BLK_RING_4x2: return launch_ring<FA, FB, 4, 2, 4, 2>(g, st);
+    case BLK_RING_4x4: return launch_ring<FA, FB, 4, 4, 4, 2>(g, st);
+    case BLK_TILE_64: return launch_tiles<FA, FB, Tile64>(g, st);
+    case BLK_TILE_128: return launch_tiles<FA, FB, Tile128>(g, st);
+    default: return launch_tiles<FA, FB, Tile256>(g, st);
     }
-    constexpr int W = 8;
-    const uint64_t tiles_n = (g.N + 15) / 16;
-    auto go = [&](auto mt_c) {
-        constexpr int MT = decltype(mt_c)::value;
-        const uint32_t tiles_m = (g.M + 16 * MT - 1) / (16 * MT);
-        const uint64_t tiles = tiles_n * tiles_m, most = 1u << 20;
-        hipLaunchKernelGGL((gemm_blocks_rows<FA, FB, MT, W>), dim3((unsigned)(tiles < most ? tiles : most)),
-                           dim3(64 * W), 0, st, g, tiles_m, tiles);
-    };
-    if (g.M <= 16) go(std::integral_constant<int, 1>{});
-    else if (g.M <= 32) go(std::integral_constant<int, 2>{});
-    else go(std::integral_constant<int, 4>{});
-    return check_launch("gemm_blocks_rows");
 }
 
 }  // namespace
@@ -439,7 +505,8 @@ RENG_HIP_API int reng_hip_gemm_fp8_blocks(const uint8_t *a, int a_format, const 
     RENG_REQUIRE(valid(a_format) && valid(b_format), "unknown fp8 format");
     RENG_REQUIRE(M > 0 && N > 0 && K > 0, "empty product %zu x %zu x %zu", M, N, K);
     RENG_REQUIRE(K % 16 == 0, "K = %zu is not a multiple of 16", K);
-    RENG_REQUIRE(M <= 0x7fffffff && N <= 0x7fffffff && K <= 0x7fffffff, "dimension too large");
+    // Offsets within a tile's 256 rows are 31 bits.
+    RENG_REQUIRE(M <= 0x7fffffff && N <= 0x7fffffff && K <= (1u << 22), "dimension too large");
     RENG_REQUIRE(a && b && scale_a && scale_b && out, "null pointer");
     RENG_REQUIRE(((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) == 0,
                  "a and b must be 16-byte aligned");

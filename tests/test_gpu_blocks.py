@@ -24,6 +24,8 @@ from helpers import bf16_bits
 
 torch = pytest.importorskip("torch")
 
+from test_block_forms import FORM_SHAPES  # noqa: E402
+
 FMTS = ["e4m3", "e5m2"]
 TORCH_FP8 = {"e4m3": torch.float8_e4m3fn, "e5m2": torch.float8_e5m2}
 
@@ -172,6 +174,14 @@ SHAPES = [(1, 1, 16), (1, 16, 128), (1, 129, 144), (1, 4096, 4096), (1, 577, 189
 @pytest.mark.parametrize("M,N,K", SHAPES)
 def test_gemm_fp8_blocks_against_float64(R, M, N, K):
     check_product(R, M, N, K, seed=M + N + K)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form,M,N,K", FORM_SHAPES)
+def test_gemm_fp8_blocks_every_form(R, form, M, N, K):
+    """Every form, at ragged sizes, block counts of 1 to 9 (scales go four blocks at a time) and a short last block."""
+    check_product(R, M, N, K, seed=M + N + K)
+    check_product(R, M, N, K, "e5m2", "e4m3", seed=1)
 
 
 @pytest.mark.gpu
