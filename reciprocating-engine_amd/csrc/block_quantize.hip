@@ -4,6 +4,8 @@
 //
 // Bound: HBM, rows * cols * (in_bytes + 1) + 4 * blocks. Every value is read
 // once and stays in registers between the absmax and the encode.
+#include <type_traits>
+
 #include "block_scale.h"
 
 namespace reng {
@@ -14,49 +16,56 @@ using namespace blk;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-// The EPV consecutive values a lane takes of a row: 16 bytes.
+// The EPV consecutive values a lane takes of a row: 16 bytes, held as they are read.
 template <typename InT>
 struct Lane;
 template <>
 struct Lane<uint16_t> {
     static constexpr int EPV = 8, LANES = BLOCK / EPV;
-    __device__ static float f(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
+    __device__ static void f(const u32x4 &v, float (&x)[EPV]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(v[i] << 16);
+            x[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+        }
+    }
 };
 template <>
 struct Lane<float> {
     static constexpr int EPV = 4, LANES = BLOCK / EPV;
-    __device__ static float f(float b) { return b; }
+    __device__ static void f(const u32x4 &v, float (&x)[EPV]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(v[i]);
+    }
 };
 
-// Columns c .. c + EPV - 1 of a row as f32, zeros past cols.
+// Columns c .. c + EPV - 1 of a row, zeros past cols.
 template <typename InT, bool VEC>
-__device__ __forceinline__ void load_values(const InT *row, size_t c, size_t cols, float (&x)[Lane<InT>::EPV]) {
-    constexpr int E = Lane<InT>::EPV;
+__device__ __forceinline__ u32x4 load_values(const InT *row, size_t c, size_t cols) {
+    u32x4 v{0u, 0u, 0u, 0u};
     if constexpr (VEC) {
-        u32x4 v{0u, 0u, 0u, 0u};
         if (c < cols) v = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(row + c));
-        if constexpr (sizeof(InT) == 2) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[2 * i] = __uint_as_float(v[i] << 16);
-                x[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(v[i]);
-        }
     } else {
 #pragma unroll
-        for (int i = 0; i < E; ++i) x[i] = c + i < cols ? Lane<InT>::f(row[c + i]) : 0.0f;
+        for (int i = 0; i < Lane<InT>::EPV; ++i)
+            if (c + i < cols) {
+                if constexpr (sizeof(InT) == 2) v[i / 2] |= (uint32_t)row[c + i] << (16 * (i % 2));
+                else v[i] = __float_as_uint(row[c + i]);
+            }
     }
+    return v;
 }
 
-template <int F, int E, bool VEC>
-__device__ __forceinline__ void store_codes(uint8_t *row, size_t c, size_t cols, const float (&x)[E],
-                                            const Encoder &enc) {
+// PLAIN: the scale is a fast one and no value is NaN.
+template <int F, int E, bool VEC, bool PLAIN>
+__device__ __forceinline__ void store_codes(uint8_t *row, size_t c, size_t cols, const u32x4 &v, const Encoder &enc) {
+    float x[E];
+    Lane<typename std::conditional<E == 8, uint16_t, float>::type>::f(v, x);
     uint32_t d[E / 4];
 #pragma unroll
-    for (int i = 0; i < E / 4; ++i) d[i] = enc.quad<F>(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+    for (int i = 0; i < E / 4; ++i)
+        d[i] = PLAIN ? enc.quad_fast<F>(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3])
+                     : enc.quad<F>(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
     if constexpr (VEC) {
         if (c >= cols) return;
         if constexpr (E == 8) *reinterpret_cast<u32x2 *>(row + c) = u32x2{d[0], d[1]};
@@ -68,14 +77,24 @@ __device__ __forceinline__ void store_codes(uint8_t *row, size_t c, size_t cols,
     }
 }
 
-template <int E>
-__device__ __forceinline__ uint32_t values_max(const float (&x)[E]) {
+// The largest magnitude's bits; NaN patterns sort above infinity's.
+template <typename InT>
+__device__ __forceinline__ uint32_t values_max(const u32x4 &v) {
+    float x[Lane<InT>::EPV];
+    Lane<InT>::f(v, x);
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        const uint32_t a = mag_no_nan(x[i]);
-        m = m > a ? m : a;
-    }
+    for (int i = 0; i < Lane<InT>::EPV; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+    return m;
+}
+// The same with NaN ignored.
+template <typename InT>
+__device__ __forceinline__ uint32_t values_max_no_nan(const u32x4 &v) {
+    float x[Lane<InT>::EPV];
+    Lane<InT>::f(v, x);
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < Lane<InT>::EPV; ++i) m = max(m, mag_no_nan(x[i]));
     return m;
 }
 
@@ -88,17 +107,28 @@ __global__ __launch_bounds__(256) void quantize_groups(const InT *__restrict__ w
     constexpr int E = Lane<InT>::EPV, L = Lane<InT>::LANES;
     const size_t total = rows * groups, step = (size_t)gridDim.x * (256 / L);
     const uint32_t gl = threadIdx.x % L;
+    // Row and group in the row, carried along.
+    const size_t first = (size_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+    size_t r = first / groups, k = first % groups;
+    const size_t step_r = step / groups, step_k = step % groups;
     // The bound is on the workgroup's first group, so that every lane of a wave takes
     // part in the lane exchange.
     for (size_t g0 = (size_t)blockIdx.x * (256 / L); g0 < total; g0 += step) {
         const size_t g = g0 + threadIdx.x / L;
         const bool on = g < total;
-        const size_t r = on ? g / groups : 0, c = on ? (g % groups) * BLOCK + gl * E : cols;
-        float x[E];
-        load_values<InT, VEC>(w + r * ld, c, cols, x);
-        const float s = scale_of(lanes_max<L>(values_max(x)), full);
-        store_codes<F, E, VEC>(codes + r * cols, c, cols, x, Encoder(s));
+        const size_t row = on ? r : 0, c = on ? k * BLOCK + gl * E : cols;
+        const u32x4 x = load_values<InT, VEC>(w + row * ld, c, cols);
+        uint32_t m = lanes_max<L>(values_max<InT>(x));
+        const bool nan = m > F32_INF;
+        if (__builtin_amdgcn_ballot_w64(nan)) m = lanes_max<L>(values_max_no_nan<InT>(x));
+        const float s = scale_of(m, full);
+        const Encoder enc(s);
+        if (__builtin_amdgcn_ballot_w64(nan || !enc.fast)) store_codes<F, E, VEC, false>(codes + row * cols, c, cols, x, enc);
+        else store_codes<F, E, VEC, true>(codes + row * cols, c, cols, x, enc);
         if (on && gl == 0) scales[g] = s;
+        r += step_r;
+        k += step_k;
+        if (k >= groups) k -= groups, ++r;
     }
 }
 
@@ -112,29 +142,50 @@ __global__ __launch_bounds__(256) void quantize_square(const InT *__restrict__ w
     __shared__ uint32_t red[4];
     for (size_t b = blockIdx.x; b < blocks; b += gridDim.x) {
         const size_t r0 = b / bcols * BLOCK + threadIdx.x / L, c = b % bcols * BLOCK + threadIdx.x % L * E;
-        float x[P][E];
+        u32x4 x[P];
         uint32_t m = 0;
 #pragma unroll
         for (int p = 0; p < P; ++p) {
             const size_t r = r0 + p * RP;
-            load_values<InT, VEC>(w + (r < rows ? r : 0) * ld, r < rows ? c : cols, cols, x[p]);
+            x[p] = load_values<InT, VEC>(w + (r < rows ? r : 0) * ld, r < rows ? c : cols, cols);
         }
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            const uint32_t a = values_max(x[p]);
+            const uint32_t a = values_max<InT>(x[p]);
             m = m > a ? m : a;
         }
-        m = lanes_max<64>(m);
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
-        __syncthreads();
-        m = max(max(red[0], red[1]), max(red[2], red[3]));
-        __syncthreads();   // red is written again for the next block
+        auto block_max = [&](uint32_t v) {
+            v = lanes_max<64>(v);
+            if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+            __syncthreads();
+            v = max(max(red[0], red[1]), max(red[2], red[3]));
+            __syncthreads();   // red is written again
+            return v;
+        };
+        m = block_max(m);
+        const bool nan = m > F32_INF;
+        if (nan) {
+            m = 0;
+#pragma unroll
+            for (int p = 0; p < P; ++p) m = max(m, values_max_no_nan<InT>(x[p]));
+            m = block_max(m);
+        }
         const float s = scale_of(m, full);
         const Encoder enc(s);
+        if (!nan && enc.fast) {
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-            const size_t r = r0 + p * RP;
-            if (r < rows) store_codes<F, E, VEC>(codes + r * cols, c, cols, x[p], enc);
+            for (int p = 0; p < P; ++p) {
+                const size_t r = r0 + p * RP;
+                if (r < rows) store_codes<F, E, VEC, true>(codes + r * cols, c, cols, x[p], enc);
+                __builtin_amdgcn_sched_barrier(0);   // or all of the quotients are held at once
+            }
+        } else {
+#pragma unroll 1
+            for (int p = 0; p < P; ++p) {
+                const size_t r = r0 + p * RP;
+                const u32x4 v = load_values<InT, VEC>(w + (r < rows ? r : 0) * ld, r < rows ? c : cols, cols);
+                if (r < rows) store_codes<F, E, VEC, false>(codes + r * cols, c, cols, v, enc);
+            }
         }
         if (threadIdx.x == 0) scales[b] = s;
     }

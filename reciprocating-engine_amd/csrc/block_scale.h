@@ -43,12 +43,16 @@ struct Encoder {
         : s(scale), r(0.0), fast(scale >= 1.17549435e-38f && scale < __builtin_inff()) {
         if (fast) r = 1.0 / (double)scale;
     }
+    // Of a fast scale and four values without a NaN.
+    template <int F>
+    __device__ __forceinline__ uint32_t quad_fast(float x0, float x1, float x2, float x3) const {
+        return cvt4<F, true>((float)((double)x0 * r), (float)((double)x1 * r), (float)((double)x2 * r),
+                             (float)((double)x3 * r));
+    }
     template <int F>
     __device__ __forceinline__ uint32_t quad(float x0, float x1, float x2, float x3) const {
         const bool nan = __builtin_isnan(x0) | __builtin_isnan(x1) | __builtin_isnan(x2) | __builtin_isnan(x3);
-        if (fast && !nan)
-            return cvt4<F, true>((float)((double)x0 * r), (float)((double)x1 * r), (float)((double)x2 * r),
-                                 (float)((double)x3 * r));
+        if (fast && !nan) return quad_fast<F>(x0, x1, x2, x3);
         return encode_div<F>(x0, s) | (encode_div<F>(x1, s) << 8) | (encode_div<F>(x2, s) << 16) |
                (encode_div<F>(x3, s) << 24);
     }

@@ -210,15 +210,13 @@ __global__ __launch_bounds__(1024) void residual_norm_any(NormArgs a) {
     }
 }
 
-template <int OUT, int NT>
-bool launch_vec(const NormArgs &a, unsigned rows, hipStream_t st) {
-    const uint32_t vpt = (a.cols + 4 * NT - 1) / (4 * NT);
-    if (vpt <= 1) hipLaunchKernelGGL((residual_norm_vec<OUT, NT, 1>), dim3(rows), dim3(NT), 0, st, a);
-    else if (vpt <= 2) hipLaunchKernelGGL((residual_norm_vec<OUT, NT, 2>), dim3(rows), dim3(NT), 0, st, a);
-    else if (vpt <= 4) hipLaunchKernelGGL((residual_norm_vec<OUT, NT, 4>), dim3(rows), dim3(NT), 0, st, a);
-    else if (vpt <= 8) hipLaunchKernelGGL((residual_norm_vec<OUT, NT, 8>), dim3(rows), dim3(NT), 0, st, a);
-    else return false;
-    return true;
+template <int OUT, int NT, int VPT>
+int launch_vpt(const NormArgs &a, unsigned rows, uint32_t vpt, hipStream_t st) {
+    if constexpr (VPT < 8) {
+        if (vpt > VPT) return launch_vpt<OUT, NT, VPT + 1>(a, rows, vpt, st);
+    }
+    hipLaunchKernelGGL((residual_norm_vec<OUT, NT, VPT>), dim3(rows), dim3(NT), 0, st, a);
+    return check_launch("residual_norm_vec");
 }
 
 template <int OUT>
@@ -229,9 +227,15 @@ int launch_norm(const NormArgs &a, size_t rows, hipStream_t st) {
     const bool vec = a.cols % 4 == 0 && a.gate_ld % 4 == 0 && f32s % 16 == 0 && bf16s % 8 == 0 &&
                      (OUT == OUT_BF16 || at(a.out) % 4 == 0);
     const unsigned grid = (unsigned)rows;
-    if (!(vec && (launch_vec<OUT, 256>(a, grid, st) || launch_vec<OUT, 1024>(a, grid, st))))
-        hipLaunchKernelGGL((residual_norm_any<OUT>), dim3(grid), dim3(1024), 0, st, a);
-    return check_launch("residual_norm");
+    auto vpt = [&](uint32_t nt) { return (a.cols + 4 * nt - 1) / (4 * nt); };
+    // Few rows wait for their own chain of loads and sums, which sixteen waves make shorter; many
+    // fill the chip with four each (5120 columns, fp8 out, 256 threads / 1024: 24 rows 7.7 / 4.9
+    // us, 512 rows 12.1 / 10.5, 1024 rows 19.9 / 20.4, 4096 rows 59 / 67).
+    const bool few = rows <= 2 * (size_t)device_props().cus && a.cols > 1024;
+    if (vec && vpt(256) <= 8 && !few) return launch_vpt<OUT, 256, 1>(a, grid, vpt(256), st);
+    if (vec && vpt(1024) <= 8) return launch_vpt<OUT, 1024, 1>(a, grid, vpt(1024), st);
+    hipLaunchKernelGGL((residual_norm_any<OUT>), dim3(grid), dim3(1024), 0, st, a);
+    return check_launch("residual_norm_any");
 }
 
 int norm_args(const NormArgs &a, size_t rows, size_t cols, size_t gate_ld) {
