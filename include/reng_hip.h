@@ -206,8 +206,9 @@ RENG_HIP_API int reng_hip_quantize_blocks(const void *w, int dtype, size_t rows,
  * a [M, K] codes with scale_a [M, ceil(K / 128)] (reng_hip_quantize_blocks with
  * block_rows 1, or reng_hip_residual_norm_fp8), b [N, K] codes with scale_b
  * [ceil(N / 128), ceil(K / 128)] (block_rows 128). Finite codes of either format
- * each; K a multiple of 16, a and b 16-byte aligned. Any M; it allocates nothing
- * and keeps nothing between calls. */
+ * each; K a multiple of 16 up to 2^22, a and b 16-byte aligned. Any M and N whose
+ * tiles fit a launch of 2^32 threads; it allocates nothing and keeps nothing
+ * between calls. */
 RENG_HIP_API int reng_hip_gemm_fp8_blocks(const uint8_t *a, int a_format, const float *scale_a, const uint8_t *b,
                                           int b_format, const float *scale_b, size_t M, size_t N, size_t K,
                                           uint16_t *out, void *stream);
@@ -349,9 +350,12 @@ RENG_HIP_API size_t reng_hip_attention_tree_workspace_bytes(size_t n_heads, size
  * scores are all -inf, or with a NaN among them, gives NaN. len >= 0, 1 <=
  * tokens <= RENG_HIP_TREE_MAX_TOKENS, len + tokens <= RENG_HIP_ATTENTION_MAX_LEN;
  * pointers 4-byte aligned, workspace 16-byte aligned with workspace_bytes >=
- * reng_hip_attention_tree_workspace_bytes(...). Fast for heads of 64, 96, 128 and
- * 256 dimensions over 16-byte aligned q and caches. Asynchronous on stream; calls
- * that share a workspace must be ordered (one stream). */
+ * reng_hip_attention_tree_workspace_bytes(...). At most 4096 query heads. On the
+ * matrix cores for heads of up to 256 dimensions, a multiple of 8, over 16-byte
+ * aligned q and caches and 8-byte aligned out; else (any even head_dim up to 1024)
+ * a general kernel, 73 to 260 times slower for a token after 4096 to 32768 rows,
+ * that leaves the workspace alone. Asynchronous on stream; calls that share a workspace must be
+ * ordered (one stream). */
 RENG_HIP_API int reng_hip_attention_tree(const uint16_t *q, const uint16_t *k_cache, const uint16_t *v_cache,
                                          size_t n_heads, size_t n_kv_heads, size_t head_dim, size_t len,
                                          size_t tokens, const uint32_t *mask, float scale, void *workspace,

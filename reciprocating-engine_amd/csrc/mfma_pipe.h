@@ -58,11 +58,6 @@ __device__ __forceinline__ void copy16_buf(__amdgpu_buffer_rsrc_t r, uint8_t *l,
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)l, 16, voff, soff, 0, 0);
 }
 
-// Four bytes a lane.
-__device__ __forceinline__ void copy4_buf(__amdgpu_buffer_rsrc_t r, uint8_t *l, uint32_t voff) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)l, 4, voff, 0, 0, 0);
-}
-
 // copy16_buf as inline asm, which the compiler does not know to write LDS: it puts
 // a wait for every copy in flight before a transposing LDS read (ds_read_tr), and
 // none after these. The caller's own waits (wait_vmcnt, then a barrier) have to
