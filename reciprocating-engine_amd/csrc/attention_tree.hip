@@ -41,9 +41,9 @@ __device__ __forceinline__ bool sees(const TreeArgs &a, uint32_t i, uint32_t j) 
 
 // The general form, any even head size up to 1024 and any 4-byte alignment: a
 // workgroup a token and head, 256 rows at a time, a thread a row for the scores
-// and a dimension pair for the values. Bound by its own loads' latency, 4 bytes a
-// lane and no split of the cache (32 heads on 8 of 128 dimensions, one token after
-// 4096 rows: 1.27 ms, where the tiled form takes 17.4 us).
+// and a dimension pair for the values. It loads 4 bytes a lane and does not split the
+// cache (32 heads on 8 of 128 dimensions, one token after 4096 rows: 1.27 ms, where the
+// tiled form takes 17.4 us).
 constexpr int ANY_T = 256, ANY_DP = 1024 / 2 / ANY_T;
 
 __global__ __launch_bounds__(ANY_T) void attention_tree_any(TreeArgs a) {
@@ -137,7 +137,7 @@ __global__ __launch_bounds__(ANY_T) void attention_tree_any(TreeArgs a) {
 //
 // Bound: HBM for few query rows on a long cache (32 heads on 8 of 128 dimensions, one
 // token after 32768 rows: 38.6 us, 3.5 TB/s; 8 tokens after 131000: 113 us, 4.8 TB/s;
-// a copy reaches 5.1), the matrix cores and the weights' arithmetic for many (40 on 8, a
+// a copy reaches 5.1), the matrix cores and the exponentials for many (40 on 8, a
 // chain of 1024 after 16384: 364 us, 975 TFLOP/s, where a library bf16 product of 8192^3
 // reaches 1400). The chain's steps, each as measured when it was taken: 1050 us, the
 // waves' halves taking turns 620, reads four products ahead 589, an order written out

@@ -7,11 +7,13 @@
 // added to an f32 accumulator, so the scales cost one multiply-add per output and
 // block beside 128 multiply-adds on the matrix cores.
 //
-// Bound: HBM for a row ([4096, 14336]: 13.2 us, 4.5 TB/s), the copies' latency for some
-// ten to 128 rows (24 rows [3584, 18944]: 22.9 us, 3.0 TB/s; 128: 38.8 us), then the matrix
-// cores ([4096, 4096, 4096]: 65.9 us, 2.09 PFLOP/s; M = 1024 [27648, 5120]: 155 us, 1.88,
-// its 432 tiles two rounds where 1.69 would do). A library fp8 product with one scale a
-// tensor takes 125 us there, and reaches 2.63 PFLOP/s at 8192^3.
+// Bound: HBM for a row ([4096, 14336]: 13.2 us, 4.5 TB/s). Some ten to 128 rows stay below
+// its rate (24 rows [3584, 18944]: 20.4-22.9 us from HBM, 14.1 out of the Infinity Cache;
+// 128: 38.8), though not for want of copies in flight: rings of 3, 4 and 5 slots take 20.5,
+// 20.5 and 20.8 us. Then the matrix cores ([4096, 4096, 4096]: 65.9 us, 2.09 PFLOP/s;
+// M = 1024 [27648, 5120]: 155 us, 1.88, its 432 tiles two rounds where 1.69 would do). A
+// library fp8 product with one scale a tensor takes 121-125 us there, and reaches 2.63-2.68
+// PFLOP/s at 8192^3.
 #include <type_traits>
 
 #include "block_forms.h"
