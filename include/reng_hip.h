@@ -347,7 +347,9 @@ RENG_HIP_API size_t reng_hip_attention_tree_workspace_bytes(size_t n_heads, size
  * [tokens, n_heads * head_dim]; otherwise as reng_hip_attention_decode, whose
  * case it is at one token that sees itself. Rows a token does not see take no
  * part, whatever they hold; a token that sees nothing gives zeros, one whose
- * scores are all -inf, or with a NaN among them, gives NaN. len >= 0, 1 <=
+ * scores are all -inf, or with a NaN among them, gives NaN. An infinite value of a
+ * row seen gives an infinity, however small the row's weight; NaN where its score
+ * is -inf (a weight of 0) or where infinities of both signs meet. len >= 0, 1 <=
  * tokens <= RENG_HIP_TREE_MAX_TOKENS, len + tokens <= RENG_HIP_ATTENTION_MAX_LEN;
  * pointers 4-byte aligned, workspace 16-byte aligned with workspace_bytes >=
  * reng_hip_attention_tree_workspace_bytes(...). At most 4096 query heads. On the

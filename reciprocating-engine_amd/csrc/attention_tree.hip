@@ -11,6 +11,10 @@
 // f32 inside. A row that a token does not see takes no part, whatever it holds
 // (NaN and infinities included); a token that sees nothing (len = 0 and an empty
 // mask row) gives zeros; a NaN score among the rows seen makes its output NaN.
+// An infinity among the values seen is an infinity of the output, however small
+// its row's weight, and NaN where the weight is exactly 0 (a score of -inf) or
+// infinities of both signs meet: settle() decides it by this rule where a sum has
+// become NaN, so that it does not depend on how the cache is cut.
 #include <type_traits>
 
 #include "common.h"
@@ -38,6 +42,28 @@ __device__ __forceinline__ bool sees(const TreeArgs &a, uint32_t i, uint32_t j) 
     if (d >= a.tokens) return false;
     return a.mask ? (a.mask[(size_t)i * a.words + d / 32] >> (d % 32)) & 1 : d <= i;
 }
+
+// Where a query's sums gave a NaN though its scores are numbers, an infinite value met a weight
+// or a factor of 0 (its row's own, or one that underflowed against the maximum of its tile, its
+// split or the whole) or an infinity of the other sign, or a value is NaN. Then the rows are gone
+// over again for such values, four bits a dimension: it sees a row with +inf (1), with -inf (2),
+// with NaN or with either at a weight of 0 (4). With a finite sum of weights no score seen is NaN
+// or +inf, so the query holds no infinity (each of its scores would be one, or NaN), and a row's
+// score is -inf exactly where its key holds one.
+__device__ __forceinline__ uint32_t special(uint32_t bf16, bool weightless) {
+    const uint32_t x = bf16 & 0x7fffu;
+    return x < 0x7f80u ? 0u : x > 0x7f80u || weightless ? 4u : bf16 & 0x8000u ? 2u : 1u;
+}
+__device__ __forceinline__ bool holds_inf(uint32_t pair) {
+    return (pair & 0x7fffu) == 0x7f80u || (pair & 0x7fff0000u) == 0x7f800000u;
+}
+// x, a sum, where it is NaN: the infinity those bits leave.
+__device__ __forceinline__ float settled(float x, uint32_t bits) {
+    return !__builtin_isnan(x) ? x : bits == 1 ? INFINITY : bits == 2 ? -INFINITY : x;
+}
+
+// Whether a sum of weights is a number that outputs can be formed with.
+__device__ __forceinline__ bool is_sum(float l) { return l > 0.0f && l < INFINITY; }
 
 // The general form, any even head size up to 1024 and any 4-byte alignment: a
 // workgroup a token and head, 256 rows at a time, a thread a row for the scores
@@ -110,12 +136,48 @@ __global__ __launch_bounds__(ANY_T) void attention_tree_any(TreeArgs a) {
         __syncthreads();   // p, seen and red are written again
     }
     // l = 0: nothing seen (zeros), or every score seen is -inf (NaN, as softmax has it).
+    float y[ANY_DP][2];
+    bool nan = false;
+#pragma unroll
+    for (int x = 0; x < ANY_DP; ++x)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            y[x][e] = o[x][e] / l;
+            nan |= __builtin_isnan(y[x][e]);
+        }
+    if (__syncthreads_or(nan && is_sum(l))) {
+        uint32_t hit[ANY_DP] = {};
+        for (uint32_t j0 = 0; j0 < rows; j0 += ANY_T) {
+            const uint32_t j = j0 + tid, n = min((uint32_t)ANY_T, rows - j0);
+            const bool on = j < rows && sees(a, i, j);
+            bool weightless = false;
+            if (on) {
+                const uint32_t *kr = reinterpret_cast<const uint32_t *>(kb + (size_t)j * pitch);
+                for (uint32_t d = 0; d < pairs; ++d) weightless |= holds_inf(kr[d]);
+            }
+            seen[tid] = on + (on && weightless);
+            __syncthreads();
+#pragma unroll
+            for (int x = 0; x < ANY_DP; ++x) {
+                const uint32_t d = tid + x * ANY_T;
+                if (d >= pairs) break;
+                for (uint32_t t = 0; t < n; ++t) {
+                    if (!seen[t]) continue;
+                    const uint32_t w = reinterpret_cast<const uint32_t *>(vb + (size_t)(j0 + t) * pitch)[d];
+                    hit[x] |= special(w & 0xffffu, seen[t] == 2) | (special(w >> 16, seen[t] == 2) << 4);
+                }
+            }
+            __syncthreads();   // seen is written again
+        }
+#pragma unroll
+        for (int x = 0; x < ANY_DP; ++x)
+            if (is_sum(l)) y[x][0] = settled(y[x][0], hit[x] & 7u), y[x][1] = settled(y[x][1], hit[x] >> 4);
+    }
     uint32_t *out = reinterpret_cast<uint32_t *>(a.out + ((size_t)i * a.nh + h) * a.hd);
 #pragma unroll
     for (int x = 0; x < ANY_DP; ++x) {
         const uint32_t d = tid + x * ANY_T;
-        if (d < pairs)
-            out[d] = any ? f32_to_bf16_bits(o[x][0] / l) | (f32_to_bf16_bits(o[x][1] / l) << 16) : 0u;
+        if (d < pairs) out[d] = any ? f32_to_bf16_bits(y[x][0]) | (f32_to_bf16_bits(y[x][1]) << 16) : 0u;
     }
 }
 
@@ -222,6 +284,73 @@ __device__ __forceinline__ u32x2 finish(const f32x4 &o, float l, bool any) {
     if (!any) return u32x2{0u, 0u};
     const float r = 1.0f / l;   // one rounding more than a division, far below bf16's
     return u32x2{pack_bf16(o.x * r, o.y * r), pack_bf16(o.z * r, o.w * r)};
+}
+
+__device__ __forceinline__ bool any_nan(const f32x4 &o) {
+    return __builtin_isnan(o.x) || __builtin_isnan(o.y) || __builtin_isnan(o.z) || __builtin_isnan(o.w);
+}
+
+// The sums o over dimensions dim .. dim + 3 of the lane's query (token tok), settled (above). Both
+// halves of a wave hold queries of the same key/value head and dimensions: the lanes of a half
+// that are on share the context's rows. (32 heads on 8 of 128 dimensions, one token after 32768
+// rows: one of them infinite and of a weight that underflows 0.16 ms, all of them 4.1 ms.)
+__device__ __forceinline__ f32x4 settle(const TreeArgs &a, uint32_t tok, uint32_t g, uint32_t dim, f32x4 o) {
+    const uint32_t lane = threadIdx.x & 63;
+    const uint64_t half = (lane & 32) ? 0xffffffff00000000ull : 0xffffffffull;
+    const uint64_t on = __builtin_amdgcn_ballot_w64(true) & half;
+    const uint32_t lanes = (uint32_t)__popcll(on), mine = (uint32_t)__popcll(on & ((1ull << lane) - 1));
+    const size_t pitch = (size_t)a.nkv * a.hd;
+    const uint16_t *vb = a.v + (size_t)g * a.hd + dim, *kb = a.k + (size_t)g * a.hd;
+    auto load = [&](uint32_t j) { return *reinterpret_cast<const u32x2 *>(vb + j * pitch); };
+    auto odd = [](const u32x2 &v) {
+        return special(v.x & 0xffffu, false) | special(v.x >> 16, false) | special(v.y & 0xffffu, false) |
+               special(v.y >> 16, false);
+    };
+    auto bits = [&](uint32_t j) {
+        const u32x2 v = load(j);
+        if (!odd(v)) return 0u;
+        bool weightless = false;
+        const u32x4 *kr = reinterpret_cast<const u32x4 *>(kb + j * pitch);
+        for (uint32_t d = 0; d < a.hd / 8; ++d) {
+            const u32x4 k = kr[d];
+            weightless |= holds_inf(k.x) || holds_inf(k.y) || holds_inf(k.z) || holds_inf(k.w);
+        }
+        return special(v.x & 0xffffu, weightless) | (special(v.x >> 16, weightless) << 4) |
+               (special(v.y & 0xffffu, weightless) << 8) | (special(v.y >> 16, weightless) << 12);
+    };
+    uint32_t found = 0;
+    for (uint32_t j0 = mine; j0 < a.len; j0 += 8 * lanes) {   // the context: every token sees it
+        uint32_t hit = 0;
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) hit |= odd(load(min(j0 + e * lanes, a.len - 1)));
+        if (!hit) continue;
+#pragma unroll 1
+        for (uint32_t e = 0; e < 8; ++e) found |= bits(min(j0 + e * lanes, a.len - 1));
+    }
+    uint32_t hit = 0;
+#pragma unroll
+    for (uint32_t b = 0; b < 16; ++b)
+        if (__builtin_amdgcn_ballot_w64((found >> b) & 1) & half) hit |= 1u << b;
+    for (uint32_t d = 0; d < a.tokens; ++d)   // the drafted rows
+        if (sees(a, tok, a.len + d)) hit |= bits(a.len + d);
+    return f32x4{settled(o.x, hit & 7u), settled(o.y, (hit >> 4) & 7u), settled(o.z, (hit >> 8) & 7u),
+                 settled(o.w, hit >> 12)};
+}
+
+// settle for all quads of a lane. Not inlined, and given the launch's arguments where they lie:
+// inlined, it costs the loops registers (a chain of 1024 without context 48.4 -> 49.7 us, so 48.6).
+__device__ __attribute__((noinline)) void settle_all(const TreeTiles *args, float *sums, uint32_t quads, uint32_t tok,
+                                                     uint32_t g, float l) {
+    const TreeArgs a = args->a;
+    for (uint32_t i = 0; i < quads; ++i) {
+        const uint32_t dim = 8 * i + 4 * (threadIdx.x >> 5 & 1);
+        f32x4 x{sums[4 * i], sums[4 * i + 1], sums[4 * i + 2], sums[4 * i + 3]};
+        if (dim >= a.hd || !__builtin_amdgcn_ballot_w64(any_nan(x) && is_sum(l))) continue;
+        x = settle(a, tok, g, dim, x);
+        if (is_sum(l))
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sums[4 * i + e] = x[e];
+    }
 }
 
 template <int HD, int RW, int KW, int TK, int S>
@@ -393,17 +522,16 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
         const u32x2 v1 = read_tr(vs + (row + 8) * ROWB + value_slot<P2>(row + 8, ch) * 16 + in);
         return u32x4{v0.x, v0.y, v1.x, v1.y};
     };
-    // What the values of a tile that are no finite numbers add: per dimension and query, the
-    // NaN, +inf and -inf among the rows seen are counted on the matrix cores. The sums go
-    // through memory, so that this seldom path asks for no registers the others would miss.
+    // The outputs that a value of the tile which is no finite number reaches become NaN (settle()
+    // decides at the end): per dimension and query, such values among the rows seen are counted on
+    // the matrix cores. The sums go through memory, so that this seldom path asks for no
+    // registers the others would miss.
     auto specials = [&](const uint8_t *vs) __attribute__((always_inline)) {
         volatile float sums[DB * 16];
 #pragma unroll
         for (int i = 0; i < DB * 16; ++i) sums[i] = o[i / 16][i % 16];
 #pragma unroll 1
-        for (int kd = 0; kd < 3 * DB; ++kd) {
-            const int kind = kd % 3, d = kd / 3;
-            const float what = kind == 0 ? __builtin_nanf("") : kind == 1 ? INFINITY : -INFINITY;
+        for (int d = 0; d < DB; ++d) {
             f32x16 cnt = zero;
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
@@ -416,12 +544,9 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
                         uint32_t z = 0, y = 0;
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            const uint32_t x = (v[i] >> (16 * e)) & 0xffffu;
-                            const bool hit = kind == 0   ? (x & 0x7fffu) > 0x7f80u
-                                             : kind == 1 ? x == 0x7f80u
-                                                         : x == 0xff80u;
+                            const uint32_t x = (v[i] >> (16 * e)) & 0x7fffu;
                             const int k = 8 * u + 2 * i + e;
-                            z |= hit ? 0x3f80u << (16 * e) : 0u;
+                            z |= x >= 0x7f80u ? 0x3f80u << (16 * e) : 0u;
                             y |= (see[kb] >> (8 * (k / 4) + k % 4)) & 1 ? 0x3f80u << (16 * e) : 0u;
                         }
                         isv[i] = z;
@@ -432,7 +557,7 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
                 }
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                if (cnt[i] > 0.0f) sums[16 * d + i] = sums[16 * d + i] + what;
+                if (cnt[i] > 0.0f) sums[16 * d + i] = __builtin_nanf("");
         }
 #pragma unroll
         for (int i = 0; i < DB * 16; ++i) o[i / 16][i % 16] = sums[i];
@@ -487,8 +612,8 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
     static_assert(BEHIND <= 2 && BEHIND * T::LOADS < 64, "vmcnt range");
     // A weight of 0 must take nothing from a row that is not seen. So the waves look through the
     // values of a tile that may hold such rows for anything that is no finite number, each at
-    // the part it copied, and where a step's tiles held some (seldom) it is added by itself and
-    // replaced by 0. `odd` is told apart by step: a wave may be one step ahead of another that
+    // the part it copied, and where a step's tiles held some (seldom) it marks the outputs that
+    // see it and is replaced by 0. `odd` is told apart by step: a wave may be one step ahead of another that
     // has not read it yet.
     auto each_copied = [&](uint32_t step, auto f) __attribute__((always_inline)) {
 #pragma unroll
@@ -642,6 +767,19 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
         w[DB * 1024 + 64 + lane] = l;
         return;
     }
+    float zeros[4] = {0.0f, 0.0f, 0.0f, 0.0f};   // unless a sum is no finite number
+#pragma unroll
+    for (int i = 0; i < DB * 16; ++i) zeros[i % 4] = fmaf(o[i / 16][i % 16], 0.0f, zeros[i % 4]);
+    const float odd_sums = (zeros[0] + zeros[1]) + (zeros[2] + zeros[3]);
+    if (__builtin_amdgcn_ballot_w64(odd_sums != 0.0f && is_sum(l))) {   // through memory, as in specials
+        float sums[DB * 16];
+#pragma unroll
+        for (int i = 0; i < DB * 16; ++i) sums[i] = o[i / 16][i % 16];
+        // A launch has its arguments, one TreeTiles, at the start of this segment.
+        settle_all((const TreeTiles *)__builtin_amdgcn_kernarg_segment_ptr(), sums, DB * 4, tok, g, l);
+#pragma unroll
+        for (int i = 0; i < DB * 16; ++i) o[i / 16][i % 16] = sums[i];
+    }
     const bool any = l != 0.0f || sees_any(a, tok);
     uint16_t *out = a.out + qrow * a.hd;
 #pragma unroll
@@ -709,8 +847,14 @@ __global__ __launch_bounds__(256) void attention_tree_merge(TreeArgs a, const fl
             for (int e = 0; e < 4; ++e) o[e] += all[384 * k + 128 + 64 * e] * f;
         }
     }
+    const uint32_t tok = min(r, R - 1) / per;
+    // (g and dim are the same in all lanes of a half, so a wave without such a head or dimension
+    // has no sums.)
+    if (__builtin_amdgcn_ballot_w64(on && any_nan(o) && is_sum(l))) {
+        const f32x4 x = settle(a, tok, g, dim, o);
+        if (is_sum(l)) o = x;
+    }
     if (!on) return;
-    const uint32_t tok = r / per;
     const bool any = l != 0.0f || sees_any(a, tok);
     uint16_t *out = a.out + ((size_t)tok * a.nh + g * per + r % per) * a.hd + dim;
     *reinterpret_cast<u32x2 *>(out) = finish(o, l, any);
