@@ -191,8 +191,9 @@ RENG_HIP_API int reng_hip_gemm_fp8_scaled(const uint8_t *a, int a_format, const 
 #define RENG_HIP_SCALE_BLOCK 128
 
 /* reng_hip_quantize's per-channel scheme with a block of block_rows x 128
- * values in the place of a row: s = absmax / (max_finite * backoff), 1 for a zero
- * block, code = encode(w / s). block_rows is 1 (activation rows) or 128
+ * values in the place of a row: s = absmax / (max_finite * backoff), 1 where that
+ * is 0 in f32 (a block of zeros, or of f32's smallest subnormals, whose codes are
+ * zeros), code = encode(w / s). block_rows is 1 (activation rows) or 128
  * (weights). w [rows, ld] as in reng_hip_quantize, aligned to its elements; codes
  * [rows, cols]; scales f32 [ceil(rows / block_rows), ceil(cols / 128)], row-major;
  * blocks at the right and lower edge are short. rows, cols, ld < 2^31. */

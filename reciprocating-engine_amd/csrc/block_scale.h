@@ -3,12 +3,14 @@
 // output as codes (residual_norm.hip).
 //
 //   m = max |x| over the block (NaN ignored, infinities counted)
-//   s = m / (max_finite * backoff), 1 where m = 0
+//   s = m / (max_finite * backoff), 1 where that is 0 in f32
 //   code = encode(x / s)
 //
 // which is the per-channel scheme of reng_fp8::quantize_with
 // (crates/reng-fp8/src/lib.rs:519-563) with a block in the place of a row, and
-// the same bits: the quotient is the IEEE one, the encoder the exact one.
+// the same bits: the quotient is the IEEE one, the encoder the exact one. (But a
+// row there has scale 0, and NaN for its zeros, where m is not 0 and m / full is:
+// m up to 2^-150 full, f32's smallest subnormals.)
 #pragma once
 
 #include "common.h"
@@ -27,7 +29,8 @@ __device__ __forceinline__ uint32_t mag_no_nan(float x) {
 }
 
 __device__ __forceinline__ float scale_of(uint32_t mbits, float full) {
-    return mbits > 0 ? __uint_as_float(mbits) / full : 1.0f;
+    const float s = __uint_as_float(mbits) / full;
+    return s == 0.0f ? 1.0f : s;
 }
 
 // Four codes in a dword. With a normal, finite s the f32 quotient is taken as
