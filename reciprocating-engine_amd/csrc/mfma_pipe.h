@@ -62,14 +62,18 @@ __device__ __forceinline__ void copy16_buf(__amdgpu_buffer_rsrc_t r, uint8_t *l,
 // a wait for every copy in flight before a transposing LDS read (ds_read_tr), and
 // none after these. The caller's own waits (wait_vmcnt, then a barrier) have to
 // order every read of the bytes. No output registers; m0 holds the LDS address,
-// one wait state before its use (a kernel that uses these has no other use of m0).
+// one wait state before its use. (The compiler warns that it does not keep a
+// reserved register that an asm changes; it is told of m0 so that it sets it anew.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void copy16_buf_asm(__amdgpu_buffer_rsrc_t r, uint8_t *l, uint32_t voff) {
     const uint32_t at = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void *)l);
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :
                  : "s"(at), "v"(voff), "s"(r)
-                 : "memory");
+                 : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 // A workgroup barrier that orders LDS traffic for the compiler (the memory
 // clobbers) without the vmcnt(0) that __syncthreads' fence would add.
