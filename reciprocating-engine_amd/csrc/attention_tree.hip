@@ -871,10 +871,11 @@ int launch_tiles(const TreeArgs &a, const TreePlan &p, float *part, hipStream_t 
     auto kern = attention_tree_tiles<HD, RW, KW, TK, S>;
     hipLaunchKernelGGL(kern, dim3(grid), dim3(64 * T::W), T::LDS, st, t);
     if (int rc = check_launch("attention_tree_tiles")) return rc;
-    if (p.splits < 2) return RENG_HIP_OK;
+    const uint32_t merge = tree_merge_waves(p, a.nkv);
+    if (merge == 0) return RENG_HIP_OK;
     const uint32_t waves = p.row_blocks * RW;
     const uint32_t pieces = a.nkv * waves * (HD / 8);
-    if (p.splits >= 8 && pieces <= 4096)   // at most a few workgroups a CU
+    if (merge == 4)
         hipLaunchKernelGGL((attention_tree_merge<HD, 4>), dim3(pieces), dim3(256), 0, st, a, part, p.splits, waves);
     else
         hipLaunchKernelGGL((attention_tree_merge<HD, 1>), dim3((pieces + 3) / 4), dim3(256), 0, st, a, part, p.splits,

@@ -97,6 +97,13 @@ inline size_t tree_part_bytes(const TreePlan &p, size_t nkv) {
                               tree_wave_floats(p.hdp) * sizeof(float);
 }
 
+// Waves of the merge that share a row's splits: a workgroup's four where it has few rows to
+// merge (at most a few workgroups a CU) from many splits; 0: nothing to merge.
+inline uint32_t tree_merge_waves(const TreePlan &p, size_t nkv) {
+    if (p.splits < 2) return 0;
+    return p.splits >= 8 && nkv * p.row_blocks * tree_form(p.hdp, p.form).rw * (p.hdp / 8) <= 4096 ? 4 : 1;
+}
+
 // No less than tree_part_bytes asks for over 1 .. tokens tokens and 0 .. len context rows.
 inline size_t tree_workspace(size_t nh, size_t nkv, size_t hd, size_t len, size_t tokens) {
     const size_t most = tree_most_splits(len + tokens);
