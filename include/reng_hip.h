@@ -206,10 +206,11 @@ RENG_HIP_API int reng_hip_quantize_blocks(const void *w, int dtype, size_t rows,
  *                           sum_{k / 128 = kb} decode(a[m, k]) decode(b[n, k])
  * a [M, K] codes with scale_a [M, ceil(K / 128)] (reng_hip_quantize_blocks with
  * block_rows 1, or reng_hip_residual_norm_fp8), b [N, K] codes with scale_b
- * [ceil(N / 128), ceil(K / 128)] (block_rows 128). Finite codes of either format
- * each; K a multiple of 16 up to 2^22, a and b 16-byte aligned. Any M and N whose
- * tiles fit a launch of 2^32 threads; it allocates nothing and keeps nothing
- * between calls. */
+ * [ceil(N / 128), ceil(K / 128)] (block_rows 128). scale_a scale_b is formed in f32:
+ * where it is no normal number there (below 2^-126, or past 2^128) outputs lose
+ * bits, or are 0, infinite or NaN. Finite codes of either format each; K a multiple
+ * of 16 up to 2^22, a and b 16-byte aligned. Any M and N whose tiles fit a launch
+ * of 2^32 threads; it allocates nothing and keeps nothing between calls. */
 RENG_HIP_API int reng_hip_gemm_fp8_blocks(const uint8_t *a, int a_format, const float *scale_a, const uint8_t *b,
                                           int b_format, const float *scale_b, size_t M, size_t N, size_t K,
                                           uint16_t *out, void *stream);
@@ -345,20 +346,30 @@ RENG_HIP_API size_t reng_hip_attention_tree_workspace_bytes(size_t n_heads, size
  * tokens - 1 the drafted tokens' own. mask [tokens, ceil(tokens / 32)] words:
  * token i sees drafted row j if bit j % 32 of word j / 32 of its row is set
  * (bits from tokens on are not read); NULL is a chain (j <= i). q and out bf16
- * [tokens, n_heads * head_dim]; otherwise as reng_hip_attention_decode, whose
- * case it is at one token that sees itself. Rows a token does not see take no
- * part, whatever they hold; a token that sees nothing gives zeros, one whose
- * scores are all -inf, or with a NaN among them, gives NaN. An infinite value of a
- * row seen gives an infinity, however small the row's weight; NaN where its score
- * is -inf (a weight of 0) or where infinities of both signs meet. len >= 0, 1 <=
- * tokens <= RENG_HIP_TREE_MAX_TOKENS, len + tokens <= RENG_HIP_ATTENTION_MAX_LEN;
- * pointers 4-byte aligned, workspace 16-byte aligned with workspace_bytes >=
+ * [tokens, n_heads * head_dim]; shapes otherwise as reng_hip_attention_decode.
+ * Scores, their maxima and sums are f32; on the matrix cores each weight is
+ * rounded to bf16 where it meets its value, which puts an output off by at most
+ * 2^-8 sum p |v| beside its own rounding. Sums are of weights up to 2^8 before they
+ * are normalised, in f32: values up to 2^102 in magnitude overflow none.
+ * One token that sees itself is reng_hip_attention_decode_split's case over len +
+ * 1 rows: that call keeps its weights in f32, and is faster on heads of 64 and 128
+ * dimensions over up to some 4096 rows (32 heads on 8 of 128: 500 rows 7.1 us, this
+ * call 13.7; 4096 rows 13.6 and 18.5; 32768 rows 37.9 and 38.6); on other heads
+ * from some 1000 rows on, and on all over 131000, this call is (256 dimensions, 16
+ * heads on 2: 4096 rows 30.1 us, this call 18.0).
+ * Rows a token does not see take no part, whatever they hold; a token that sees
+ * nothing gives zeros, one whose scores are all -inf, or with a NaN among them,
+ * gives NaN. An infinite value of a row seen gives an infinity, however small the
+ * row's weight; NaN where its score is -inf (a weight of 0) or where infinities of
+ * both signs meet.
+ * len >= 0, 1 <= tokens <= RENG_HIP_TREE_MAX_TOKENS, len + tokens <=
+ * RENG_HIP_ATTENTION_MAX_LEN; pointers 4-byte aligned, workspace 16-byte aligned with workspace_bytes >=
  * reng_hip_attention_tree_workspace_bytes(...). At most 4096 query heads. On the
  * matrix cores for heads of up to 256 dimensions, a multiple of 8, over 16-byte
  * aligned q and caches and 8-byte aligned out; else (any even head_dim up to 1024)
- * a general kernel, 73 to 260 times slower for a token after 4096 to 32768 rows,
- * that leaves the workspace alone. Asynchronous on stream; calls that share a workspace must be
- * ordered (one stream). */
+ * a general kernel, 70 to 280 times slower for a token after 4096 to 32768 rows,
+ * with f32 weights, that leaves the workspace alone. Asynchronous on stream; calls
+ * that share a workspace must be ordered (one stream). */
 RENG_HIP_API int reng_hip_attention_tree(const uint16_t *q, const uint16_t *k_cache, const uint16_t *v_cache,
                                          size_t n_heads, size_t n_kv_heads, size_t head_dim, size_t len,
                                          size_t tokens, const uint32_t *mask, float scale, void *workspace,

@@ -68,8 +68,8 @@ __device__ __forceinline__ bool is_sum(float l) { return l > 0.0f && l < INFINIT
 // The general form, any even head size up to 1024 and any 4-byte alignment: a
 // workgroup a token and head, 256 rows at a time, a thread a row for the scores
 // and a dimension pair for the values. It loads 4 bytes a lane and does not split the
-// cache (32 heads on 8 of 128 dimensions, one token after 4096 rows: 1.27 ms, where the
-// tiled form takes 17.4 us).
+// cache (32 heads on 8 of 128 dimensions, one token after 4096 rows: 1.35 ms, where the
+// tiled form takes 18.6 us).
 constexpr int ANY_T = 256, ANY_DP = 1024 / 2 / ANY_T;
 
 __global__ __launch_bounds__(ANY_T) void attention_tree_any(TreeArgs a) {
@@ -198,10 +198,11 @@ __global__ __launch_bounds__(ANY_T) void attention_tree_any(TreeArgs a) {
 // past the context look at the mask.
 //
 // Bound: HBM for few query rows on a long cache (32 heads on 8 of 128 dimensions, one
-// token after 32768 rows: 38.6 us, 3.5 TB/s; 8 tokens after 131000: 113 us, 4.8 TB/s;
+// token after 32768 rows: 38.6 us, 3.5 TB/s; 8 tokens after 131000: 108 us, 5.0 TB/s;
 // a copy reaches 5.1), the matrix cores and the exponentials for many (40 on 8, a
-// chain of 1024 after 16384: 364 us, 975 TFLOP/s, where a library bf16 product of 8192^3
-// reaches 1400). The chain's steps, each as measured when it was taken: 1050 us, the
+// chain of 1024 after 16384: 357-369 us, 960-993 TFLOP/s, where a library bf16 product of
+// 8192^3 reaches 1400). A tile past the context looks at its mask, a chain's too: 1024 tokens
+// after 0 take 50.6 us (212 TFLOP/s), after 1024 72.5 (445). The chain's steps, each as measured when it was taken: 1050 us, the
 // waves' halves taking turns 620, reads four products ahead 589, an order written out
 // with the masked tiles in a loop of their own 477, splits that fill the XCDs 351 to 373.
 // Copies issued between the weights were slower (364 -> 385 us).
@@ -796,8 +797,8 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
 // Merges the splits' (o, m, l), which lie as a wave of attention_tree_tiles held them: a wave
 // here takes one quad of dimensions of each of its lanes (32 rows, two quads each). With SW = 4
 // the four waves of a workgroup take a quarter of the splits each and meet in LDS: few rows over
-// many splits otherwise wait for one wave's chain of loads (one token after 4096 rows 20.5 ->
-// 15.3 us for the call).
+// many splits otherwise wait for one wave's chain of loads (one token after 4096 rows, in 32
+// splits, 20.5 -> 15.3 us for the call).
 template <int HD, int SW>
 __global__ __launch_bounds__(256) void attention_tree_merge(TreeArgs a, const float *__restrict__ part,
                                                             uint32_t splits, uint32_t waves) {

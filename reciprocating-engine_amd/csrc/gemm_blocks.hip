@@ -7,11 +7,11 @@
 // added to an f32 accumulator, so the scales cost one multiply-add per output and
 // block beside 128 multiply-adds on the matrix cores.
 //
-// Bound: HBM for a row ([4096, 14336]: 13.2 us, 4.5 TB/s). Some ten to 128 rows stay below
-// its rate (24 rows [3584, 18944]: 20.4-22.9 us from HBM, 14.1 out of the Infinity Cache;
-// 128: 38.8), though not for want of copies in flight: rings of 3, 4 and 5 slots take 20.5,
-// 20.5 and 20.8 us. Then the matrix cores ([4096, 4096, 4096]: 65.9 us, 2.09 PFLOP/s;
-// M = 1024 [27648, 5120]: 155 us, 1.88, its 432 tiles two rounds where 1.69 would do). A
+// Bound: HBM for a row ([4096, 14336]: 12.9 us, 4.5 TB/s). Some ten to 128 rows stay below
+// its rate (24 rows [3584, 18944]: 20-23 us from HBM, 14.1 out of the Infinity Cache;
+// 128: 38.4), though not for want of copies in flight: rings of 3, 4 and 5 slots take 20.5,
+// 20.5 and 20.8 us. Then the matrix cores ([4096, 4096, 4096]: 66-69 us, 2.0 PFLOP/s;
+// M = 1024 [27648, 5120]: 148-156 us, 1.9, its 432 tiles two rounds where 1.69 would do). A
 // library fp8 product with one scale a tensor takes 121-125 us there, and reaches 2.63-2.68
 // PFLOP/s at 8192^3.
 #include <type_traits>
@@ -46,13 +46,14 @@ __device__ __forceinline__ i32x8 join(const u32x4 &x, const u32x4 &y) {
 
 // ------------------------------------------------------------ few rows
 //
-// Up to 64 activation rows: the weight's bytes are the time. A workgroup computes 16 MT
-// rows of a by 16 NT rows of b; its KW waves split the blocks of k evenly and their sums
-// meet in LDS, in the waves' order. A wave copies its own stages (one scale block of its
-// rows) through a ring of its own, S - 1 of them in flight, and waits for nobody until
-// the end. The copies are 8 rows x 128 bytes an instruction: read straight into
-// registers in the matrix operand's layout the codes come in 64-byte pieces. Scales are
-// copied four stages at a time.
+// Where the weight's bytes are the time, or larger tiles would leave CUs idle: up to 16
+// rows always, more where block_pick's model has it faster (128 x [3584, 18944] and 256 x
+// [4096, 4096] too). A workgroup computes 16 MT rows of a, 64 at most, by 16 NT rows of b;
+// its KW waves split the blocks of k evenly and their sums meet in LDS, in the waves' order.
+// A wave copies its own stages (one scale block of its rows) through a ring of its own,
+// S - 1 of them in flight, and waits for nobody until the end. The copies are 8 rows x 128
+// bytes an instruction: read straight into registers in the matrix operand's layout the
+// codes come in 64-byte pieces. Scales are copied four stages at a time.
 // v_mfma_f32_16x16x128 with the weight as the first operand: lane l holds row l % 16 of
 // either operand and the chunks 2 (l / 16) and 2 (l / 16) + 1 of its 128 codes; the
 // result's lane has activation row l % 16 and the four weight rows from 4 (l / 16).

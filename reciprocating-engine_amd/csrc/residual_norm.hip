@@ -13,8 +13,8 @@
 //
 // Bound: HBM (x, d, gate, h and the output once each) for many rows, the chain
 // of two block sums for few. A row stays in registers from its first read to
-// its last write (with post-norm and gate, fp8 out: 4096 rows of 5120 60.6 us, 4.5
-// TB/s, 1024 rows 20 us; a row of 4096 3.9 us, bf16 out 3.3). Loading the gate and
+// its last write (with post-norm and gate, fp8 out: 4096 rows of 5120 63.5 us, 4.3
+// TB/s, 1024 rows 22.8 us, 3.0; a row of 4096 3.9 us, bf16 out 3.3). Loading the gate and
 // the weights of the norms ahead of the first sum made a row slower (3.1 -> 4.9 us).
 #include "block_scale.h"
 
@@ -231,8 +231,8 @@ int launch_norm(const NormArgs &a, size_t rows, hipStream_t st) {
     const unsigned grid = (unsigned)rows;
     auto vpt = [&](uint32_t nt) { return (a.cols + 4 * nt - 1) / (4 * nt); };
     // Few rows wait for their own chain of loads and sums, which sixteen waves make shorter; many
-    // fill the chip with four each (5120 columns, fp8 out, 256 threads / 1024: 24 rows 7.7 / 4.9
-    // us, 512 rows 12.1 / 10.5, 1024 rows 19.9 / 20.4, 4096 rows 59 / 67).
+    // fill the chip with four each (5120 columns, fp8 out into the Infinity Cache, 256 threads /
+    // 1024: 24 rows 7.7 / 4.9 us, 512 rows 12.1 / 10.5, 1024 rows 19.9 / 20.4, 4096 rows 59 / 67).
     const bool few = rows <= 2 * (size_t)device_props().cus && a.cols > 1024;
     if (vec && vpt(256) <= 8 && !few) return launch_vpt<OUT, 256, 1>(a, grid, vpt(256), st);
     if (vec && vpt(1024) <= 8) return launch_vpt<OUT, 1024, 1>(a, grid, vpt(1024), st);

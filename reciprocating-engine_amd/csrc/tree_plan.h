@@ -44,12 +44,21 @@ inline size_t tree_most_splits(size_t cache) {
     return s < 1 ? 1 : s > TREE_SPLIT_MAX ? TREE_SPLIT_MAX : s;
 }
 
-// A step's microseconds by form and head size, 64, 96, 128 and 256; the start of a round of
-// workgroups, the merge's launch, and its share of a megabyte of partials. Fitted to
-// graph-replayed timings of forms and splits on calls of 1 to 1024 tokens over 500 to 131000
-// rows (32 heads on 8 of 128 dimensions, 16 tokens after 500: 11.6 us by the model, 11.8
-// measured, where one split a workgroup a CU took 13.2; 28 on 4, 255 after 8191: 50 and 50, 72;
-// 40 on 8, 1024 after 16384: 293 and 360, 475).
+// What a choice weighs: a step's microseconds by form and head size, 64, 96, 128 and 256; the
+// start of a round of workgroups, the merge's launch, and its share of a megabyte of partials.
+// They put forms and splits in order and are below the times themselves (the eight-wave form's
+// step takes about 2 us at 128 dimensions). Graph replays of every form with up to 64 splits:
+// us by the model, as chosen (form, splits), and at best.
+//   32 heads on 8 of 128, 16 tokens after 500    10   15.2 (1, 5)    12.6 (0, 8)
+//   the same, one token after 4096               13   17.8 (0, 22)   15.8 (0, 32)
+//   one token after 32768                        29   38.7 (0, 31)   36.3 (0, 32)
+//   63 after 32768                               53   54.7 (3, 27)   53.2 (3, 26)
+//   28 on 4 of 128, 255 after 8191               51   53.4 (3, 7)    52.5 (3, 8)
+//   40 on 8 of 128, chain of 1024 after 0        25   48.1 (3, 1)    the same
+//   the same after 16384                        294    357 (3, 3)    the same
+//   28 on 4 of 64, 100 after 9000                24   25.6 (2, 10)   25.1 (1, 9)
+//   32 on 8 of 96, chain of 300 after 4000       38   39.3 (3, 5)    37.6 (3, 6)
+//   16 on 2 of 256, 27 after 30000               40   45.5 (1, 32)   41.7 (2, 64)
 constexpr float TREE_STEP_US[4][4] = {
     {0.70f, 0.90f, 1.05f, 1.30f}, {0.80f, 1.10f, 1.40f, 1.35f}, {0.70f, 0.95f, 1.10f, 1.50f}, {0.80f, 1.10f, 1.30f, 0.0f}};
 constexpr float TREE_ROUND_US = 4.0f, TREE_MERGE_US = 4.0f, TREE_MERGE_US_MB = 0.7f;

@@ -522,7 +522,8 @@ def attention_tree(q, k_cache, v_cache, n_heads, n_kv_heads, head_dim, length, t
     rows 0 .. length - 1 and, of their own rows length .. length + tokens - 1, those
     whose bit is set in mask (int32 or uint32 words [tokens, ceil(tokens / 32)]; None:
     a chain, token i sees drafted rows 0 .. i). workspace: a device tensor of at least
-    attention_tree_workspace_bytes(...) bytes (allocated here when None)."""
+    attention_tree_workspace_bytes(...) bytes (allocated here when None). The weights
+    meet the values as bf16; for one token attention_decode_split keeps them in f32."""
     T = _torch()
     if out is None:
         out = T.empty(tokens * n_heads * head_dim, dtype=T.bf16, device=q.device)

@@ -122,6 +122,20 @@ def test_infinities_whose_weight_underflows_later(R, heads, kv, hd, length, toke
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,hd,length,tokens", SHAPES + [(32, 8, 128, 60000, 2)])
+def test_the_largest_values_do_not_overflow(R, heads, kv, hd, length, tokens):
+    """Values of up to 2^102, over weights that reach 2^8 before they are normalised: the first half of the rows scores
+    5.5 below the rest (2^7.9), where a maximum does not move."""
+    q, k, v, vis, _ = planted(heads, kv, hd, length, tokens, 6)
+    k.view(-1, kv, hd)[:, :, 1:] = 0.0
+    k.view(-1, kv, hd)[length // 2:length + tokens, :, 0] = 55.0
+    v = torch.where(v.view(-1, kv, hd) < 0, -1.0, 1.0).to(v.dtype) * 2.0**102
+    v[:, :, 0] = 2.0**102
+    want = check(R, q, k, v, heads, kv, hd, length, tokens, vis, True, 0.1)
+    assert torch.isfinite(want).all()   # and check held every output to it
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("hd,length", [(128, 130), (128, 5000), (34, 130)])
 def test_a_dimension_of_infinities(R, hd, length):
     """Every row infinite in one dimension (every row but the last underflows), and a key of -inf among them."""
