@@ -202,10 +202,11 @@ __global__ __launch_bounds__(ANY_T) void attention_tree_any(TreeArgs a) {
 // a copy reaches 5.1), the matrix cores and the exponentials for many (40 on 8, a
 // chain of 1024 after 16384: 357-369 us, 960-993 TFLOP/s, where a library bf16 product of
 // 8192^3 reaches 1400). A tile past the context looks at its mask, a chain's too: 1024 tokens
-// after 0 take 50.6 us (212 TFLOP/s), after 1024 72.5 (445). The chain's steps, each as measured when it was taken: 1050 us, the
-// waves' halves taking turns 620, reads four products ahead 589, an order written out
-// with the masked tiles in a loop of their own 477, splits that fill the XCDs 351 to 373.
-// Copies issued between the weights were slower (364 -> 385 us).
+// after 0 take 50.6 us (212 TFLOP/s), after 1024 72.5 (445). The longest chain's steps, each
+// as measured when it was taken: 1050 us, the waves' halves taking turns 620, reads four
+// products ahead 589, an order written out with the masked tiles in a loop of their own 477,
+// splits that fill the XCDs 351 to 373. Copies issued between the weights were slower (364 ->
+// 385 us).
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -614,8 +615,8 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
     // A weight of 0 must take nothing from a row that is not seen. So the waves look through the
     // values of a tile that may hold such rows for anything that is no finite number, each at
     // the part it copied, and where a step's tiles held some (seldom) it marks the outputs that
-    // see it and is replaced by 0. `odd` is told apart by step: a wave may be one step ahead of another that
-    // has not read it yet.
+    // see it and is replaced by 0. `odd` is told apart by step: a wave may be one step ahead of
+    // another that has not read it yet.
     auto each_copied = [&](uint32_t step, auto f) __attribute__((always_inline)) {
 #pragma unroll
         for (int q = 0; q < T::CPW; ++q)
