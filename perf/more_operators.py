@@ -111,6 +111,11 @@ def _pitch(cols):
     return 4 * -(-cols // 128)
 
 
+def _pow2(e):
+    """2^e of whole numbers, in f32 (ldexp's own powers are off by a bit on the GPU, exp2 in f64 is exact)."""
+    return torch.exp2(e.double()).float()
+
+
 def _plain_quantize(x):
     """x f32 [rows, cols] -> signed levels (indices 0 .. 15) [rows, cols], exponents [rows, ceil(cols / 32)]."""
     rows, cols = x.shape
@@ -118,7 +123,7 @@ def _plain_quantize(x):
     f, e = torch.frexp(b.abs().amax(dim=2))
     # The largest magnitude is f 2^e, f in [0.5, 1): below 7 of the scale.
     e = torch.where(f > 0, e + (f >= 0.875).int() - 3, torch.zeros_like(e)).clamp(min=-127)
-    q = torch.ldexp(b, -e[:, :, None])
+    q = b * _pow2(-e)[:, :, None]
     a = q.abs()
     code = ((a > 0.25).byte() + (a >= 0.75).byte() + (a > 1.25).byte() + (a >= 1.75).byte() + (a > 2.5).byte()
             + (a >= 3.5).byte() + (a > 5.0).byte())
@@ -130,10 +135,10 @@ def _values(code, e):
     """f32 values of levels [rows, cols] and exponents [rows, blocks]."""
     rows, cols = code.shape
     mag = (code & 7).int()   # 0, 0.5, then 1 or 1.5 times a power of two
-    v = torch.where(mag < 2, 0.5 * mag, torch.ldexp(1 + 0.5 * (mag & 1), (mag >> 1) - 1))
+    v = torch.where(mag < 2, 0.5 * mag, (1 + 0.5 * (mag & 1)) * _pow2((mag >> 1) - 1))
     v = torch.where(code >= 8, -v, v)
     v = torch.nn.functional.pad(v, (0, -cols % BLOCK)).view(rows, -1, BLOCK)
-    return torch.ldexp(v, e[:, :, None]).view(rows, -1)[:, :cols]
+    return (v * _pow2(e)[:, :, None]).view(rows, -1)[:, :cols]
 
 
 def _unpack(codes, scales, cols):
