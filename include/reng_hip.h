@@ -399,6 +399,116 @@ RENG_HIP_API int reng_hip_residual_norm_fp8(const float *x, const uint16_t *d, c
                                             const float *gamma, size_t rows, size_t cols, float eps, int format,
                                             float backoff, float *h, uint8_t *codes, float *scales, void *stream);
 
+/* ---------------------------------------------------------------------------
+ * A layer held in 4 bits: MXFP4 weights, activations and cache (no counterpart
+ * in the reference)
+ *
+ * Codes of e2m1 (sign, two exponent bits, one mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4,
+ * 6) and a power-of-two scale for each block of 32 columns of a row. A matrix of
+ * [rows, cols] has codes [rows, ceil(cols / 2)], an even column in the low half of
+ * its byte, and scales [rows, 4 ceil(cols / 128)], byte b for columns 32 b .. 32 b +
+ * 31: a byte e stands for 2^(e - 127), 255 for NaN. Bytes of blocks past the row's
+ * last are 127.
+ * ------------------------------------------------------------------------- */
+
+#define RENG_HIP_MX_BLOCK 32
+
+/* The scale of a block is the smallest power of two under which its largest magnitude
+ * is below 7 (so that none is off by more than the rounding of its code), 2^-127 at
+ * least, and 1 for a block of zeros; a code is the nearest value, ties to the even code,
+ * of the f32 quotient, which is exact. A block that holds an infinity or NaN has the
+ * scale NaN and codes of 0. w dtype [rows, ld], aligned to its elements; codes and
+ * scales as above, scales 4-byte aligned; rows, cols, ld < 2^31. */
+RENG_HIP_API int reng_hip_quantize_mxfp4(const void *w, int dtype, size_t rows, size_t cols, size_t ld, uint8_t *codes,
+                                         uint8_t *scales, void *stream);
+
+/* What such codes stand for: out[rows, cols] = value(code) * scale, as f32 or bf16
+ * (both hold every one of them; magnitudes of 2^128 and more, which scale bytes from 253
+ * on reach, are infinite). scales 4-byte aligned, out aligned to its elements. */
+RENG_HIP_API int reng_hip_dequantize_mxfp4(const uint8_t *codes, const uint8_t *scales, size_t rows, size_t cols,
+                                           int out_dtype, void *out, void *stream);
+
+/* out[M, N] (bf16, RNE) = sum_k a[m, k] b[n, k] of two such matrices, a [M, K] the
+ * activation and b [N, K] the weight, on the matrix cores, which apply the scales; f32
+ * sums. A NaN scale makes its row's outputs NaN. K a multiple of 32 up to 2^22, a and b
+ * 16-byte and scales 4-byte aligned. Any M and N whose tiles fit a launch of 2^32
+ * threads; it allocates nothing and keeps nothing between calls. */
+RENG_HIP_API int reng_hip_gemm_mxfp4(const uint8_t *a, const uint8_t *scale_a, const uint8_t *b, const uint8_t *scale_b,
+                                     size_t M, size_t N, size_t K, uint16_t *out, void *stream);
+
+/* A key/value cache held in 4 bits (device pointers): per key/value head a matrix of
+ * [capacity, head_dim] as above, one head after the other. head_dim a multiple of 32 up
+ * to 256, 1 to 4096 heads; codes 16-byte and scales 4-byte aligned. */
+typedef struct reng_hip_mx_cache {
+    uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
+    size_t n_kv_heads, head_dim, capacity;
+} reng_hip_mx_cache;
+
+/* Rows first .. first + rows - 1 of a cache as bf16 [rows, n_kv_heads * head_dim]
+ * (reng_hip_dequantize_mxfp4's values); k or v may be NULL. 16-byte aligned outputs. */
+RENG_HIP_API int reng_hip_cache_read_mxfp4(const reng_hip_mx_cache *cache, size_t first, size_t rows, uint16_t *k,
+                                           uint16_t *v, void *stream);
+
+/* Most axes of a position (time, height, width and one more). */
+#define RENG_HIP_ROPE_MAX_AXES 4
+
+/* Rotate-half RoPE of the first rot_dim values of a head, half = rot_dim / 2 pairs (d,
+ * d + half), by tables of device f32 [table_rows, rot_dim]. A token has a position on
+ * each of `axes` axes; pair d takes row positions[pair_axis[d], token] of the tables.
+ * pair_axis is a host array of half entries below axes, NULL where all are 0. rot_dim a
+ * multiple of 16, at most head_dim; tables 16-byte aligned. */
+typedef struct reng_hip_rope {
+    const float *sin_table, *cos_table;
+    size_t table_rows, rot_dim, axes;
+    const uint8_t *pair_axis;
+} reng_hip_rope;
+
+/* The norm of each query's and key's head and the rotation of their positions in one
+ * pass, in f32, rounded to bf16 once: x = x / sqrt(mean(x^2) + eps) * gamma over a head's
+ * head_dim values, then reng_hip_rope. q bf16 [tokens, q_ld], its first n_heads * head_dim
+ * columns; k and v [tokens, kv_ld] (the columns of a fused projection's output row, for
+ * one); q_gamma, k_gamma f32 [head_dim], NULL for no norm; rope NULL for no rotation,
+ * else positions device int32 [axes, tokens]: a token with a position outside the
+ * tables gets NaN in the values it would rotate. Out: q_out bf16 [tokens, n_heads * head_dim] (may be q with that
+ * pitch), k_rows and v_rows [tokens, n_kv_heads * head_dim] (may be k, v with that pitch;
+ * these rows of a bf16 cache; v and v_rows may both be NULL). n_heads may be 0, with q
+ * and q_out NULL. head_dim a multiple of 32 up to 256, tokens < 2^22, at most 4096 heads
+ * of each; fastest on 16-byte aligned rows. */
+RENG_HIP_API int reng_hip_head_norm_rope_bf16(const uint16_t *q, size_t q_ld, const uint16_t *k, const uint16_t *v,
+                                              size_t kv_ld, size_t tokens, size_t n_heads, size_t n_kv_heads,
+                                              size_t head_dim, const float *q_gamma, const float *k_gamma, float eps,
+                                              const reng_hip_rope *rope, const int32_t *positions, uint16_t *q_out,
+                                              uint16_t *k_rows, uint16_t *v_rows, void *stream);
+
+/* The same with keys and values quantized from f32 into rows first .. first + tokens - 1
+ * of a cache, as reng_hip_quantize_mxfp4 does: without gammas and rope the cache's
+ * append. Other rows stay as they are. */
+RENG_HIP_API int reng_hip_head_norm_rope_mxfp4(const uint16_t *q, size_t q_ld, const uint16_t *k, const uint16_t *v,
+                                               size_t kv_ld, size_t tokens, size_t n_heads, const float *q_gamma,
+                                               const float *k_gamma, float eps, const reng_hip_rope *rope,
+                                               const int32_t *positions, uint16_t *q_out, const reng_hip_mx_cache *cache,
+                                               size_t first, void *stream);
+
+/* Bytes of device workspace reng_hip_attention_mxfp4 asks for, for every call with
+ * these heads, up to len context rows and up to tokens tokens. */
+RENG_HIP_API size_t reng_hip_attention_mxfp4_workspace_bytes(size_t n_heads, size_t n_kv_heads, size_t head_dim,
+                                                             size_t len, size_t tokens);
+
+/* reng_hip_attention_tree over a cache held in 4 bits, for one token or many: rows 0 ..
+ * len - 1 are context, rows len .. len + tokens - 1 the tokens' own, mask as there (NULL:
+ * a chain). Scores, their maxima and sums are f32; each weight is rounded to bf16 where
+ * it meets its value, and values up to 2^102 in magnitude overflow none, as there. Rows a token does not
+ * see take no part, whatever they hold. A row that is seen and has a scale byte of 253 or more
+ * in its key or its value (a NaN block, or magnitudes of some 2^128) makes all of the token's
+ * outputs NaN; so does a NaN or +inf score. A token that sees nothing gives zeros, one whose scores are all
+ * -inf NaN. q and out bf16 [tokens, n_heads * head_dim], 16-byte aligned; 1 <= tokens <=
+ * RENG_HIP_TREE_MAX_TOKENS, len + tokens at most RENG_HIP_ATTENTION_MAX_LEN and the
+ * capacity; workspace 16-byte aligned. Asynchronous on stream; calls that share a
+ * workspace must be ordered (one stream). */
+RENG_HIP_API int reng_hip_attention_mxfp4(const uint16_t *q, const reng_hip_mx_cache *cache, size_t n_heads, size_t len,
+                                          size_t tokens, const uint32_t *mask, float scale, void *workspace,
+                                          size_t workspace_bytes, uint16_t *out, void *stream);
+
 /* out = bf16(silu(gate) * up), silu(g) = g / (1 + exp(-g)) (layer_cpu's
  * Activation::Silu, model.rs:3070-3080). */
 RENG_HIP_API int reng_hip_silu_mul_bf16(const uint16_t *gate, const uint16_t *up, size_t n, uint16_t *out,

@@ -40,6 +40,17 @@ class _Matrix(ctypes.Structure):
                 ("ld", ctypes.c_size_t)]
 
 
+class _MxCache(ctypes.Structure):
+    _fields_ = [("k_codes", ctypes.c_void_p), ("k_scales", ctypes.c_void_p), ("v_codes", ctypes.c_void_p),
+                ("v_scales", ctypes.c_void_p), ("n_kv_heads", ctypes.c_size_t), ("head_dim", ctypes.c_size_t),
+                ("capacity", ctypes.c_size_t)]
+
+
+class _Rope(ctypes.Structure):
+    _fields_ = [("sin_table", ctypes.c_void_p), ("cos_table", ctypes.c_void_p), ("table_rows", ctypes.c_size_t),
+                ("rot_dim", ctypes.c_size_t), ("axes", ctypes.c_size_t), ("pair_axis", ctypes.c_char_p)]
+
+
 _lib = None
 _P, _SZ, _I, _F, _U32 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_float, ctypes.c_uint32
 
@@ -65,6 +76,14 @@ SIGNATURES = {
     "reng_hip_residual_norm_fp8": (_I, [_P, _P, _P, _P, _SZ, _F, _P, _SZ, _SZ, _F, _I, _F, _P, _P, _P, _P]),
     "reng_hip_attention_tree_workspace_bytes": (_SZ, [_SZ, _SZ, _SZ, _SZ, _SZ]),
     "reng_hip_attention_tree": (_I, [_P, _P, _P, _SZ, _SZ, _SZ, _SZ, _SZ, _P, _F, _P, _SZ, _P, _P]),
+    "reng_hip_quantize_mxfp4": (_I, [_P, _I, _SZ, _SZ, _SZ, _P, _P, _P]),
+    "reng_hip_dequantize_mxfp4": (_I, [_P, _P, _SZ, _SZ, _I, _P, _P]),
+    "reng_hip_gemm_mxfp4": (_I, [_P, _P, _P, _P, _SZ, _SZ, _SZ, _P, _P]),
+    "reng_hip_cache_read_mxfp4": (_I, [_P, _SZ, _SZ, _P, _P, _P]),
+    "reng_hip_head_norm_rope_bf16": (_I, [_P, _SZ, _P, _P, _SZ, _SZ, _SZ, _SZ, _SZ, _P, _P, _F, _P, _P, _P, _P, _P, _P]),
+    "reng_hip_head_norm_rope_mxfp4": (_I, [_P, _SZ, _P, _P, _SZ, _SZ, _SZ, _P, _P, _F, _P, _P, _P, _P, _SZ, _P]),
+    "reng_hip_attention_mxfp4_workspace_bytes": (_SZ, [_SZ, _SZ, _SZ, _SZ, _SZ]),
+    "reng_hip_attention_mxfp4": (_I, [_P, _P, _SZ, _SZ, _SZ, _P, _F, _P, _SZ, _P, _P]),
     "reng_hip_verify_hw_convert": (_I, [_I, ctypes.POINTER(ctypes.c_uint64), ctypes.POINTER(ctypes.c_uint32)]),
     "reng_hip_rms_norm_bf16": (_I, [_P, _P, _SZ, _SZ, _F, _P, _P]),
     "reng_hip_add_rms_norm_bf16": (_I, [_P, _P, _P, _SZ, _SZ, _F, _P, _P, _P]),
@@ -384,6 +403,7 @@ class _Torch:
         self.empty, self.u8, self.f32, self.bf16 = torch.empty, torch.uint8, torch.float32, torch.bfloat16
         self.is16 = frozenset((torch.bfloat16, torch.int16, torch.uint16))
         self.is32 = frozenset((torch.int32, torch.uint32))
+        self.i32 = torch.int32
         self.several = torch.cuda.device_count() > 1
         self.current_device = torch.cuda.current_device
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -538,6 +558,213 @@ def attention_tree(q, k_cache, v_cache, n_heads, n_kv_heads, head_dim, length, t
     _check(lib().reng_hip_attention_tree(
         _16bit(q, "q", nq), _16bit(k_cache, "k_cache", nc), _16bit(v_cache, "v_cache", nc), n_heads, n_kv_heads,
         head_dim, length, tokens, None if mask is None else _at(mask, "mask", tokens * _nblocks(tokens, 32), 4), scale,
+        None if workspace is None else _at(workspace, "workspace", 0, 1), wb, _16bit(out, "out", nq), T.stream()))
+    return out
+
+
+# ---------------------------------------------------------------- a layer held in 4 bits
+# MXFP4: e2m1 codes, two a byte, with a power-of-two scale byte for 32 columns of a row.
+
+MX_BLOCK = 32
+ROPE_MAX_AXES = 4
+
+
+def mx_scale_pitch(cols):
+    """Bytes of a row's scales: one for 32 columns, in words of four."""
+    return 4 * _nblocks(cols)
+
+
+def quantize_mxfp4_into(w, rows, cols, codes, scales, ld=None):
+    """quantize_mxfp4 into caller-owned tensors (no allocation)."""
+    T = _torch()
+    ld = cols if ld is None else ld
+    dt = _dtype_code(w)
+    _check(lib().reng_hip_quantize_mxfp4(_at(w, "weight", _span(rows, cols, ld), 2 if dt == BF16 else 4), dt, rows, cols, ld,
+                                         _8bit(codes, "codes", rows * _nblocks(cols, 2)),
+                                         _8bit(scales, "scales", rows * mx_scale_pitch(cols)), T.stream()))
+
+
+def quantize_mxfp4(w, rows, cols, ld=None):
+    """(codes [rows * ceil(cols / 2)], scales [rows * mx_scale_pitch(cols)]) of a device tensor of bf16 (or its
+    int16 bits) or f32, [rows, ld] row-major: e2m1 codes under the smallest power of two that leaves a block's
+    largest magnitude below 7."""
+    T, dev = _torch(), w.device
+    codes = T.empty(rows * _nblocks(cols, 2), dtype=T.u8, device=dev)
+    scales = T.empty(rows * mx_scale_pitch(cols), dtype=T.u8, device=dev)
+    quantize_mxfp4_into(w, rows, cols, codes, scales, ld)
+    return codes, scales
+
+
+def dequantize_mxfp4(codes, scales, rows, cols, out=None):
+    """The values of quantize_mxfp4's codes, [rows * cols] as bf16, or as `out` is: bf16 (or its bits) or f32."""
+    T = _torch()
+    if out is None:
+        out = T.empty(rows * cols, dtype=T.bf16, device=codes.device)
+    dt = _dtype_code(out)
+    _check(lib().reng_hip_dequantize_mxfp4(_8bit(codes, "codes", rows * _nblocks(cols, 2)),
+                                           _8bit(scales, "scales", rows * mx_scale_pitch(cols)), rows, cols, dt,
+                                           _at(out, "out", rows * cols, 2 if dt == BF16 else 4), T.stream()))
+    return out
+
+
+def gemm_mxfp4(a, scale_a, b, scale_b, M, N, K, out=None):
+    """bf16 out[M, N] of codes a [M, K / 2] and b [N, K / 2] with their scales, as quantize_mxfp4 gives them."""
+    T = _torch()
+    if out is None:
+        out = T.empty(M * N, dtype=T.bf16, device=a.device)
+    sp = mx_scale_pitch(K)
+    _check(lib().reng_hip_gemm_mxfp4(_8bit(a, "a", M * _nblocks(K, 2)), _8bit(scale_a, "scale_a", M * sp),
+                                     _8bit(b, "b", N * _nblocks(K, 2)), _8bit(scale_b, "scale_b", N * sp), M, N, K,
+                                     _16bit(out, "out", M * N), T.stream()))
+    return out
+
+
+class MxCache:
+    """A key/value cache held in 4 bits: per key/value head a matrix of [capacity, head_dim] as quantize_mxfp4 lays
+    it out. Its tensors are allocated here, or given as (k_codes, k_scales, v_codes, v_scales); rows that
+    nothing was written to hold what was there."""
+
+    def __init__(self, n_kv_heads, head_dim, capacity, device="cuda", tensors=None):
+        T = _torch()
+        self.n_kv_heads, self.head_dim, self.capacity = n_kv_heads, head_dim, capacity
+        rows, sp = n_kv_heads * capacity, mx_scale_pitch(head_dim)
+        if tensors is None:
+            tensors = tuple(T.empty(rows * n, dtype=T.u8, device=device) for n in (head_dim // 2, sp) * 2)
+        self.tensors = tuple(tensors)
+        at = [_8bit(t, what, rows * n) for t, what, n in zip(self.tensors, ("k_codes", "k_scales", "v_codes", "v_scales"),
+                                                             (head_dim // 2, sp) * 2)]
+        self.device = self.tensors[0].device
+        self._struct = _MxCache(*at, n_kv_heads, head_dim, capacity)
+        self._ref = ctypes.addressof(self._struct)
+
+    def _here(self):
+        """The descriptor's address, for a call on the current device."""
+        if _T.several and self.device.index != _T.current_device():
+            raise ValueError(f"the cache is on {self.device}, the current device is cuda:{_T.current_device()}")
+        return self._ref
+
+    def write(self, k, v, first, tokens):
+        """Rows first .. first + tokens - 1 from bf16 k and v [tokens, n_kv_heads * head_dim] (rows may be strided)."""
+        head_norm_rope_mxfp4(None, k, v, tokens, 0, self, first)
+
+    def read(self, first, rows, k=None, v=None):
+        """(k, v) bf16 [rows * n_kv_heads * head_dim] of rows first .. first + rows - 1."""
+        T, n = _torch(), rows * self.n_kv_heads * self.head_dim
+        k = T.empty(n, dtype=T.bf16, device=self.device) if k is None else k
+        v = T.empty(n, dtype=T.bf16, device=self.device) if v is None else v
+        _check(lib().reng_hip_cache_read_mxfp4(self._here(), first, rows, _16bit(k, "k", n), _16bit(v, "v", n), T.stream()))
+        return k, v
+
+
+class Rope:
+    """Rotation tables: sin and cos f32 [rows, rot_dim], and which axis' position each of the rot_dim / 2 pairs
+    takes: sections (s0, s1, ..) for the first s0 pairs axis 0, the next s1 axis 1 and so on, or pair_axis with an
+    axis for each pair; without either all take axis 0."""
+
+    def __init__(self, sin, cos, sections=None, pair_axis=None):
+        _torch()
+        if sin.dim() != 2 or sin.shape != cos.shape:
+            raise ValueError(f"tables of shapes {tuple(sin.shape)} and {tuple(cos.shape)}; expected the same [rows, rot_dim]")
+        rows, rot = sin.shape
+        if sections is not None:
+            if pair_axis is not None:
+                raise ValueError("sections and pair_axis both given")
+            pair_axis = [a for a, n in enumerate(sections) for _ in range(n)]
+        if pair_axis is not None and len(pair_axis) != rot // 2:
+            raise ValueError(f"axes for {len(pair_axis)} pairs; the tables rotate {rot // 2}")
+        self.axes = 1 if pair_axis is None else len(sections) if sections is not None else max(pair_axis) + 1
+        self.device, self.tables = sin.device, (sin, cos)
+        # ctypes keeps the bytes alive with the descriptor; one axis needs no map.
+        self._struct = _Rope(_f32(sin, "sin", rows * rot), _f32(cos, "cos", rows * rot), rows, rot, self.axes,
+                             bytes(pair_axis) if self.axes > 1 else None)
+        self._ref = ctypes.addressof(self._struct)
+
+
+def _rows16(t, what, tokens, width):
+    """(address, row pitch) of bf16 rows: a contiguous tensor of any shape but two dimensions, or [>= tokens, >= width]
+    with contiguous columns."""
+    if t.dim() != 2:
+        return _16bit(t, what, tokens * width), width
+    if t.dtype not in _T.is16 or not t.is_cuda or t.stride(1) != 1 or t.shape[0] < tokens or t.shape[1] < width:
+        raise ValueError(f"{what} must be bf16 (or its bits) rows on the GPU, [{tokens}, {width}] with contiguous columns, "
+                         f"not {t.dtype} {tuple(t.shape)} of strides {t.stride()}")
+    if _T.several and t.get_device() != _T.current_device():
+        raise ValueError(f"{what} is on cuda:{t.get_device()}, the current device is cuda:{_T.current_device()}")
+    return t.data_ptr(), t.stride(0)
+
+
+def _heads_args(T, q, k, v, tokens, n_heads, n_kv_heads, head_dim, q_gamma, k_gamma, rope, positions, q_out):
+    """What both calls share: the rows' addresses and pitches, gammas, rope, positions, and q_out."""
+    nq, nk = n_heads * head_dim, n_kv_heads * head_dim
+    kp, k_ld = _rows16(k, "k", tokens, nk)
+    vp, v_ld = (None, k_ld) if v is None else _rows16(v, "v", tokens, nk)
+    if k_ld != v_ld and tokens > 1:
+        raise ValueError(f"k and v must have one row pitch, not {k_ld} and {v_ld}")
+    qp, q_ld = (None, 0) if q is None else _rows16(q, "q", tokens, nq)
+    if q is not None and q_out is None:
+        q_out = T.empty(tokens * nq, dtype=T.bf16, device=q.device)
+    ref = pos = None
+    if rope is not None:
+        if _T.several and rope.device.index != _T.current_device():
+            raise ValueError(f"the tables are on {rope.device}, the current device is cuda:{_T.current_device()}")
+        if positions is None or positions.dtype != T.i32:
+            raise ValueError("positions must be int32 [axes, tokens]")
+        ref, pos = rope._ref, _at(positions, "positions", rope.axes * tokens, 4)
+    gq = None if q_gamma is None else _f32(q_gamma, "q_gamma", head_dim)
+    gk = None if k_gamma is None else _f32(k_gamma, "k_gamma", head_dim)
+    return (qp, q_ld, kp, vp, k_ld, gq, gk, ref, pos, None if q_out is None else _16bit(q_out, "q_out", tokens * nq)), q_out
+
+
+def head_norm_rope_bf16(q, k, v, tokens, n_heads, n_kv_heads, head_dim, q_gamma=None, k_gamma=None, eps=1e-6, rope=None,
+                        positions=None, q_out=None, k_rows=None, v_rows=None):
+    """(q_out, k_rows, v_rows): queries and keys normalised per head (where gammas f32 [head_dim] are given) and rotated
+    (rope, a Rope, at positions int32 [axes, tokens]), values as they are, bf16 [tokens, heads * head_dim]. q, k and v
+    are bf16 rows, which may be column ranges of a wider tensor; k_rows and v_rows a bf16 cache's rows."""
+    T = _torch()
+    nk = n_kv_heads * head_dim
+    a, q_out = _heads_args(T, q, k, v, tokens, n_heads, n_kv_heads, head_dim, q_gamma, k_gamma, rope, positions, q_out)
+    k_rows = T.empty(tokens * nk, dtype=T.bf16, device=k.device) if k_rows is None else k_rows
+    if v is not None and v_rows is None:
+        v_rows = T.empty(tokens * nk, dtype=T.bf16, device=k.device)
+    _check(lib().reng_hip_head_norm_rope_bf16(*a[:5], tokens, n_heads, n_kv_heads, head_dim, *a[5:7], eps, *a[7:],
+                                              _16bit(k_rows, "k_rows", tokens * nk),
+                                              None if v_rows is None else _16bit(v_rows, "v_rows", tokens * nk), T.stream()))
+    return q_out, k_rows, v_rows
+
+
+def head_norm_rope_mxfp4(q, k, v, tokens, n_heads, cache, first, q_gamma=None, k_gamma=None, eps=1e-6, rope=None,
+                         positions=None, q_out=None):
+    """q_out: head_norm_rope_bf16 with keys and values quantized into rows first .. first + tokens - 1 of an MxCache."""
+    T = _torch()
+    a, q_out = _heads_args(T, q, k, v, tokens, n_heads, cache.n_kv_heads, cache.head_dim, q_gamma, k_gamma, rope, positions,
+                           q_out)
+    _check(lib().reng_hip_head_norm_rope_mxfp4(*a[:5], tokens, n_heads, *a[5:7], eps, *a[7:], cache._here(), first, T.stream()))
+    return q_out
+
+
+def attention_mxfp4_workspace_bytes(n_heads, n_kv_heads, head_dim, length, tokens):
+    """Device workspace attention_mxfp4 needs for up to `length` context rows and `tokens` tokens."""
+    return lib().reng_hip_attention_mxfp4_workspace_bytes(n_heads, n_kv_heads, head_dim, length, tokens)
+
+
+def attention_mxfp4(q, cache, n_heads, length, tokens, scale, mask=None, workspace=None, out=None):
+    """bf16 out [tokens, n_heads * head_dim]: attention_tree over an MxCache, whose rows 0 .. length - 1 are
+    context and the next `tokens` the tokens' own (mask as there; None: a chain). workspace: a device tensor of
+    at least attention_mxfp4_workspace_bytes(...) bytes (allocated here when None)."""
+    T = _torch()
+    nq = tokens * n_heads * cache.head_dim
+    if out is None:
+        out = T.empty(nq, dtype=T.bf16, device=q.device)
+    if workspace is None:
+        wb = attention_mxfp4_workspace_bytes(n_heads, cache.n_kv_heads, cache.head_dim, length, tokens)
+        workspace = T.empty(wb, dtype=T.u8, device=q.device) if wb else None
+    else:
+        wb = workspace.numel() * workspace.element_size()
+    if mask is not None and mask.dtype not in T.is32:
+        raise ValueError(f"mask must hold 32-bit words, not {mask.dtype}")
+    _check(lib().reng_hip_attention_mxfp4(
+        _16bit(q, "q", nq), cache._here(), n_heads, length, tokens,
+        None if mask is None else _at(mask, "mask", tokens * _nblocks(tokens, 32), 4), scale,
         None if workspace is None else _at(workspace, "workspace", 0, 1), wb, _16bit(out, "out", nq), T.stream()))
     return out
 

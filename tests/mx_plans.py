@@ -1,0 +1,38 @@
+"""The choices of the 4-bit operators' launchers, from the headers that the launchers themselves use."""
+import ctypes
+import os
+import subprocess
+import tempfile
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "reciprocating-engine_amd", "csrc")
+CUS = 256   # an MI355X
+SOURCE = """
+#include "mx_attention_plan.h"
+using namespace reng;
+extern "C" void plan(size_t nh, size_t nkv, size_t hd, size_t len, size_t tokens, size_t cus, uint64_t *out) {
+    const MxAttnPlan p = mxa_plan(nh, nkv, hd, len, tokens, cus);
+    const uint64_t v[] = {p.hdp, p.qt, p.row_blocks, p.splits, p.tiles, mxa_part_bytes(p, nkv, tokens * (nh / nkv))};
+    for (int i = 0; i < 6; ++i) out[i] = v[i];
+}
+"""
+_lib = None
+
+
+def lib():
+    global _lib
+    if _lib is None:
+        with tempfile.TemporaryDirectory() as d:
+            src, so = os.path.join(d, "plans.cpp"), os.path.join(d, "plans.so")
+            with open(src, "w") as f:
+                f.write(SOURCE)
+            subprocess.run(["g++", "-O2", "-std=c++17", "-Wall", "-Wextra", "-Werror", "-shared", "-fPIC", "-I", CSRC, "-o", so, src],
+                           check=True)
+            _lib = ctypes.CDLL(so)
+        _lib.plan.argtypes = [ctypes.c_size_t] * 6 + [ctypes.c_void_p]
+    return _lib
+
+
+def mx_attention_plan(nh, nkv, hd, length, tokens, cus=CUS):
+    out = (ctypes.c_uint64 * 6)()
+    lib().plan(nh, nkv, hd, length, tokens, cus, out)
+    return dict(zip(("hdp", "qt", "row_blocks", "splits", "tiles", "bytes"), out))
