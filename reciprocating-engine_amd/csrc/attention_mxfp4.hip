@@ -23,7 +23,10 @@
 // A row whose key or value holds a scale from 253 on (NaN, or magnitudes bf16 ends at) counts as NaN: its
 // key's scale becomes NaN and its value's 1, so that its score decides who meets it, and a
 // weight of 0 takes nothing from a value.
+#include <type_traits>
+
 #include "common.h"
+#include "mfma_pipe.h"
 #include "mx.h"
 #include "mx_attention_plan.h"
 
@@ -37,6 +40,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
@@ -196,12 +200,21 @@ __global__ __launch_bounds__(64 * MXA_WAVES) void attention_mxfp4(const MxAttn a
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d][t] = f32x4{0, 0, 0, 0};
     }
+    Codes kn[2], vn[2];   // the next tile's
+    auto fetch = [&](uint32_t tile) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            kn[u] = load(a.kc, a.ks, tile * MXA_TILE + 16 * u + r16);
+            vn[u] = load(a.vc, a.vs, tile * MXA_TILE + 16 * u + r16);
+        }
+    };
+    if (t0 + wave < t1) fetch(t0 + wave);
     for (uint32_t tile = t0 + wave; tile < t1; tile += NW) {
         const uint32_t j0 = tile * MXA_TILE;
         f32x4 s[2][QT];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {   // keys 16 u ..
-            Codes k = load(a.kc, a.ks, j0 + 16 * u + r16), v = load(a.vc, a.vs, j0 + 16 * u + r16);
+            Codes k = kn[u], v = vn[u];
 #pragma unroll
             for (int i = 0; i < CH; ++i) {
                 const bool odd = max(k.s[i], v.s[i]) >= 253;
@@ -223,6 +236,7 @@ __global__ __launch_bounds__(64 * MXA_WAVES) void attention_mxfp4(const MxAttn a
                     s[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, __builtin_bit_cast(bf16x8, qf[t][e]), s[u][t], 0, 0, 0);
             }
         }
+        fetch(min(tile + NW, t1 - 1));
         asm volatile("" ::: "memory");   // the values are read by other lanes than wrote them, in the wave's own order
         const bool masked = j0 + MXA_TILE > a.len;
         u32x4 pw[QT];
@@ -321,6 +335,379 @@ __global__ __launch_bounds__(64 * MXA_WAVES) void attention_mxfp4(const MxAttn a
     }
 }
 
+// ------------------------------------------------------------ many query rows
+//
+// The query rows go 32 to a wave. A workgroup's RW waves of a key group share its tiles of TK
+// cache rows, which they bring into LDS as bf16: a wave reads its share of a later tile's codes into
+// registers and writes their values a step after. KW key groups take tiles in turn and merge
+// in LDS. Products are v_mfma_f32_32x32x16_bf16: S^T = K Q^T leaves a lane 16 scores of one query per
+// 32 keys, in the order in which O^T = V^T P^T takes the weights.
+template <int HD, int RW, int KW, int TK, int S>
+struct MxShape {
+    static constexpr int W = RW * KW, P2 = HD / 8, ROWB = 2 * HD;   // 16-byte chunks and bytes of a row
+    static constexpr int TILE = TK * ROWB, STAGE = 2 * TILE;        // keys then values
+    static constexpr int NB = HD / 32, RT = 64 / NB;                // blocks of a row; rows of a wave's part
+    static constexpr int PARTS = 2 * TK / RT, MINE = (PARTS + RW - 1) / RW;   // parts of a tile; of a wave
+    static constexpr int PW = HD * 32 + 128;                        // floats that a wave merges
+    static constexpr int RING = KW * S * STAGE, MERGE = (KW - 1) * RW * PW * 4, LDS = RING > MERGE ? RING : MERGE;
+    static constexpr int DB = HD / 32, KB = TK / 32;
+    static constexpr int AHEAD = 6;                                 // products whose operands are read ahead
+    static constexpr bool TURNS = RW == 8;                          // the waves' halves take turns
+    static_assert(!TURNS || (KW == 1 && S == 4), "one wave of each half on a SIMD, four slots");
+    static_assert(TURNS || S == 2, "a tile is written while the one before it is used");
+    static_assert(LDS <= 160 * 1024, "LDS");
+};
+
+// 32 rows are read at one chunk, eight consecutive ones are written at one.
+__device__ __forceinline__ uint32_t key_slot(uint32_t r, uint32_t c) { return c ^ (r & 7); }
+
+__device__ __forceinline__ float both_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float both_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+template <int HD, int RW, int KW, int TK, int S>
+__global__ __launch_bounds__(64 * RW * KW) void attention_mxfp4_tiles(const MxAttn a) {
+    using T = MxShape<HD, RW, KW, TK, S>;
+    constexpr int ROWB = T::ROWB, DB = T::DB, KB = T::KB, AHEAD = T::AHEAD, MINE = T::MINE;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    const uint32_t b = blockIdx.x / MXA_XCDS, rb = b % a.row_blocks;
+    const uint32_t unit = b / a.row_blocks * MXA_XCDS + blockIdx.x % MXA_XCDS;
+    if (unit >= a.units) return;
+    const uint32_t g = unit % a.nkv, split = unit / a.nkv;
+    const uint32_t lane = threadIdx.x & 63, h = lane >> 5, ql = lane & 31;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = wave % RW, kg = wave / RW;
+    const uint32_t per = a.nh / a.nkv, R = a.tokens * per, rows = a.len + a.tokens;
+
+    // This lane's query row (clamped: rows past the last are not stored).
+    const uint32_t r0 = (rb * RW + rw) * 32 + ql, r = min(r0, R - 1), tok = r / per;
+    const size_t qrow = (size_t)tok * a.nh + g * per + r % per;
+    const float c = fabsf(a.scale) * 1.44269504088896341f;
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+    bf16x8 qf[HD / 16];
+#pragma unroll
+    for (int s = 0; s < HD / 16; ++s) {
+        const uint32_t d = 16 * s + 8 * h;
+        u32x4 v{0u, 0u, 0u, 0u};
+        if (d < a.hd) v = *reinterpret_cast<const u32x4 *>(a.q + qrow * a.hd + d);
+        qf[s] = __builtin_bit_cast(bf16x8, v ^ flip);
+    }
+
+    // The split's tiles, cut for a chain at the last row its tokens see.
+    const uint32_t t0 = split * a.base + min(split, a.more);
+    uint32_t t1 = t0 + a.base + (split < a.more);
+    if (!a.mask) {
+        const uint32_t last = min((rb * RW + RW) * 32 - 1, R - 1) / per;
+        t1 = min(t1, (a.len + last) / TK + 1);
+    }
+    const uint32_t n = t1 > t0 ? t1 - t0 : 0, steps = (n + KW - 1) / KW;
+    auto has = [&](uint32_t step) { return step * KW + kg < n; };
+    auto tile_row = [&](uint32_t step) { return (t0 + step * KW + kg) * TK; };
+    uint8_t *ring = lds + kg * (S * T::STAGE);
+    auto keys = [&](uint32_t step) { return ring + (step % S) * T::STAGE; };
+
+    // A part is 64 blocks of 32 codes: a block a lane, RT rows of keys (the first half of the parts)
+    // or values. fetch() reads this wave's parts of a tile, put() writes their values.
+    const size_t head = (size_t)g * a.cap;
+    const uint32_t prow = lane % T::RT, blk = lane / T::RT;
+    u32x4 codes[MINE];
+    uint32_t byte[MINE], other[MINE];   // the block's scale; for a key its value's, too
+    auto fetch = [&](uint32_t step) __attribute__((always_inline)) {
+        const uint32_t j0 = min(tile_row(step), rows - 1);
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) {
+            const uint32_t part = rw + i * RW, half = T::PARTS / 2;
+            if (part >= T::PARTS) break;
+            const bool values = part >= half;
+            const size_t row = head + min(j0 + (values ? part - half : part) * T::RT + prow, rows - 1);
+            codes[i] = u32x4{0u, 0u, 0u, 0u};
+            byte[i] = other[i] = ONE_BYTE;
+            if (32 * blk < a.hd) {
+                codes[i] = *reinterpret_cast<const u32x4 *>((values ? a.vc : a.kc) + row * (a.hd / 2) + 16 * blk);
+                byte[i] = (values ? a.vs : a.ks)[row * a.sp + blk];
+                if (!values) other[i] = a.vs[row * a.sp + blk];
+            }
+        }
+    };
+    auto put = [&](uint32_t step) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) {
+            const uint32_t part = rw + i * RW, half = T::PARTS / 2;
+            if (part >= T::PARTS) break;
+            const bool values = part >= half;
+            const uint32_t row = (values ? part - half : part) * T::RT + prow;
+            const bool odd = max(byte[i], other[i]) >= 253;
+            const float s = scale_operand(odd ? (values ? ONE_BYTE : NAN_BYTE) : byte[i]);
+            uint8_t *to = keys(step) + (values ? T::TILE : 0) + row * ROWB;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t ch = 4 * blk + e;
+                *reinterpret_cast<u32x4 *>(to + 16 * (values ? value_slot(row, ch) : key_slot(row, ch))) = decode8(codes[i][e], s);
+            }
+        }
+    };
+
+    f32x16 o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+    float m = -INFINITY, l = 0.0f;   // the running maximum of the products, this lane's share of the sum
+    f32x16 s[KB];                    // a tile's scores, before the scale
+    u32x4 pw[2 * KB];                // its weights in bf16: the 16 rows 16 u .. of each 32 as PV takes them
+
+    // 16 dimensions of 32 of a tile's keys as the matrix cores take them.
+    auto key_frag = [&](const uint8_t *ks, int kb, int st) __attribute__((always_inline)) {
+        const uint32_t row = 32 * kb + ql;
+        return *reinterpret_cast<const u32x4 *>(ks + row * ROWB + key_slot(row, 2 * st + h) * 16);
+    };
+    const f32x16 zero = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f,
+                         0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    auto weights = [&](auto masked_c, uint32_t j0) __attribute__((always_inline)) {
+        constexpr bool MASKED = decltype(masked_c)::value;
+        uint32_t see[KB];   // bit 8 (i / 4) + i % 4: whether score i counts
+        if constexpr (MASKED) {
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                see[kb] = seen_bits(a, tok, j0 + 32 * kb) >> (4 * h);
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (!((see[kb] >> (8 * (i / 4) + i % 4)) & 1)) s[kb][i] = -INFINITY;
+            }
+        }
+        // Four chains each for the maximum and the sum: one would wait for every step's result.
+        float mx4[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx4[i] = s[0][i];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = kb ? 0 : 4; i < 16; i += 8)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    mx4[e] = i + 4 < 16 ? fmaxf(fmaxf(mx4[e], s[kb][i + e]), s[kb][i + 4 + e]) : fmaxf(mx4[e], s[kb][i + e]);
+        const float mx = both_max(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])));
+        // The maximum moves, and what is summed so far is scaled down, only where a
+        // score passes it by more than 2^8: weights up to 256 lose nothing in f32 or bf16.
+        const bool move = (mx - m) * c > 8.0f || (m == -INFINITY && mx > m);
+        if (__builtin_amdgcn_ballot_w64(move)) {
+            const float f = !move ? 1.0f : m == -INFINITY ? 0.0f : exp2f((m - mx) * c);
+            if (move) m = mx;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= f;
+        }
+        // With nothing above -inf so far, exponents are taken against 0: they are 0.
+        const float mc = m == -INFINITY ? 0.0f : m * c;
+        float l4[4] = {l, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                float p[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int k = 8 * u + i;
+                    p[i] = __builtin_amdgcn_exp2f(fmaf(s[kb][k], c, -mc));
+                    if constexpr (MASKED) p[i] = (see[kb] >> (8 * (k / 4) + k % 4)) & 1 ? p[i] : 0.0f;
+                    l4[i % 4] += p[i];
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) pw[2 * kb + u][i] = pack_bf16(p[2 * i], p[2 * i + 1]);
+            }
+        l = (l4[0] + l4[1]) + (l4[2] + l4[3]);
+        // Formed here, not where they are used: that may be behind a barrier.
+#pragma unroll
+        for (int i = 0; i < 2 * KB; ++i) asm volatile("" : "+v"(pw[i]));
+    };
+    // V^T of the 16 rows from 32 kb + 16 u as the matrix cores take it. Lane: dimensions
+    // 4 (l % 4) .. + 3 of a row, from the 16 at 32 d + 16 (l / 16 % 2).
+    auto value_frag = [&](const uint8_t *vs, int kb, int u, int d) __attribute__((always_inline)) {
+        const uint32_t row = 32 * kb + 16 * u + 4 * h + (lane & 15) / 4;
+        const uint32_t dim = 32 * d + (lane & 16) + 4 * (lane & 3), in = 2 * (dim & 7), ch = dim / 8;
+        const u32x2 v0 = read_tr(vs + row * ROWB + value_slot(row, ch) * 16 + in);
+        const u32x2 v1 = read_tr(vs + (row + 8) * ROWB + value_slot(row + 8, ch) * 16 + in);
+        return u32x4{v0.x, v0.y, v1.x, v1.y};
+    };
+    // A run of matrix products in the order written, each one's operand read from LDS AHEAD
+    // products before it is used: the values of a tile (VALUES) and the scores of another.
+    auto run = [&](auto values_c, auto scores_c, const uint8_t *vs, const uint8_t *ks) __attribute__((always_inline)) {
+        constexpr int NV = decltype(values_c)::value ? 2 * KB * DB : 0, NK = decltype(scores_c)::value ? KB * HD / 16 : 0;
+        constexpr int N = NV + NK;
+        auto read = [&](int p) __attribute__((always_inline)) {
+            return p < NV ? value_frag(vs, p / DB / 2, p / DB % 2, p % DB) : key_frag(ks, (p - NV) % KB, (p - NV) / KB);
+        };
+        u32x4 f[AHEAD];
+#pragma unroll
+        for (int p = 0; p < AHEAD && p < N; ++p) f[p] = read(p);
+#pragma unroll
+        for (int p = 0; p < N; ++p) {
+            const bf16x8 x = __builtin_bit_cast(bf16x8, f[p % AHEAD]);
+            if (p < NV) {
+                o[p % DB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, __builtin_bit_cast(bf16x8, pw[p / DB]), o[p % DB],
+                                                                    0, 0, 0);
+            } else {
+                const int kb = (p - NV) % KB, st = (p - NV) / KB;
+                s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, qf[st], st ? s[kb] : zero, 0, 0, 0);
+            }
+            if (p + AHEAD < N) f[p % AHEAD] = read(p + AHEAD);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    const std::true_type yes{};
+    const std::false_type no{};
+    // Every LDS access of this wave is done before another wave reads or writes there.
+    auto barrier = [&] {
+        pipe::wait_lgkm0();
+        pipe::lds_barrier();
+    };
+    // The first `whole` steps' tiles lie within the context; the others look at the mask, in
+    // a loop of their own, whose registers the first does not pay for.
+    const uint32_t in = min(n, max(a.len / TK, t0) - t0), whole = in / KW;
+    auto masked_step = [&](uint32_t step, uint32_t next) __attribute__((always_inline)) {
+        barrier();   // the tile is written, and every wave is done with the slot before
+        if (has(next)) {
+            put(next);
+            fetch(next + 1);
+        }
+        if (!has(step)) return;
+        run(no, yes, nullptr, keys(step));
+        weights(yes, tile_row(step));
+        run(yes, no, keys(step) + T::TILE, nullptr);
+    };
+    if constexpr (T::TURNS) {
+        // The waves' two halves, one of each on a SIMD, take turns: while one half runs its
+        // matrix products (a tile's values, the next tile's scores), the other half's weights and
+        // its share of a later tile use the vector unit. A phase ends at a barrier; the
+        // second half runs one phase behind. Tile i's scores are formed in phases 2 i and 2 i + 1
+        // and its values used in phases 2 i + 2 and 2 i + 3, so with four slots the first half
+        // may write tile i + 2 in phase 2 i + 1, the second tile i + 3 in phase 2 i + 2.
+        const bool second = wave >= T::W / 2;
+        const uint32_t far = second ? 3 : 2;
+        if (n) fetch(0);
+#pragma unroll
+        for (uint32_t i = 0; i < 3; ++i)
+            if (i < far && has(i)) {
+                put(i);
+                fetch(i + 1);
+            }
+        if (whole) {
+            barrier();
+            if (second) barrier();
+            run(no, yes, nullptr, keys(0));
+            for (uint32_t i = 0; i < whole; ++i) {
+                barrier();
+                if (has(i + far)) {
+                    put(i + far);
+                    fetch(i + far + 1);
+                }
+                weights(no, 0);
+                barrier();
+                // Behind the last tile these scores are not used.
+                run(yes, yes, keys(i) + T::TILE, keys(i + 1));
+            }
+            if (!second) barrier();
+        }
+        for (uint32_t i = whole; i < steps; ++i) masked_step(i, i + far);
+    } else {
+        if (has(0)) {
+            fetch(0);
+            put(0);
+            fetch(1);
+        }
+        uint32_t step = 0;
+        for (; step < whole; ++step) {
+            barrier();
+            if (has(step + 1)) {
+                put(step + 1);
+                fetch(step + 2);
+            }
+            run(no, yes, nullptr, keys(step));
+            weights(no, 0);
+            run(yes, no, keys(step) + T::TILE, nullptr);
+        }
+        for (; step < steps; ++step) masked_step(step, step + 1);
+    }
+    l = both_sum(l);
+    float mc = m == -INFINITY ? -INFINITY : m * c;
+
+    if constexpr (KW > 1) {
+        // The other key groups' (o, m, l) through LDS, lane by lane.
+        __syncthreads();
+        float *buf = reinterpret_cast<float *>(lds);
+        constexpr int PW = T::PW;
+        if (kg > 0) {
+            float *w = buf + ((kg - 1) * RW + rw) * PW;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<f32x4 *>(w + (d * 4 + i) * 256 + lane * 4) =
+                        f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+            w[DB * 1024 + lane] = mc;
+            w[DB * 1024 + 64 + lane] = l;
+        }
+        __syncthreads();
+        if (kg > 0) return;
+        float top = mc;
+#pragma unroll
+        for (int k = 0; k < KW - 1; ++k) top = fmaxf(top, buf[(k * RW + rw) * PW + DB * 1024 + lane]);
+        const float at = top == -INFINITY ? 0.0f : top;
+        float f = exp2f(mc - at);
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] *= f;
+#pragma unroll
+        for (int k = 0; k < KW - 1; ++k) {
+            const float *w = buf + (k * RW + rw) * PW;
+            f = exp2f(w[DB * 1024 + lane] - at);
+            l += w[DB * 1024 + 64 + lane] * f;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 v = *reinterpret_cast<const f32x4 *>(w + (d * 4 + i) * 256 + lane * 4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[d][4 * i + e] += v[e] * f;
+                }
+        }
+        mc = top;
+    }
+    if (r0 >= R) return;
+    // A lane has dimensions 32 d + 8 i + 4 h .. + 3 of its row.
+    if (a.part) {
+        const size_t at_row = ((size_t)split * a.nkv + g) * R + r0;
+        float *w = a.part + at_row * HD, *mlp = a.part + (size_t)a.splits * a.nkv * R * HD + 2 * at_row;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<f32x4 *>(w + 32 * d + 8 * i + 4 * h) =
+                    f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+        if (h == 0) mlp[0] = mc, mlp[1] = l;
+        return;
+    }
+    const bool any = l != 0.0f || sees_any(a, tok);
+    uint16_t *out = a.out + qrow * a.hd;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t dim = 32 * d + 8 * i + 4 * h;
+            if (dim < a.hd)
+                *reinterpret_cast<u32x2 *>(out + dim) =
+                    finish(f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]}, l, any);
+        }
+}
+
 // Merges the splits' (o, m, l): a thread takes four dimensions of a query row, GR threads its
 // splits in turn.
 template <int HD, int GR>
@@ -371,13 +758,8 @@ __global__ __launch_bounds__(256) void attention_mxfp4_merge(const MxAttn a) {
     *reinterpret_cast<u32x2 *>(a.out + ((size_t)tok * a.nh + g * per + r % per) * a.hd + 4 * quad) = finish(o, l, any);
 }
 
-template <int HD, int QT>
-int launch(const MxAttn &a, hipStream_t st) {
-    constexpr int LDS = MXA_WAVES * MXA_TILE * 2 * HD;
-    static_assert(LDS <= 160 * 1024, "LDS");
-    const unsigned grid = (a.units + MXA_XCDS - 1) / MXA_XCDS * MXA_XCDS * a.row_blocks;
-    hipLaunchKernelGGL((attention_mxfp4<HD, QT>), dim3(grid), dim3(64 * MXA_WAVES), LDS, st, a);
-    if (int rc = check_launch("attention_mxfp4")) return rc;
+template <int HD>
+int launch_merge(const MxAttn &a, hipStream_t st) {
     if (a.splits < 2) return RENG_HIP_OK;
     const uint32_t rows = a.tokens * a.nh;
     constexpr int GR = 256 / (HD / 4);
@@ -386,6 +768,46 @@ int launch(const MxAttn &a, hipStream_t st) {
     else
         hipLaunchKernelGGL((attention_mxfp4_merge<HD, 1>), dim3((rows + GR - 1) / GR), dim3(256), 0, st, a);
     return check_launch("attention_mxfp4_merge");
+}
+
+unsigned grid_of(const MxAttn &a) { return (a.units + MXA_XCDS - 1) / MXA_XCDS * MXA_XCDS * a.row_blocks; }
+
+template <int HD, int QT>
+int launch_rows(const MxAttn &a, hipStream_t st) {
+    constexpr int LDS = MXA_WAVES * MXA_TILE * 2 * HD;
+    static_assert(LDS <= 160 * 1024, "LDS");
+    hipLaunchKernelGGL((attention_mxfp4<HD, QT>), dim3(grid_of(a)), dim3(64 * MXA_WAVES), LDS, st, a);
+    if (int rc = check_launch("attention_mxfp4")) return rc;
+    return launch_merge<HD>(a, st);
+}
+
+template <int HD, int RW, int KW, int TK, int S>
+int launch_tiles(const MxAttn &a, hipStream_t st) {
+    using T = MxShape<HD, RW, KW, TK, S>;
+    hipLaunchKernelGGL((attention_mxfp4_tiles<HD, RW, KW, TK, S>), dim3(grid_of(a)), dim3(64 * T::W), T::LDS, st, a);
+    if (int rc = check_launch("attention_mxfp4_tiles")) return rc;
+    return launch_merge<HD>(a, st);
+}
+
+template <int HD>
+int launch_form(const MxAttn &a, int form, hipStream_t st) {
+    if constexpr (HD == 256) {
+        switch (form) {
+        case MXA_ROWS_16: return launch_rows<HD, 1>(a, st);
+        case MXA_ROWS_32: return launch_rows<HD, 2>(a, st);
+        case MXA_TILES_64: return launch_tiles<HD, 2, 2, 32, 2>(a, st);
+        default: return launch_tiles<HD, 4, 1, 32, 2>(a, st);
+        }
+    } else {
+        switch (form) {
+        case MXA_ROWS_16: return launch_rows<HD, 1>(a, st);
+        case MXA_ROWS_32: return launch_rows<HD, 2>(a, st);
+        case MXA_ROWS_64: return launch_rows<HD, 4>(a, st);
+        case MXA_TILES_64: return launch_tiles<HD, 2, 4, 32, 2>(a, st);
+        case MXA_TILES_128: return launch_tiles<HD, 4, 2, 32, 2>(a, st);
+        default: return launch_tiles<HD, 8, 1, 64, 4>(a, st);
+        }
+    }
 }
 
 }  // namespace
@@ -448,7 +870,6 @@ RENG_HIP_API int reng_hip_attention_mxfp4(const uint16_t *q, const reng_hip_mx_c
                    p.tiles % p.splits,
                    p.splits > 1 ? static_cast<float *>(workspace) : nullptr};
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (p.hdp == 256) return p.qt == 1 ? launch<256, 1>(a, st) : launch<256, 2>(a, st);
-    if (p.hdp == 128) return p.qt == 1 ? launch<128, 1>(a, st) : p.qt == 2 ? launch<128, 2>(a, st) : launch<128, 4>(a, st);
-    return p.qt == 1 ? launch<64, 1>(a, st) : p.qt == 2 ? launch<64, 2>(a, st) : launch<64, 4>(a, st);
+    if (p.hdp == 256) return launch_form<256>(a, p.form, st);
+    return p.hdp == 128 ? launch_form<128>(a, p.form, st) : launch_form<64>(a, p.form, st);
 }

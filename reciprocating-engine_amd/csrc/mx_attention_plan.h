@@ -10,39 +10,59 @@ namespace reng {
 
 constexpr uint32_t MXA_XCDS = 8, MXA_WAVES = 4, MXA_TILE = 32, MXA_SPLIT_MAX = 64;
 
-// Workgroups of a split cache, at most: their partials are 64 rows of at most 256 values each.
-constexpr size_t MXA_PART_UNITS = 1024;
+// Waves with query rows of their own (16, 32 or 64), four of which share a split's tiles; or
+// workgroups of 64, 128 or 256 query rows that share tiles in LDS.
+enum MxAttnForm { MXA_ROWS_16, MXA_ROWS_32, MXA_ROWS_64, MXA_TILES_64, MXA_TILES_128, MXA_TILES_256, MXA_FORMS };
+
+// Query rows of a workgroup, cache rows of a tile, and how many tiles it takes at a time.
+struct MxAttnShape {
+    uint32_t rows, tile, groups;
+};
+constexpr MxAttnShape MXA_SHAPES[MXA_FORMS] = {{16, 32, 4}, {32, 32, 4}, {64, 32, 4}, {64, 32, 4}, {128, 32, 2}, {256, 64, 1}};
+constexpr MxAttnShape MXA_SHAPES_256[MXA_FORMS] = {{16, 32, 4}, {32, 32, 4}, {0, 0, 0}, {64, 32, 2}, {128, 32, 1}, {0, 0, 0}};
+
+inline MxAttnShape mxa_shape(uint32_t hdp, int form) { return hdp == 256 ? MXA_SHAPES_256[form] : MXA_SHAPES[form]; }
+
+// Workgroups of a split cache, at most.
+constexpr size_t MXA_PART_UNITS = 1024, MXA_PART_ROWS = 64;
 
 struct MxAttnPlan {
     uint32_t hdp;           // the head size the kernel is built for: 64, 128 or 256
-    uint32_t qt;            // 16-row query tiles of a wave
+    int form;
     uint32_t row_blocks;    // per key/value head
     uint32_t splits, tiles; // of the cache, and all its tiles
 };
 
 inline uint32_t mxa_head(size_t hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 
-// Query tiles of a wave: as many as its rows ask for, four at most (two of 256 dimensions).
-inline uint32_t mxa_tiles(size_t rows, uint32_t hdp) {
-    if (rows <= 16) return 1;
-    return rows <= 32 || hdp == 256 ? 2 : 4;
+inline int mxa_form(size_t rows, uint32_t hdp) {
+    if (rows <= 16) return MXA_ROWS_16;
+    if (rows <= 32) return MXA_ROWS_32;
+    if (rows <= 64) return MXA_TILES_64;
+    return rows <= 128 || hdp == 256 ? MXA_TILES_128 : MXA_TILES_256;
 }
 
-inline MxAttnPlan mxa_plan(size_t nh, size_t nkv, size_t hd, size_t len, size_t tokens, size_t cus) {
+inline MxAttnPlan mxa_plan_of(int form, size_t nh, size_t nkv, size_t hd, size_t len, size_t tokens, size_t cus) {
     MxAttnPlan p{};
     p.hdp = mxa_head(hd);
     const size_t rows = tokens * (nh / nkv), cache = len + tokens;
-    p.qt = mxa_tiles(rows, p.hdp);
-    const size_t blocks = (rows + 16 * p.qt - 1) / (16 * p.qt), tiles = (cache + MXA_TILE - 1) / MXA_TILE;
+    p.form = form;
+    const MxAttnShape s = mxa_shape(p.hdp, form);
+    const size_t blocks = (rows + s.rows - 1) / s.rows, tiles = (cache + s.tile - 1) / s.tile;
     p.row_blocks = (uint32_t)blocks;
     p.tiles = (uint32_t)tiles;
-    // Two workgroups a CU, each wave with a tile or more.
-    const size_t units = nkv * blocks, want = 2 * cus / units, most = tiles / MXA_WAVES;
-    size_t s = want < most ? want : most;
-    if (s > MXA_SPLIT_MAX) s = MXA_SPLIT_MAX;
-    if (s * units > MXA_PART_UNITS) s = MXA_PART_UNITS / units;
-    p.splits = (uint32_t)(s < 1 ? 1 : s);
+    // Two workgroups of four waves a CU, or one of eight, and every group of waves with a tile or more.
+    const size_t units = nkv * blocks, want = (form <= MXA_ROWS_64 ? 2 : 1) * cus / units, most = cache / 128;
+    size_t n = want < most ? want : most;
+    if (n > MXA_SPLIT_MAX) n = MXA_SPLIT_MAX;
+    if (n > tiles) n = tiles;
+    if (n * nkv * rows > MXA_PART_UNITS * MXA_PART_ROWS) n = MXA_PART_UNITS * MXA_PART_ROWS / (nkv * rows);
+    p.splits = (uint32_t)(n < 1 ? 1 : n);
     return p;
+}
+
+inline MxAttnPlan mxa_plan(size_t nh, size_t nkv, size_t hd, size_t len, size_t tokens, size_t cus) {
+    return mxa_plan_of(mxa_form(tokens * (nh / nkv), mxa_head(hd)), nh, nkv, hd, len, tokens, cus);
 }
 
 // A split leaves for each query row its unnormalised outputs, its maximum and its sum.
@@ -51,17 +71,14 @@ inline size_t mxa_part_bytes(const MxAttnPlan &p, size_t nkv, size_t rows) {
 }
 
 // No less than mxa_part_bytes asks for over 1 .. tokens tokens and 0 .. len context rows:
-// splits are at most a tile a wave, and splits times row blocks at most MXA_PART_UNITS.
+// splits are of 128 cache rows or more, and splits times query rows at most 2^16.
 inline size_t mxa_workspace(size_t nh, size_t nkv, size_t hd, size_t len, size_t tokens) {
-    const size_t tiles = (len + tokens + MXA_TILE - 1) / MXA_TILE;
-    size_t splits = tiles / MXA_WAVES;
+    size_t splits = (len + tokens) / 128;
     if (splits > MXA_SPLIT_MAX) splits = MXA_SPLIT_MAX;
     if (splits < 2) return 0;
-    const uint32_t hdp = mxa_head(hd);
     size_t rows = splits * nkv * tokens * (nh / nkv);
-    const size_t most = MXA_PART_UNITS * 16 * (hdp == 256 ? 2 : 4);
-    if (rows > most) rows = most;
-    return rows * (hdp + 2) * sizeof(float);
+    if (rows > MXA_PART_UNITS * MXA_PART_ROWS) rows = MXA_PART_UNITS * MXA_PART_ROWS;
+    return rows * (mxa_head(hd) + 2) * sizeof(float);
 }
 
 }  // namespace reng

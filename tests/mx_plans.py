@@ -11,8 +11,11 @@ SOURCE = """
 using namespace reng;
 extern "C" void plan(size_t nh, size_t nkv, size_t hd, size_t len, size_t tokens, size_t cus, uint64_t *out) {
     const MxAttnPlan p = mxa_plan(nh, nkv, hd, len, tokens, cus);
-    const uint64_t v[] = {p.hdp, p.qt, p.row_blocks, p.splits, p.tiles, mxa_part_bytes(p, nkv, tokens * (nh / nkv))};
+    const uint64_t v[] = {p.hdp, (uint64_t)p.form, p.row_blocks, p.splits, p.tiles, mxa_part_bytes(p, nkv, tokens * (nh / nkv))};
     for (int i = 0; i < 6; ++i) out[i] = v[i];
+}
+extern "C" void shape(uint32_t hdp, int form, uint32_t *out) {
+    out[0] = mxa_shape(hdp, form).rows, out[1] = mxa_shape(hdp, form).tile;
 }
 """
 _lib = None
@@ -35,4 +38,11 @@ def lib():
 def mx_attention_plan(nh, nkv, hd, length, tokens, cus=CUS):
     out = (ctypes.c_uint64 * 6)()
     lib().plan(nh, nkv, hd, length, tokens, cus, out)
-    return dict(zip(("hdp", "qt", "row_blocks", "splits", "tiles", "bytes"), out))
+    return dict(zip(("hdp", "form", "row_blocks", "splits", "tiles", "bytes"), out))
+
+
+def shape(hdp, form):
+    """Query rows of a workgroup and cache rows of a tile."""
+    out = (ctypes.c_uint32 * 2)()
+    lib().shape(hdp, form, out)
+    return tuple(out)

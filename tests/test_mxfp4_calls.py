@@ -171,14 +171,14 @@ def test_plans_cover_the_cache_within_the_workspace():
         p = D.mx_attention_plan(heads, kv, hd, length, tokens)
         rows, cache_rows = tokens * heads // kv, length + tokens
         assert p["hdp"] >= hd and p["hdp"] in (64, 128, 256)
-        assert p["qt"] in ((1, 2) if p["hdp"] == 256 else (1, 2, 4))
-        assert (p["row_blocks"] - 1) * 16 * p["qt"] < rows <= p["row_blocks"] * 16 * p["qt"]
-        assert p["tiles"] * 32 >= cache_rows > (p["tiles"] - 1) * 32
+        block, tile = D.shape(p["hdp"], p["form"])
+        assert block > 0 and (p["row_blocks"] - 1) * block < rows <= p["row_blocks"] * block
+        assert p["tiles"] * tile >= cache_rows > (p["tiles"] - 1) * tile
         assert 1 <= p["splits"] <= 64 and p["splits"] <= p["tiles"]
         need = R.attention_mxfp4_workspace_bytes(heads, kv, hd, length, tokens)
         assert p["bytes"] <= need <= 70 << 20, (p, need)
         # A workspace for the longest call serves the shorter ones.
         less = D.mx_attention_plan(heads, kv, hd, rng.randint(0, length), rng.randint(1, tokens))
         assert less["bytes"] <= need
-        seen.add((p["hdp"], p["qt"], p["splits"] > 1))
-    assert len(seen) >= 14
+        seen.add((p["hdp"], p["form"], p["splits"] > 1))
+    assert len(seen) >= 2 * (5 + 5 + 4), seen
