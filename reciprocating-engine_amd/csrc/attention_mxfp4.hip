@@ -113,6 +113,13 @@ __device__ __forceinline__ u32x2 finish(const f32x4 &o, float l, bool any) {
     return u32x2{pack_bf16(o.x * r, o.y * r), pack_bf16(o.z * r, o.w * r)};
 }
 
+// The rows of a head as a buffer: what lies behind them reads as zeros. (A scalar offset would not
+// count in that: the whole offset is the lane's.)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const uint8_t *p, size_t head, uint32_t rows, uint32_t pitch) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(p) + head * pitch, 0, rows * pitch, 0x00020000);
+}
+constexpr uint32_t NOTHING = 0x7fffffffu;   // past every buffer
+
 // The slot of 16-byte chunk c of a tile's row r. Eight consecutive rows written at one chunk
 // and four read over two chunks lie in different slots.
 __device__ __forceinline__ uint32_t value_slot(uint32_t r, uint32_t c) {
@@ -171,25 +178,37 @@ __global__ __launch_bounds__(64 * MXA_WAVES) void attention_mxfp4(const MxAttn a
         uint32_t w[LB / 4];
         uint32_t s[CH];   // scale bytes
     };
-    // Row j's codes of this lane; zeros past the head's dimensions.
-    auto load = [&](const uint8_t *codes, const uint8_t *scales, uint32_t j) __attribute__((always_inline)) {
-        const size_t row = head + min(j, rows - 1);
-        Codes v;
-        const uint8_t *p = codes + row * rowb + dim0 / 2, *s = scales + row * a.sp + dim0 / 32;
+    // Where this lane's codes of a row lie, chunk by chunk; zeros past the head's dimensions.
+    uint32_t at_codes[CH], at_scale[CH];
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            const bool on = dim0 + 32 * i < a.hd;
-            v.s[i] = on ? s[i] : ONE_BYTE;
-            if constexpr (LB == 8) {
-                const u32x2 x = on ? *reinterpret_cast<const u32x2 *>(p) : u32x2{0u, 0u};
-                v.w[0] = x.x, v.w[1] = x.y;
-            } else {
-                const u32x4 x = on ? reinterpret_cast<const u32x4 *>(p)[i] : u32x4{0u, 0u, 0u, 0u};
+    for (int i = 0; i < CH; ++i) {
+        const bool on = dim0 + 32 * i < a.hd;
+        at_codes[i] = on ? r16 * rowb + dim0 / 2 + 16 * i : NOTHING;
+        at_scale[i] = on ? r16 * a.sp + dim0 / 32 + i : NOTHING;
+    }
+    Codes kn[2], vn[2];   // the next tile's: keys 16 u + l % 16
+    const __amdgpu_buffer_rsrc_t rkc = rows_of(a.kc, head, rows, rowb), rks = rows_of(a.ks, head, rows, a.sp);
+    const __amdgpu_buffer_rsrc_t rvc = rows_of(a.vc, head, rows, rowb), rvs = rows_of(a.vs, head, rows, a.sp);
+    auto fetch = [&](uint32_t tile) __attribute__((always_inline)) {
+        auto load = [&](Codes &v, const __amdgpu_buffer_rsrc_t &rc, const __amdgpu_buffer_rsrc_t &rs, uint32_t j) __attribute__((always_inline)) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v.w[4 * i + e] = x[e];
+            for (int i = 0; i < CH; ++i) {
+                v.s[i] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(rs, at_scale[i] + j * a.sp, 0, 0);
+                if constexpr (LB == 8) {
+                    const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rc, at_codes[i] + j * rowb, 0, 0));
+                    v.w[0] = x.x, v.w[1] = x.y;
+                } else {
+                    const u32x4 x = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rc, at_codes[i] + j * rowb, 0, 0));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v.w[4 * i + e] = x[e];
+                }
             }
+        };
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            load(kn[u], rkc, rks, tile * MXA_TILE + 16 * u);
+            load(vn[u], rvc, rvs, tile * MXA_TILE + 16 * u);
         }
-        return v;
     };
 
     f32x4 o[DT][QT];
@@ -200,14 +219,6 @@ __global__ __launch_bounds__(64 * MXA_WAVES) void attention_mxfp4(const MxAttn a
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d][t] = f32x4{0, 0, 0, 0};
     }
-    Codes kn[2], vn[2];   // the next tile's
-    auto fetch = [&](uint32_t tile) __attribute__((always_inline)) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            kn[u] = load(a.kc, a.ks, tile * MXA_TILE + 16 * u + r16);
-            vn[u] = load(a.vc, a.vs, tile * MXA_TILE + 16 * u + r16);
-        }
-    };
     if (t0 + wave < t1) fetch(t0 + wave);
     for (uint32_t tile = t0 + wave; tile < t1; tile += NW) {
         const uint32_t j0 = tile * MXA_TILE;
@@ -413,24 +424,28 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_mxfp4_tiles(const MxAt
     // A part is 64 blocks of 32 codes: a block a lane, RT rows of keys (the first half of the parts)
     // or values. fetch() reads this wave's parts of a tile, put() writes their values.
     const size_t head = (size_t)g * a.cap;
-    const uint32_t prow = lane % T::RT, blk = lane / T::RT;
+    const uint32_t prow = lane % T::RT, blk = lane / T::RT, rowb = a.hd / 2;
+    const uint32_t at_codes = 32 * blk < a.hd ? prow * rowb + 16 * blk : NOTHING;
+    const uint32_t at_scale = 32 * blk < a.hd ? prow * a.sp + blk : NOTHING;
     u32x4 codes[MINE];
     uint32_t byte[MINE], other[MINE];   // the block's scale; for a key its value's, too
+    __amdgpu_buffer_rsrc_t rc[MINE], rs[MINE];
+    const __amdgpu_buffer_rsrc_t rvs = rows_of(a.vs, head, rows, a.sp);
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+        const bool values = rw + i * RW >= T::PARTS / 2;
+        rc[i] = rows_of(values ? a.vc : a.kc, head, rows, rowb);
+        rs[i] = rows_of(values ? a.vs : a.ks, head, rows, a.sp);
+    }
     auto fetch = [&](uint32_t step) __attribute__((always_inline)) {
-        const uint32_t j0 = min(tile_row(step), rows - 1);
 #pragma unroll
         for (int i = 0; i < MINE; ++i) {
-            const uint32_t part = rw + i * RW, half = T::PARTS / 2;
+            const uint32_t part = rw + i * RW;
             if (part >= T::PARTS) break;
-            const bool values = part >= half;
-            const size_t row = head + min(j0 + (values ? part - half : part) * T::RT + prow, rows - 1);
-            codes[i] = u32x4{0u, 0u, 0u, 0u};
-            byte[i] = other[i] = ONE_BYTE;
-            if (32 * blk < a.hd) {
-                codes[i] = *reinterpret_cast<const u32x4 *>((values ? a.vc : a.kc) + row * (a.hd / 2) + 16 * blk);
-                byte[i] = (values ? a.vs : a.ks)[row * a.sp + blk];
-                if (!values) other[i] = a.vs[row * a.sp + blk];
-            }
+            const uint32_t j = tile_row(step) + part % (T::PARTS / 2) * T::RT;
+            codes[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rc[i], at_codes + j * rowb, 0, 0));
+            byte[i] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(rs[i], at_scale + j * a.sp, 0, 0);
+            other[i] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(rvs, at_scale + j * a.sp, 0, 0);
         }
     };
     auto put = [&](uint32_t step) __attribute__((always_inline)) {

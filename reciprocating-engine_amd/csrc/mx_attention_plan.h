@@ -23,8 +23,8 @@ constexpr MxAttnShape MXA_SHAPES_256[MXA_FORMS] = {{16, 32, 4}, {32, 32, 4}, {0,
 
 inline MxAttnShape mxa_shape(uint32_t hdp, int form) { return hdp == 256 ? MXA_SHAPES_256[form] : MXA_SHAPES[form]; }
 
-// Workgroups of a split cache, at most.
-constexpr size_t MXA_PART_UNITS = 1024, MXA_PART_ROWS = 64;
+// Query rows that splits leave, at most (68 MB of 128 dimensions).
+constexpr size_t MXA_PART_ROWS = 1 << 17;
 
 struct MxAttnPlan {
     uint32_t hdp;           // the head size the kernel is built for: 64, 128 or 256
@@ -56,7 +56,7 @@ inline MxAttnPlan mxa_plan_of(int form, size_t nh, size_t nkv, size_t hd, size_t
     size_t n = want < most ? want : most;
     if (n > MXA_SPLIT_MAX) n = MXA_SPLIT_MAX;
     if (n > tiles) n = tiles;
-    if (n * nkv * rows > MXA_PART_UNITS * MXA_PART_ROWS) n = MXA_PART_UNITS * MXA_PART_ROWS / (nkv * rows);
+    if (n * nkv * rows > MXA_PART_ROWS) n = MXA_PART_ROWS / (nkv * rows);
     p.splits = (uint32_t)(n < 1 ? 1 : n);
     return p;
 }
@@ -71,13 +71,13 @@ inline size_t mxa_part_bytes(const MxAttnPlan &p, size_t nkv, size_t rows) {
 }
 
 // No less than mxa_part_bytes asks for over 1 .. tokens tokens and 0 .. len context rows:
-// splits are of 128 cache rows or more, and splits times query rows at most 2^16.
+// splits are of 128 cache rows or more, and splits times query rows at most 2^17.
 inline size_t mxa_workspace(size_t nh, size_t nkv, size_t hd, size_t len, size_t tokens) {
     size_t splits = (len + tokens) / 128;
     if (splits > MXA_SPLIT_MAX) splits = MXA_SPLIT_MAX;
     if (splits < 2) return 0;
     size_t rows = splits * nkv * tokens * (nh / nkv);
-    if (rows > MXA_PART_UNITS * MXA_PART_ROWS) rows = MXA_PART_UNITS * MXA_PART_ROWS;
+    if (rows > MXA_PART_ROWS) rows = MXA_PART_ROWS;
     return rows * (mxa_head(hd) + 2) * sizeof(float);
 }
 
