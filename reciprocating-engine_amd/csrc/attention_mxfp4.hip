@@ -9,11 +9,11 @@
 // rounded on the way to the matrix cores.
 //
 // The query rows of a key/value head (row r: token r / per, query head r % per of the per
-// that share it) go 16 to a tile and QT tiles to a wave; the four waves of a workgroup take
-// tiles of 32 cache rows in turn, and merge in LDS; splits of the cache merge in a second
-// kernel (mx_attention_plan.h). A wave needs nothing of the others until then.
+// that share it) go 16 to a wave, eight waves taking tiles of 32 cache rows of their own in turn, or, where there are many,
+// 32 to a wave over tiles that a workgroup shares in LDS. Splits of the cache merge in a
+// second kernel (mx_attention_plan.h).
 //
-// Per tile a wave forms S^T = K Q^T on v_mfma_f32_16x16x32_bf16. Lane l has key l % 16 and,
+// Few rows: per tile a wave forms S^T = K Q^T on v_mfma_f32_16x16x32_bf16. Lane l has key l % 16 and,
 // of its dimensions, the quarter l / 16: the order in which dimensions are summed is free, so
 // a lane's codes are consecutive bytes and lie under one scale (two of 256 dimensions), and the
 // queries' registers follow that order. The results have query l % 16 and four keys from
@@ -126,9 +126,13 @@ __device__ __forceinline__ uint32_t value_slot(uint32_t r, uint32_t c) {
     return c ^ (((r & 3) << 1) | ((r >> 2) & 1));
 }
 
-template <int HD, int QT>
-__global__ __launch_bounds__(64 * MXA_WAVES) void attention_mxfp4(const MxAttn a) {
-    constexpr int NW = MXA_WAVES, ST = HD / 32, DT = HD / 16;   // products a score; tiles of dimensions
+// ------------------------------------------------------------ few query rows
+//
+// NW waves, each with the same 16 query rows and tiles of its own, whose codes are on the way while the
+// one before is worked on.
+template <int HD, int NW>
+__global__ __launch_bounds__(64 * NW) void attention_mxfp4(const MxAttn a) {
+    constexpr int ST = HD / 32, DT = HD / 16;   // products a score; tiles of dimensions
     constexpr int LB = HD / 8, CH = LB <= 16 ? 1 : LB / 16;     // bytes of a lane; 16-byte chunks of them
     constexpr int ROWB = 2 * HD, VBUF = MXA_TILE * ROWB;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
@@ -144,31 +148,26 @@ __global__ __launch_bounds__(64 * MXA_WAVES) void attention_mxfp4(const MxAttn a
     const uint32_t per = a.nh / a.nkv, R = a.tokens * per, rows = a.len + a.tokens;
     uint8_t *vbuf = lds + wave * VBUF;
 
-    // This lane's query rows (clamped: rows past the last are not stored).
+    // This lane's query row (clamped: rows past the last are not stored).
     // scale < 0 goes into the queries' signs, so that the largest product is the largest score.
     const float c = fabsf(a.scale) * 1.44269504088896341f;
     const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
-    uint32_t tok[QT];
-    u32x4 qf[QT][ST];
     const uint32_t dim0 = q4 * (HD / 4);   // this lane's dimensions
+    const uint32_t r0 = rb * 16 + r16, r = min(r0, R - 1), tok = r / per;
+    const size_t qrow = (size_t)tok * a.nh + g * per + r % per;
+    bf16x8 qf[ST];
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-        const uint32_t r = min((rb * QT + t) * 16 + r16, R - 1);
-        tok[t] = r / per;
-        const uint16_t *qr = a.q + ((size_t)tok[t] * a.nh + g * per + r % per) * a.hd;
-#pragma unroll
-        for (int s = 0; s < ST; ++s) {
-            u32x4 v{0u, 0u, 0u, 0u};
-            if (dim0 + 8 * s < a.hd) v = *reinterpret_cast<const u32x4 *>(qr + dim0 + 8 * s);
-            qf[t][s] = v ^ flip;
-        }
+    for (int e = 0; e < ST; ++e) {
+        u32x4 v{0u, 0u, 0u, 0u};
+        if (dim0 + 8 * e < a.hd) v = *reinterpret_cast<const u32x4 *>(a.q + qrow * a.hd + dim0 + 8 * e);
+        qf[e] = __builtin_bit_cast(bf16x8, v ^ flip);
     }
 
     // The split's tiles, cut for a chain at the last row its tokens see.
     const uint32_t t0 = split * a.base + min(split, a.more);
     uint32_t t1 = t0 + a.base + (split < a.more);
     if (!a.mask) {
-        const uint32_t last = min((rb * QT + QT) * 16 - 1, R - 1) / per;
+        const uint32_t last = min(rb * 16 + 15, R - 1) / per;
         t1 = min(t1, (a.len + last) / MXA_TILE + 1);
     }
 
@@ -211,18 +210,14 @@ __global__ __launch_bounds__(64 * MXA_WAVES) void attention_mxfp4(const MxAttn a
         }
     };
 
-    f32x4 o[DT][QT];
-    float m[QT], l[QT];   // the running maximum of the products, this lane's share of the sum
+    f32x4 o[DT];
+    float m = -INFINITY, l = 0.0f;   // the running maximum of the products, this lane's share of the sum
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-        m[t] = -INFINITY, l[t] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[d][t] = f32x4{0, 0, 0, 0};
-    }
+    for (int d = 0; d < DT; ++d) o[d] = f32x4{0, 0, 0, 0};
     if (t0 + wave < t1) fetch(t0 + wave);
     for (uint32_t tile = t0 + wave; tile < t1; tile += NW) {
         const uint32_t j0 = tile * MXA_TILE;
-        f32x4 s[2][QT];
+        f32x4 s[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {   // keys 16 u ..
             Codes k = kn[u], v = vn[u];
@@ -237,54 +232,47 @@ __global__ __launch_bounds__(64 * MXA_WAVES) void attention_mxfp4(const MxAttn a
             for (int e = 0; e < ST; ++e)
                 *reinterpret_cast<u32x4 *>(vbuf + row * ROWB + 16 * value_slot(row, dim0 / 8 + e)) =
                     decode8(v.w[e], scale_operand(v.s[e * CH / ST]));
-#pragma unroll
-            for (int t = 0; t < QT; ++t) s[u][t] = f32x4{0, 0, 0, 0};
+            s[u] = f32x4{0, 0, 0, 0};
 #pragma unroll
             for (int e = 0; e < ST; ++e) {
                 const bf16x8 kf = __builtin_bit_cast(bf16x8, decode8(k.w[e], scale_operand(k.s[e * CH / ST])));
-#pragma unroll
-                for (int t = 0; t < QT; ++t)
-                    s[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, __builtin_bit_cast(bf16x8, qf[t][e]), s[u][t], 0, 0, 0);
+                s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[e], s[u], 0, 0, 0);
             }
         }
-        fetch(min(tile + NW, t1 - 1));
+        if (tile + NW < t1) fetch(tile + NW);
         asm volatile("" ::: "memory");   // the values are read by other lanes than wrote them, in the wave's own order
         const bool masked = j0 + MXA_TILE > a.len;
-        u32x4 pw[QT];
+        uint32_t see = 0xffffffffu;
+        if (masked) {
+            see = seen_bits(a, tok, j0) >> (4 * q4);
 #pragma unroll
-        for (int t = 0; t < QT; ++t) {
-            uint32_t see = 0xffffffffu;
-            if (masked) {
-                see = seen_bits(a, tok[t], j0) >> (4 * q4);
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (!((see >> (16 * (i / 4) + i % 4)) & 1)) s[i / 4][t][i % 4] = -INFINITY;
-            }
-            float mx = fmaxf(fmaxf(fmaxf(s[0][t][0], s[0][t][1]), fmaxf(s[0][t][2], s[0][t][3])),
-                             fmaxf(fmaxf(s[1][t][0], s[1][t][1]), fmaxf(s[1][t][2], s[1][t][3])));
-            // The maximum moves, and what is summed so far is scaled down, only where a
-            // score passes it by more than 2^8: weights up to 256 lose nothing in f32 or bf16.
-            if (__builtin_amdgcn_ballot_w64((mx - m[t]) * c > 8.0f || (m[t] == -INFINITY && mx > m[t]))) {
-                mx = query_max(mx);
-                const bool move = (mx - m[t]) * c > 8.0f || (m[t] == -INFINITY && mx > m[t]);
-                const float f = !move ? 1.0f : m[t] == -INFINITY ? 0.0f : exp2f((m[t] - mx) * c);
-                if (move) m[t] = mx;
-                l[t] *= f;
-#pragma unroll
-                for (int d = 0; d < DT; ++d) o[d][t] *= f;
-            }
-            // With nothing above -inf so far, exponents are taken against 0: they are 0.
-            const float mc = m[t] == -INFINITY ? 0.0f : m[t] * c;
-            float p[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                p[i] = __builtin_amdgcn_exp2f(fmaf(s[i / 4][t][i % 4], c, -mc));
-                if (masked) p[i] = (see >> (16 * (i / 4) + i % 4)) & 1 ? p[i] : 0.0f;
-                l[t] += p[i];
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) pw[t][i] = pack_bf16(p[2 * i], p[2 * i + 1]);
+            for (int i = 0; i < 8; ++i)
+                if (!((see >> (16 * (i / 4) + i % 4)) & 1)) s[i / 4][i % 4] = -INFINITY;
         }
+        float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                         fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        // The maximum moves, and what is summed so far is scaled down, only where a
+        // score passes it by more than 2^8: weights up to 256 lose nothing in f32 or bf16.
+        if (__builtin_amdgcn_ballot_w64((mx - m) * c > 8.0f || (m == -INFINITY && mx > m))) {
+            mx = query_max(mx);
+            const bool move = (mx - m) * c > 8.0f || (m == -INFINITY && mx > m);
+            const float f = !move ? 1.0f : m == -INFINITY ? 0.0f : exp2f((m - mx) * c);
+            if (move) m = mx;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[d] *= f;
+        }
+        // With nothing above -inf so far, exponents are taken against 0: they are 0.
+        const float mc = m == -INFINITY ? 0.0f : m * c;
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(fmaf(s[i / 4][i % 4], c, -mc));
+            if (masked) p[i] = (see >> (16 * (i / 4) + i % 4)) & 1 ? p[i] : 0.0f;
+            l += p[i];
+        }
+        const bf16x8 pw = __builtin_bit_cast(bf16x8, u32x4{pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]),
+                                                           pack_bf16(p[4], p[5]), pack_bf16(p[6], p[7])});
         // V^T of the tile's rows in the order of the weights. Lane: dimensions 4 (l % 4) .. + 3 of a row.
         const uint32_t row = 4 * q4 + r16 / 4;
 #pragma unroll
@@ -293,56 +281,48 @@ __global__ __launch_bounds__(64 * MXA_WAVES) void attention_mxfp4(const MxAttn a
             const u32x2 v0 = read_tr(vbuf + row * ROWB + 16 * value_slot(row, ch) + in);
             const u32x2 v1 = read_tr(vbuf + (row + 16) * ROWB + 16 * value_slot(row + 16, ch) + in);
             const bf16x8 vf = __builtin_bit_cast(bf16x8, u32x4{v0.x, v0.y, v1.x, v1.y});
-#pragma unroll
-            for (int t = 0; t < QT; ++t)
-                o[d][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, __builtin_bit_cast(bf16x8, pw[t]), o[d][t], 0, 0, 0);
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pw, o[d], 0, 0, 0);
         }
         asm volatile("" ::: "memory");
     }
 
-    // The waves' (o, m, l) through LDS, a query tile at a time: a wave merges a quarter of its dimensions.
-    constexpr int MD = DT / NW;
+    // The waves' (o, m, l) through LDS, the dimensions' tiles merged by the waves in turn.
+    constexpr int MD = (DT + NW - 1) / NW;
+    __syncthreads();
+    const float sum = query_sum(l), top_c = m == -INFINITY ? -INFINITY : m * c;
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-        __syncthreads();
-        const float sum = query_sum(l[t]), top_c = m[t] == -INFINITY ? -INFINITY : m[t] * c;
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(vbuf + d * 1024 + lane * 16) = o[d];
+    if (q4 == 0) ml[0][wave][r16] = top_c, ml[1][wave][r16] = sum;
+    __syncthreads();
+    float top = ml[0][0][r16];
 #pragma unroll
-        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4 *>(vbuf + d * 1024 + lane * 16) = o[d][t];
-        if (q4 == 0) ml[0][wave][r16] = top_c, ml[1][wave][r16] = sum;
-        __syncthreads();
-        float top = ml[0][0][r16];
+    for (int w = 1; w < NW; ++w) top = fmaxf(top, ml[0][w][r16]);
+    const float at = top == -INFINITY ? 0.0f : top;
+    float all = 0.0f;
+    f32x4 x[MD];
 #pragma unroll
-        for (int w = 1; w < NW; ++w) top = fmaxf(top, ml[0][w][r16]);
-        const float at = top == -INFINITY ? 0.0f : top;
-        float all = 0.0f;
-        f32x4 x[MD];
+    for (int i = 0; i < MD; ++i) x[i] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int d = 0; d < MD; ++d) x[d] = f32x4{0, 0, 0, 0};
+    for (int w = 0; w < NW; ++w) {
+        const float f = exp2f(ml[0][w][r16] - at);
+        all += ml[1][w][r16] * f;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const float f = exp2f(ml[0][w][r16] - at);
-            all += ml[1][w][r16] * f;
+        for (int i = 0; i < MD; ++i)
+            x[i] += *reinterpret_cast<const f32x4 *>(lds + w * VBUF + (wave + i * NW) % DT * 1024 + lane * 16) * f;
+    }
+    if (r0 >= R) return;
+    const size_t at_row = ((size_t)split * a.nkv + g) * R + r0;
+    const bool any = a.part || all != 0.0f || sees_any(a, tok);
+    if (a.part && wave == 0 && q4 == 0) {
+        float *mlp = a.part + (size_t)a.splits * a.nkv * R * HD + 2 * at_row;
+        mlp[0] = top, mlp[1] = all;
+    }
 #pragma unroll
-            for (int d = 0; d < MD; ++d)
-                x[d] += *reinterpret_cast<const f32x4 *>(lds + w * VBUF + (wave * MD + d) * 1024 + lane * 16) * f;
-        }
-        const uint32_t r = (rb * QT + t) * 16 + r16;
-        if (r >= R) continue;
-        if (a.part) {
-            const size_t at_row = ((size_t)split * a.nkv + g) * R + r;
-            float *w = a.part + at_row * HD, *mlp = a.part + (size_t)a.splits * a.nkv * R * HD + 2 * at_row;
-#pragma unroll
-            for (int d = 0; d < MD; ++d) *reinterpret_cast<f32x4 *>(w + 16 * (wave * MD + d) + 4 * q4) = x[d];
-            if (wave == 0 && q4 == 0) mlp[0] = top, mlp[1] = all;
-        } else {
-            const bool any = all != 0.0f || sees_any(a, tok[t]);
-            uint16_t *out = a.out + ((size_t)tok[t] * a.nh + g * per + r % per) * a.hd;
-#pragma unroll
-            for (int d = 0; d < MD; ++d) {
-                const uint32_t dim = 16 * (wave * MD + d) + 4 * q4;
-                if (dim < a.hd) *reinterpret_cast<u32x2 *>(out + dim) = finish(x[d], all, any);
-            }
-        }
+    for (int i = 0; i < MD; ++i) {
+        const uint32_t d = wave + i * NW, dim = 16 * d + 4 * q4;
+        if (d >= DT) break;
+        if (a.part) *reinterpret_cast<f32x4 *>(a.part + at_row * HD + dim) = x[i];
+        else if (dim < a.hd) *reinterpret_cast<u32x2 *>(a.out + qrow * a.hd + dim) = finish(x[i], all, any);
     }
 }
 
@@ -723,34 +703,48 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_mxfp4_tiles(const MxAt
         }
 }
 
-// Merges the splits' (o, m, l): a thread takes four dimensions of a query row, GR threads its
-// splits in turn.
+// Merges the splits' (o, m, l): a thread takes four dimensions of a query row and up to eight splits, all of which
+// it asks for at once; GR threads share a row's splits and meet in LDS.
+constexpr uint32_t MERGE_SPLITS = 8;
+static_assert(MXA_SPLIT_MAX <= 8 * MERGE_SPLITS, "eight threads a row hold all splits");
+
 template <int HD, int GR>
-__global__ __launch_bounds__(256) void attention_mxfp4_merge(const MxAttn a) {
-    constexpr uint32_t QUADS = HD / 4, PER = 256 / (QUADS * GR);   // rows of a workgroup
-    static_assert(PER >= 1, "rows");
-    __shared__ float lds[GR > 1 ? 6 * 256 : 1];
+__global__ __launch_bounds__(GR > 1 ? HD / 4 * GR : 256) void attention_mxfp4_merge(const MxAttn a) {
+    constexpr uint32_t T = GR > 1 ? HD / 4 * GR : 256, QUADS = HD / 4, PER = T / (QUADS * GR);   // threads, rows of a workgroup
+    __shared__ float lds[GR > 1 ? 6 * T : 1];
     const uint32_t quad = threadIdx.x % QUADS, grp = threadIdx.x / QUADS % GR;
     const uint32_t per = a.nh / a.nkv, R = a.tokens * per, all_rows = a.nkv * R;
     const uint32_t at = blockIdx.x * PER + threadIdx.x / (QUADS * GR), row = min(at, all_rows - 1);
     const float *w = a.part + (size_t)row * HD + 4 * quad, *mlp = a.part + (size_t)a.splits * all_rows * HD + 2 * (size_t)row;
     const size_t step = (size_t)all_rows * HD, step_ml = 2 * (size_t)all_rows;
+    float ms[MERGE_SPLITS], ls[MERGE_SPLITS];
+    f32x4 os[MERGE_SPLITS];
+#pragma unroll
+    for (uint32_t i = 0; i < MERGE_SPLITS; ++i) {
+        const uint32_t s = grp + i * GR;
+        ms[i] = -INFINITY, ls[i] = 0.0f, os[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (s < a.splits) {
+            const float2 v = *reinterpret_cast<const float2 *>(mlp + s * step_ml);
+            ms[i] = v.x, ls[i] = v.y;
+            os[i] = *reinterpret_cast<const f32x4 *>(w + s * step);
+        }
+    }
     float top = -INFINITY, l = 0.0f;
     f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 8
-    for (uint32_t s = grp; s < a.splits; s += GR) top = fmaxf(top, mlp[s * step_ml]);
+#pragma unroll
+    for (uint32_t i = 0; i < MERGE_SPLITS; ++i) top = fmaxf(top, ms[i]);
     const float ref = top == -INFINITY ? 0.0f : top;
-#pragma unroll 8
-    for (uint32_t s = grp; s < a.splits; s += GR) {
-        const float f = exp2f(mlp[s * step_ml] - ref);
-        l += mlp[s * step_ml + 1] * f;
-        o += *reinterpret_cast<const f32x4 *>(w + s * step) * f;
+#pragma unroll
+    for (uint32_t i = 0; i < MERGE_SPLITS; ++i) {
+        const float f = exp2f(ms[i] - ref);
+        l += ls[i] * f;
+        o += os[i] * f;
     }
     if constexpr (GR > 1) {
         float *mine = lds + threadIdx.x;
-        mine[0] = top, mine[256] = l;
+        mine[0] = top, mine[T] = l;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mine[512 + 256 * e] = o[e];
+        for (int e = 0; e < 4; ++e) mine[(2 + e) * T] = o[e];
         __syncthreads();
         if (grp > 0) return;
         const float *p = lds + threadIdx.x;
@@ -762,9 +756,9 @@ __global__ __launch_bounds__(256) void attention_mxfp4_merge(const MxAttn a) {
 #pragma unroll
         for (int k = 0; k < GR; ++k) {
             const float f = exp2f(p[k * QUADS] - base);
-            l += p[k * QUADS + 256] * f;
+            l += p[k * QUADS + T] * f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] += p[k * QUADS + 512 + 256 * e] * f;
+            for (int e = 0; e < 4; ++e) o[e] += p[k * QUADS + (2 + e) * T] * f;
         }
     }
     if (at >= all_rows || 4 * quad >= a.hd) return;
@@ -777,21 +771,21 @@ template <int HD>
 int launch_merge(const MxAttn &a, hipStream_t st) {
     if (a.splits < 2) return RENG_HIP_OK;
     const uint32_t rows = a.tokens * a.nh;
-    constexpr int GR = 256 / (HD / 4);
-    if (a.splits >= 8)
-        hipLaunchKernelGGL((attention_mxfp4_merge<HD, GR>), dim3(rows), dim3(256), 0, st, a);
+    constexpr uint32_t PER = 256 / (HD / 4);
+    if (a.splits > MERGE_SPLITS)
+        hipLaunchKernelGGL((attention_mxfp4_merge<HD, 8>), dim3(rows), dim3(HD / 4 * 8), 0, st, a);
     else
-        hipLaunchKernelGGL((attention_mxfp4_merge<HD, 1>), dim3((rows + GR - 1) / GR), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((attention_mxfp4_merge<HD, 1>), dim3((rows + PER - 1) / PER), dim3(256), 0, st, a);
     return check_launch("attention_mxfp4_merge");
 }
 
 unsigned grid_of(const MxAttn &a) { return (a.units + MXA_XCDS - 1) / MXA_XCDS * MXA_XCDS * a.row_blocks; }
 
-template <int HD, int QT>
+template <int HD, int NW>
 int launch_rows(const MxAttn &a, hipStream_t st) {
-    constexpr int LDS = MXA_WAVES * MXA_TILE * 2 * HD;
+    constexpr int LDS = NW * MXA_TILE * 2 * HD;
     static_assert(LDS <= 160 * 1024, "LDS");
-    hipLaunchKernelGGL((attention_mxfp4<HD, QT>), dim3(grid_of(a)), dim3(64 * MXA_WAVES), LDS, st, a);
+    hipLaunchKernelGGL((attention_mxfp4<HD, NW>), dim3(grid_of(a)), dim3(64 * NW), LDS, st, a);
     if (int rc = check_launch("attention_mxfp4")) return rc;
     return launch_merge<HD>(a, st);
 }
@@ -808,16 +802,13 @@ template <int HD>
 int launch_form(const MxAttn &a, int form, hipStream_t st) {
     if constexpr (HD == 256) {
         switch (form) {
-        case MXA_ROWS_16: return launch_rows<HD, 1>(a, st);
-        case MXA_ROWS_32: return launch_rows<HD, 2>(a, st);
+        case MXA_ROWS_16: return launch_rows<HD, 4>(a, st);
         case MXA_TILES_64: return launch_tiles<HD, 2, 2, 32, 2>(a, st);
         default: return launch_tiles<HD, 4, 1, 32, 2>(a, st);
         }
     } else {
         switch (form) {
-        case MXA_ROWS_16: return launch_rows<HD, 1>(a, st);
-        case MXA_ROWS_32: return launch_rows<HD, 2>(a, st);
-        case MXA_ROWS_64: return launch_rows<HD, 4>(a, st);
+        case MXA_ROWS_16: return launch_rows<HD, 8>(a, st);
         case MXA_TILES_64: return launch_tiles<HD, 2, 4, 32, 2>(a, st);
         case MXA_TILES_128: return launch_tiles<HD, 4, 2, 32, 2>(a, st);
         default: return launch_tiles<HD, 8, 1, 64, 4>(a, st);

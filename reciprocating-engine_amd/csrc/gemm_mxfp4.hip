@@ -67,6 +67,129 @@ __device__ __forceinline__ uint32_t within(uint32_t pair, uint32_t q, uint32_t b
     return q >= blocks ? ONE_BYTE | (ONE_BYTE << 8) : 4 + q >= blocks ? (pair & 0xffu) | (ONE_BYTE << 8) : pair;
 }
 
+// ------------------------------------------------------------ one to four rows
+//
+// A wave takes NR rows of b, 2048 of k at a time: a lane has one block of 32 codes of each, and of each
+// row of a. The codes become bf16 pairs without their scale, whose products (quarters of at most 36)
+// v_dot2_f32_bf16 sums exactly; the two scale bytes then move the sum's exponent. KS waves share
+// rows and take pieces of k in turn. All of a wave's loads of a piece are on the way while it works on the
+// one before.
+constexpr uint32_t VEC_NR = 4, VEC_K = 2048, VEC_M = 4;
+
+__device__ __forceinline__ bf16x2_t pair_of(uint32_t d, int i) {
+    switch (i) {
+    case 0: return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, 1.0f, 0);
+    case 1: return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, 1.0f, 1);
+    case 2: return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, 1.0f, 2);
+    default: return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, 1.0f, 3);
+    }
+}
+
+template <int M, int KS>
+__global__ __launch_bounds__(256) void gemm_mx_vectors(MxArgs g) {
+    constexpr uint32_t NR = VEC_NR, GROUPS = 4 / KS;   // groups of rows of a workgroup
+    __shared__ float sums[KS > 1 ? 4 * NR * M : 1];
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % KS, grp = wave / KS;
+    const uint32_t n0 = (blockIdx.x * GROUPS + grp) * NR, kb = g.K / 2, sp = (uint32_t)scale_pitch(g.K);
+    const uint32_t pieces = (g.K + VEC_K - 1) / VEC_K;
+    const uint32_t rows = n0 < g.N ? min(NR, g.N - n0) : 0;   // rows past N arrive as zeros
+    const __amdgpu_buffer_rsrc_t rb = resource(g.b + (size_t)n0 * kb, (size_t)rows * kb);
+    const __amdgpu_buffer_rsrc_t rsb = resource(g.sb + (size_t)n0 * sp, (size_t)rows * sp);
+    const __amdgpu_buffer_rsrc_t ra = resource(g.a, (size_t)M * kb), rsa = resource(g.sa, (size_t)M * sp);
+    struct Piece {
+        u32x4 a[M], b[NR];
+        uint32_t sa[M], sb[NR];
+    };
+    auto fetch = [&](uint32_t p) __attribute__((always_inline)) {
+        Piece v;
+        const uint32_t at = p * (VEC_K / 2) + lane * 16, blk = p * (VEC_K / BLOCK) + lane;
+        const bool on = at < kb;   // past K codes of zeros
+        auto codes = [&](const __amdgpu_buffer_rsrc_t &r, uint32_t row) __attribute__((always_inline)) {
+            return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, on ? at + row * kb : NOTHING, 0, 0));
+        };
+        auto scale = [&](const __amdgpu_buffer_rsrc_t &r, uint32_t row) __attribute__((always_inline)) {
+            return (uint32_t)(uint8_t)__builtin_amdgcn_raw_buffer_load_b8(r, on ? blk + row * sp : NOTHING, 0, 0);
+        };
+#pragma unroll
+        for (uint32_t i = 0; i < NR; ++i) v.b[i] = codes(rb, i), v.sb[i] = scale(rsb, i);
+#pragma unroll
+        for (uint32_t i = 0; i < M; ++i) v.a[i] = codes(ra, i), v.sa[i] = scale(rsa, i);
+        return v;
+    };
+    float acc[NR][M];
+#pragma unroll
+    for (uint32_t i = 0; i < NR; ++i)
+#pragma unroll
+        for (int m = 0; m < M; ++m) acc[i][m] = 0.0f;
+    Piece v;
+    if (part < pieces) v = fetch(part);
+    for (uint32_t p = part; p < pieces; p += KS) {
+        const Piece w = v;
+        if (p + KS < pieces) v = fetch(p + KS);
+        bf16x2_t x[M][16];
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[m][e] = pair_of(w.a[m][e / 4], e % 4);
+#pragma unroll
+        for (uint32_t i = 0; i < NR; ++i) {
+            float s[M] = {};
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const bf16x2_t y = pair_of(w.b[i][e / 4], e % 4);
+#pragma unroll
+                for (int m = 0; m < M; ++m) s[m] = __builtin_amdgcn_fdot2_f32_bf16(x[m][e], y, s[m], false);
+            }
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+                const float t = __builtin_amdgcn_ldexpf(s[m], (int)(w.sa[m] + w.sb[i]) - 2 * (int)ONE_BYTE);
+                acc[i][m] += max(w.sa[m], w.sb[i]) == NAN_BYTE ? __builtin_nanf("") : t;
+            }
+        }
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < NR; ++i)
+#pragma unroll
+        for (int m = 0; m < M; ++m) acc[i][m] = wave_sum_dpp(acc[i][m]);
+    if constexpr (KS > 1) {
+        if (lane == 0)
+#pragma unroll
+            for (uint32_t i = 0; i < NR; ++i)
+#pragma unroll
+                for (int m = 0; m < M; ++m) sums[(wave * NR + i) * M + m] = acc[i][m];
+        __syncthreads();
+        // A lane an output, the waves' sums in their order.
+        const uint32_t i = lane / M, m = lane % M;
+        if (part > 0 || lane >= NR * M || i >= rows) return;
+        float t = sums[(wave * NR + i) * M + m];
+#pragma unroll
+        for (uint32_t w = 1; w < KS; ++w) t += sums[((wave + w) * NR + i) * M + m];
+        g.out[(size_t)m * g.N + n0 + i] = (uint16_t)f32_to_bf16_bits(t);
+    } else {
+        if (lane > 0) return;
+#pragma unroll
+        for (uint32_t i = 0; i < NR; ++i)
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+                if (i < rows) g.out[(size_t)m * g.N + n0 + i] = (uint16_t)f32_to_bf16_bits(acc[i][m]);
+    }
+}
+
+template <int M>
+int launch_vectors(const MxArgs &g, hipStream_t st) {
+    const uint32_t groups = (g.N + VEC_NR - 1) / VEC_NR, pieces = (g.K + VEC_K - 1) / VEC_K;
+    // Sixteen waves a CU, where there are as many pieces.
+    const uint32_t want = (uint32_t)device_props().cus * 16;
+    auto go = [&](auto kern, uint32_t ks) {
+        hipLaunchKernelGGL(kern, dim3((groups * ks + 3) / 4), dim3(256), 0, st, g);
+        return check_launch("gemm_mx_vectors");
+    };
+    if (groups >= want || pieces < 2) return go(gemm_mx_vectors<M, 1>, 1);
+    if (groups * 2 >= want || pieces < 4) return go(gemm_mx_vectors<M, 2>, 2);
+    return go(gemm_mx_vectors<M, 4>, 4);
+}
+
 // ------------------------------------------------------------ few rows
 //
 // Where the weight's bytes are the time, or larger tiles would leave CUs idle. A workgroup
@@ -474,6 +597,10 @@ static_assert(Tile256::BM == 256 && Tile256::BN == 256 && Tile128::BM == 128 && 
               "MX_COST's tiles");
 
 int launch_product(const MxArgs &g, hipStream_t st) {
+    if (g.M == 1) return launch_vectors<1>(g, st);
+    if (g.M == 2) return launch_vectors<2>(g, st);
+    if (g.M == 3) return launch_vectors<3>(g, st);
+    if (g.M == 4) return launch_vectors<4>(g, st);
     switch (mx_pick(g.M, g.N, g.K, (uint64_t)device_props().cus)) {
     case MX_RING_1x1: return launch_ring<1, 1, 4, 4>(g, st);
     case MX_RING_1x2: return launch_ring<1, 2, 4, 3>(g, st);
