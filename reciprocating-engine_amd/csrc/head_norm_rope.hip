@@ -31,35 +31,34 @@ struct HeadsArgs {
     uint16_t *q_out, *k_rows, *v_rows;
     reng_hip_mx_cache cache;
     size_t first;
-    uint32_t axes;        // 1: pair_axis is not looked at
+    uint64_t axes8;       // of each 8 pairs their axis, four bits; MIXED: pair_axis says it pair by pair
     uint8_t pair_axis[128];
 };
+constexpr uint32_t MIXED = 15;
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 template <bool VEC>
-__device__ __forceinline__ void load8(const uint16_t *p, float (&x)[8]) {
-    if constexpr (VEC) {
-        const u32x4_t v = *reinterpret_cast<const u32x4_t *>(p);
+__device__ __forceinline__ u32x4_t load8(const uint16_t *p) {
+    if constexpr (VEC) return *reinterpret_cast<const u32x4_t *>(p);
+    u32x4_t v;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = __uint_as_float(v[i] << 16);
-            x[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = __uint_as_float((uint32_t)p[i] << 16);
-    }
+    for (int i = 0; i < 4; ++i) v[i] = (uint32_t)p[2 * i] | ((uint32_t)p[2 * i + 1] << 16);
+    return v;
 }
 
 template <bool VEC>
 __device__ __forceinline__ void store8(uint16_t *p, const float (&x)[8]) {
-    uint32_t b[8];
+    u32x4_t v;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) b[i] = f32_to_bf16_bits(x[i]);
+    for (int i = 0; i < 4; ++i)
+        v[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x[2 * i], x[2 * i + 1]}, bf16x2));
     if constexpr (VEC) {
-        *reinterpret_cast<u32x4_t *>(p) = u32x4_t{b[0] | (b[1] << 16), b[2] | (b[3] << 16), b[4] | (b[5] << 16), b[6] | (b[7] << 16)};
+        *reinterpret_cast<u32x4_t *>(p) = v;
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = (uint16_t)b[i];
+        for (int i = 0; i < 8; ++i) p[i] = (uint16_t)(v[i / 2] >> (16 * (i % 2)));
     }
 }
 
@@ -75,114 +74,174 @@ __device__ __forceinline__ void load8f(const float *p, float (&x)[8]) {
 __device__ __forceinline__ void tables(const HeadsArgs &a, uint32_t token, uint32_t d, uint32_t pair, float (&sn)[8],
                                        float (&cs)[8]) {
     auto row_of = [&](uint32_t axis) { return (uint32_t)a.positions[(size_t)axis * a.tokens + token]; };
-    bool one = true;
-    if (a.axes > 1)
-#pragma unroll
-        for (int i = 1; i < 8; ++i) one &= a.pair_axis[pair + i] == a.pair_axis[pair];
-    if (one) {
-        const uint32_t row = row_of(a.axes > 1 ? a.pair_axis[pair] : 0);
-        if (row < a.table_rows) {
-            const size_t at = (size_t)row * a.rot + d;
-            load8f(a.sin_table + at, sn);
-            load8f(a.cos_table + at, cs);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sn[i] = cs[i] = __builtin_nanf("");
-        }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint32_t row = row_of(a.pair_axis[pair + i]);
-        const size_t at = (size_t)row * a.rot + d + i;
+    // A row outside the tables is read as row 0 and then made NaN: no branch holds the loads up.
+    const uint32_t axis = (uint32_t)(a.axes8 >> (pair / 2)) & 15;
+    if (axis != MIXED) {
+        const uint32_t row = row_of(axis);
         const bool in = row < a.table_rows;
-        sn[i] = in ? a.sin_table[at] : __builtin_nanf("");
-        cs[i] = in ? a.cos_table[at] : __builtin_nanf("");
+        const size_t at = (size_t)(in ? row : 0) * a.rot + d;
+        load8f(a.sin_table + at, sn);
+        load8f(a.cos_table + at, cs);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            sn[i] = in ? sn[i] : __builtin_nanf("");
+            cs[i] = in ? cs[i] : __builtin_nanf("");
+        }
+    } else {
+        uint32_t row[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) row[i] = row_of(a.pair_axis[pair + i]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const bool in = row[i] < a.table_rows;
+            const size_t at = (size_t)(in ? row[i] : 0) * a.rot + d + i;
+            const float x = a.sin_table[at], y = a.cos_table[at];
+            sn[i] = in ? x : __builtin_nanf("");
+            cs[i] = in ? y : __builtin_nanf("");
+        }
     }
 }
 
-// L lanes a head: 4, 8, 16 or 32, at least hd / 8. VEC: 16-byte aligned rows. MX: into the cache.
-template <int L, bool VEC, bool MX>
-__global__ __launch_bounds__(256) void head_norm_rope(const HeadsArgs a) {
-    const uint32_t lane = threadIdx.x & 63, li = threadIdx.x % L, heads = a.nh + 2 * a.nkv;
-    const size_t total = (size_t)a.tokens * heads, item = (size_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-    const bool on = item < total && li * 8 < a.hd;   // a lane without values still takes part in the exchanges
-    const uint32_t token = item < total ? (uint32_t)(item / heads) : 0, h = item < total ? (uint32_t)(item % heads) : 0;
-    const uint32_t part = h < a.nh ? 0 : h < a.nh + a.nkv ? 1 : 2;   // q, k or v
-    const uint32_t g = h - (part == 0 ? 0 : part == 1 ? a.nh : a.nh + a.nkv), d = li * 8;
-    const uint16_t *base = part == 0 ? a.q : part == 1 ? a.k : a.v;
-    float x[8] = {};
-    if (on && base) load8<VEC>(base + (size_t)token * (part == 0 ? a.q_ld : a.kv_ld) + (size_t)g * a.hd + d, x);
-    const float *gamma = part == 0 ? a.q_gamma : part == 1 ? a.k_gamma : nullptr;
-    if (a.q_gamma || a.k_gamma) {
-        float ss = 0.0f;
+// The value of lane ^ (L / 2) of a group of L; for 16 lanes without LDS.
+template <int L>
+__device__ __forceinline__ float across(float v) {
+    if constexpr (L == 16) return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, true));   // row_ror:8
+    return __shfl_xor(v, L / 2, 64);
+}
+template <int L>
+__device__ __forceinline__ float group_sum(float v) {
+    v += across<L>(v);
+    if constexpr (L == 16) {
+        v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x124, 0xf, 0xf, true));   // row_ror:4
+        v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x122, 0xf, 0xf, true));   // row_ror:2
+        v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x121, 0xf, 0xf, true));   // row_ror:1
+    } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-        if (on && gamma) {
-            const float inv = 1.0f / sqrtf(ss / (float)a.hd + a.eps);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * gamma[d + i];
-        }
+        for (int o = L / 4; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
     }
-    if (a.sin_table) {
-        const uint32_t half = a.rot / 2;
-        const bool low = d < half, turns = on && part < 2 && d < a.rot;
-        float y[8];
-        const uint32_t other = low ? lane + half / 8 : lane - half / 8;
+    return v;
+}
+
+// L lanes a head: 4, 8, 16 or 32, at least hd / 8. A workgroup takes IT times 256 / L heads of a token, whose
+// rows and the token's sines and cosines are asked for at once. VEC: 16-byte aligned rows. MX: into the cache.
+template <int L, int IT, bool VEC, bool MX>
+__global__ __launch_bounds__(256) void head_norm_rope(const HeadsArgs a, uint32_t parts) {
+    constexpr uint32_t G = 256 / L;
+    const uint32_t lane = threadIdx.x & 63, li = threadIdx.x % L, heads = a.nh + 2 * a.nkv;
+    const uint32_t token = blockIdx.x / parts, h0 = blockIdx.x % parts * (IT * G) + threadIdx.x / L;
+    const bool has = li * 8 < a.hd;   // a lane without values still takes part in the exchanges, with zeros
+    const uint32_t d = has ? li * 8 : 0;
+    struct Head {
+        uint32_t part, g;   // q, k or v, and which of its heads
+    };
+    auto head_of = [&](uint32_t h) {
+        return h < a.nh ? Head{0, h} : h < a.nh + a.nkv ? Head{1, h - a.nh} : Head{2, h - a.nh - a.nkv};
+    };
+    u32x4_t raw[IT];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = __shfl(x[i], (int)other, 64);
-        if (turns) {
-            float sn[8], cs[8];
-            tables(a, token, d, low ? d : d - half, sn, cs);
+    for (int it = 0; it < IT; ++it) {   // past the last head the last one again, which is not stored
+        const Head h = head_of(min(h0 + it * G, heads - 1));
+        const uint16_t *base = h.part == 0 ? a.q : h.part == 2 && a.v ? a.v : a.k;
+        raw[it] = load8<VEC>(base + (size_t)token * (h.part == 0 ? a.q_ld : a.kv_ld) + h.g * a.hd + d);
+        if (a.hd != 8 * L && !has) raw[it] = u32x4_t{0u, 0u, 0u, 0u};
+    }
+    const uint32_t half = a.rot / 2;
+    const bool low = d < half, turns = a.sin_table && d < a.rot, whole = a.rot == 8 * L;
+    float gq[8], gk[8], sn[8], cs[8];
+    if (turns) tables(a, token, d, low ? d : d - half, sn, cs);
+    if (a.q_gamma)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float t = y[i] * sn[i];
-                x[i] = fmaf(x[i], cs[i], low ? -t : t);
+        for (int i = 0; i < 8; ++i) gq[i] = a.q_gamma[d + i];
+    if (a.k_gamma)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) gk[i] = a.k_gamma[d + i];
+    // y[d] = x[d] cos - x[d + half] sin, y[d + half] = x[d + half] cos + x[d] sin
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sn[i] = low ? -sn[i] : sn[i];
+    const uint32_t other = low ? lane + half / 8 : lane - half / 8;
+#pragma unroll
+    for (int it = 0; it < IT; ++it) {
+        const bool on = has && h0 + it * G < heads;
+        const Head h = head_of(min(h0 + it * G, heads - 1));
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(raw[it][i] << 16);
+            x[2 * i + 1] = __uint_as_float(raw[it][i] & 0xffff0000u);
+        }
+        if (a.q_gamma || a.k_gamma) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+            ss = group_sum<L>(ss);
+            const float inv = 1.0f / sqrtf(ss / (float)a.hd + a.eps);
+            if (h.part == 0 && a.q_gamma)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * gq[i];
+            if (h.part == 1 && a.k_gamma)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * gk[i];
+        }
+        if (a.sin_table) {
+            float y[8];
+            if (whole)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = across<L>(x[i]);
+            else
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[i] = __shfl(x[i], (int)other, 64);
+            if (turns && h.part < 2)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = fmaf(x[i], cs[i], y[i] * sn[i]);
+        }
+        if (!MX || h.part == 0) {
+            uint16_t *out = h.part == 0 ? a.q_out : h.part == 1 ? a.k_rows : a.v_rows;
+            if (on && out) store8<VEC>(out + (size_t)token * ((h.part == 0 ? a.nh : a.nkv) * a.hd) + h.g * a.hd + d, x);
+        }
+        if constexpr (MX) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+            const uint32_t top = quad_max(m), byte = has ? scale_byte(top) : ONE_BYTE;
+            uint32_t word;
+            if constexpr (L >= 16) {
+                word = scale_word(byte);
+            } else {   // one or two blocks
+                word = byte << (8 * (li / 4));
+                if constexpr (L == 8) word |= (uint32_t)__builtin_amdgcn_ds_swizzle((int)word, 0x101f);   // lane ^ 4
+                word |= L == 8 ? 0x7f7f0000u : 0x7f7f7f00u;
+            }
+            if (on && h.part > 0) {
+                const size_t row = (size_t)h.g * a.cache.capacity + a.first + token, sp = scale_pitch(a.hd);
+                uint8_t *codes = h.part == 1 ? a.cache.k_codes : a.cache.v_codes;
+                uint8_t *scales = h.part == 1 ? a.cache.k_scales : a.cache.v_scales;
+                *reinterpret_cast<uint32_t *>(codes + row * (a.hd / 2) + d / 2) = encode8(x, byte);
+                if (li % 16 == 0) *reinterpret_cast<uint32_t *>(scales + row * sp + li / 4) = word;
             }
         }
     }
-    if (!MX || part == 0) {
-        uint16_t *out = part == 0 ? a.q_out : part == 1 ? a.k_rows : a.v_rows;
-        if (on && out) store8<VEC>(out + ((size_t)token * (part == 0 ? a.nh : a.nkv) + g) * a.hd + d, x);
-    }
-    if constexpr (MX) {
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
-        const uint32_t byte = scale_byte(quad_max(m));
-        uint32_t word;
-        if constexpr (L >= 16) {
-            word = scale_word(byte);
-        } else {   // one or two blocks
-            word = byte << (8 * (li / 4));
-            if constexpr (L == 8) word |= (uint32_t)__builtin_amdgcn_ds_swizzle((int)word, 0x101f);   // lane ^ 4
-            word |= L == 8 ? 0x7f7f0000u : 0x7f7f7f00u;
-        }
-        if (on && part > 0) {
-            const size_t row = (size_t)g * a.cache.capacity + a.first + token, sp = scale_pitch(a.hd);
-            uint8_t *codes = part == 1 ? a.cache.k_codes : a.cache.v_codes;
-            uint8_t *scales = part == 1 ? a.cache.k_scales : a.cache.v_scales;
-            *reinterpret_cast<uint32_t *>(codes + row * (a.hd / 2) + d / 2) = encode8(x, byte);
-            if (li % 16 == 0) *reinterpret_cast<uint32_t *>(scales + row * sp + li / 4) = word;
-        }
-    }
+}
+
+template <int L, bool VEC, bool MX>
+int launch_lanes(const HeadsArgs &a, hipStream_t st) {
+    const uint32_t heads = a.nh + 2 * a.nkv;
+    auto go = [&](auto kern, uint32_t it) {
+        const uint32_t parts = (heads + it * (256 / L) - 1) / (it * (256 / L));
+        RENG_REQUIRE((uint64_t)a.tokens * parts < (1u << 24), "%u tokens of %u heads are too many for a launch", a.tokens, heads);
+        hipLaunchKernelGGL(kern, dim3(a.tokens * parts), dim3(256), 0, st, a, parts);
+        return check_launch("head_norm_rope");
+    };
+    // Four heads a group of lanes where that leaves four workgroups a CU.
+    if ((uint64_t)a.tokens * heads >= (uint64_t)device_props().cus * 16 * (256 / L)) return go(head_norm_rope<L, 4, VEC, MX>, 4);
+    return go(head_norm_rope<L, 1, VEC, MX>, 1);
 }
 
 template <bool MX>
 int launch_heads(const HeadsArgs &a, bool vec, hipStream_t st) {
-    auto go = [&](auto kern, unsigned lanes) {
-        const size_t items = (size_t)a.tokens * (a.nh + 2 * a.nkv), per = 256 / lanes;
-        const size_t blocks = (items + per - 1) / per;
-        RENG_REQUIRE(blocks < (1u << 24), "%u tokens of %u heads are too many for a launch", a.tokens, a.nh + 2 * a.nkv);
-        hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), 0, st, a);
-        return check_launch("head_norm_rope");
-    };
-    if (a.hd <= 32) return vec ? go(head_norm_rope<4, true, MX>, 4) : go(head_norm_rope<4, false, MX>, 4);
-    if (a.hd <= 64) return vec ? go(head_norm_rope<8, true, MX>, 8) : go(head_norm_rope<8, false, MX>, 8);
-    if (a.hd <= 128) return vec ? go(head_norm_rope<16, true, MX>, 16) : go(head_norm_rope<16, false, MX>, 16);
-    return vec ? go(head_norm_rope<32, true, MX>, 32) : go(head_norm_rope<32, false, MX>, 32);
+    if (a.hd <= 32) return vec ? launch_lanes<4, true, MX>(a, st) : launch_lanes<4, false, MX>(a, st);
+    if (a.hd <= 64) return vec ? launch_lanes<8, true, MX>(a, st) : launch_lanes<8, false, MX>(a, st);
+    if (a.hd <= 128) return vec ? launch_lanes<16, true, MX>(a, st) : launch_lanes<16, false, MX>(a, st);
+    return vec ? launch_lanes<32, true, MX>(a, st) : launch_lanes<32, false, MX>(a, st);
 }
 
 // What both entry points check and fill in.
@@ -208,7 +267,7 @@ int heads_args(HeadsArgs &a, const uint16_t *q, size_t q_ld, const uint16_t *k, 
     a.tokens = (uint32_t)tokens, a.nh = (uint32_t)nh, a.nkv = (uint32_t)nkv, a.hd = (uint32_t)hd;
     a.q_gamma = q_gamma, a.k_gamma = k_gamma, a.eps = eps, a.q_out = q_out;
     a.sin_table = a.cos_table = nullptr;
-    a.axes = 1;
+    a.axes8 = 0;
     if (!rope) return RENG_HIP_OK;
     const reng_hip_rope &r = *rope;
     RENG_REQUIRE(r.rot_dim >= 16 && r.rot_dim % 16 == 0 && r.rot_dim <= hd, "rot_dim %zu is no multiple of 16 in [16, %zu]",
@@ -223,10 +282,12 @@ int heads_args(HeadsArgs &a, const uint16_t *q, size_t q_ld, const uint16_t *k, 
             RENG_REQUIRE(r.pair_axis[i] < r.axes, "pair %zu has axis %d of %zu", i, r.pair_axis[i], r.axes);
     a.sin_table = r.sin_table, a.cos_table = r.cos_table, a.table_rows = (uint32_t)r.table_rows;
     a.rot = (uint32_t)r.rot_dim, a.positions = positions;
-    if (r.pair_axis) {
-        a.axes = (uint32_t)r.axes;
-        for (size_t i = 0; i < r.rot_dim / 2; ++i) a.pair_axis[i] = r.pair_axis[i];
-    }
+    if (r.pair_axis)
+        for (size_t i = 0; i < r.rot_dim / 2; ++i) {
+            a.pair_axis[i] = r.pair_axis[i];
+            const uint64_t eight = r.pair_axis[i / 8 * 8] == r.pair_axis[i] ? r.pair_axis[i] : MIXED;
+            a.axes8 |= eight << (i / 8 * 4);
+        }
     return RENG_HIP_OK;
 }
 
