@@ -58,6 +58,11 @@ __device__ __forceinline__ Frag fragment(const uint8_t *tile, uint32_t row, uint
     return Frag{*reinterpret_cast<const u32x4 *>(p + (q ^ w) * 16), *reinterpret_cast<const u32x4 *>(p + ((4 + q) ^ w) * 16)};
 }
 
+typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ u32x2 bf16x4(const f32x4 &v) {
+    return __builtin_bit_cast(u32x2, __builtin_convertvector(v, bf16x4_t));
+}
+
 // A lane's scales of a stage: of a row's two words byte q each, in the lowest bytes. Past K,
 // where the codes are zeros, a scale of 1: `blocks` is how many of 32 are left from the stage on.
 __device__ __forceinline__ uint32_t scale_pair(const u32x2 &w, uint32_t q) {
@@ -74,7 +79,7 @@ __device__ __forceinline__ uint32_t within(uint32_t pair, uint32_t q, uint32_t b
 // v_dot2_f32_bf16 sums exactly; the two scale bytes then move the sum's exponent. KS waves share
 // rows and take pieces of k in turn. All of a wave's loads of a piece are on the way while it works on the
 // one before.
-constexpr uint32_t VEC_NR = 4, VEC_K = 2048, VEC_M = 4;
+constexpr uint32_t VEC_NR = 4, VEC_K = 2048;
 
 __device__ __forceinline__ bf16x2_t pair_of(uint32_t d, int i) {
     switch (i) {
@@ -294,8 +299,7 @@ __global__ __launch_bounds__(64 * KW) void gemm_mx_ring(MxArgs g, uint32_t tiles
         if (m >= g.M || nn >= g.N) continue;
         uint16_t *out = g.out + (size_t)m * g.N + nn;
         if (vec) {
-            *reinterpret_cast<u32x2 *>(out) = u32x2{f32_to_bf16_bits(v.x) | (f32_to_bf16_bits(v.y) << 16),
-                                                    f32_to_bf16_bits(v.z) | (f32_to_bf16_bits(v.w) << 16)};
+            *reinterpret_cast<u32x2 *>(out) = bf16x4(v);
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -556,10 +560,8 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_mx_tiles(MxArgs g, uint32_t t
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
-            const f32x4 v = acc[i][j];
             *reinterpret_cast<u32x2 *>(lds + (wm * (16 * TM) + 16 * i + row) * RB + 2 * (wn * (16 * TN) + 16 * j + 4 * q)) =
-                u32x2{f32_to_bf16_bits(v.x) | (f32_to_bf16_bits(v.y) << 16),
-                      f32_to_bf16_bits(v.z) | (f32_to_bf16_bits(v.w) << 16)};
+                bf16x4(acc[i][j]);
         }
     __syncthreads();
     constexpr uint32_t CC = T::BN / 8;
