@@ -338,7 +338,7 @@ struct MxTile {
     static constexpr int OUT = BM * (BN * 2 + 16);   // the epilogue's rows, padded by a chunk
     static constexpr int LDS = RING > OUT ? RING : OUT;
     static constexpr bool TURNS = TM == 8;   // the halves of the rows take turns
-    static_assert(!TURNS || (WGM == 2 && WGN == 4 && S == 2), "a wave of each half on a SIMD");
+    static_assert(!TURNS || (WGM == 2 && WGN == 4 && S == 2 && LS == 1), "a wave of each half on a SIMD");
     static_assert(LA * 8 * NW == BM && LB * 8 * NW == BN && LS * 64 * NW == BM + BN && BM % 64 == 0, "copies split evenly");
     static_assert(TM % 2 == 0 && (S - 1) * LOADS + LS < 64 && S >= 2 && S <= 3 && LDS <= 160 * 1024, "vmcnt range, LDS");
 };
@@ -451,9 +451,10 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_mx_tiles(MxArgs g, uint32_t t
         // 2 t + 2. Both halves have stage t's weight fragments in registers by the end of phase 2 t,
         // so in phase 2 t + 1 the first half puts its rows and the weight codes of stage t + 2 into
         // the slot, in phase 2 t + 2 the second its rows; each has landed before its next
-        // products' phase ends. Scales of stages 2 g and 2 g + 1 are copied in the turnovers
-        // of stage 2 g - 2, of either half those it copies; the buffer was last read, by both, in
-        // the turnovers that end phase 2 (2 g - 4) + 2 and land a phase before they are read.
+        // products' phase ends. The scales of stages 2 g and 2 g + 1 are copied in the turnovers behind
+        // products 2 g - 3, a's by the first half in phase 4 g - 5, b's by the second in 4 g - 4. They
+        // have landed by the end of phase 4 g - 3 and are first read in phase 4 g - 1; their buffer was
+        // last read, for stage 2 g - 3, in phases 4 g - 7 and 4 g - 6.
         auto turnover = [&](uint32_t t) __attribute__((always_inline)) {
             read_scales(t);
             take_scales(t);
@@ -489,6 +490,7 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_mx_tiles(MxArgs g, uint32_t t
                 for (int j = 0; j < TN; ++j) asm volatile("" : "+a"(acc[i][j]));
         };
         issue_scales(0);
+        issue_scales(1);
         issue(0);
         issue(1);
         pipe::wait_vmcnt<0>();
@@ -500,7 +502,7 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_mx_tiles(MxArgs g, uint32_t t
             products(t);
             pipe::wait_vmcnt<0>();
             barrier();
-            if (t % G == 0) issue_scales(t / G + 1);
+            if (t % G == 1) issue_scales((t + 3) / G);
             issue_a(t + 2, wave * T::LA, la);
             if (wm == 0) issue_b(t + 2, wave * 2 * T::LB, std::integral_constant<int, 2 * T::LB>{});
             turnover(t + 1);
