@@ -72,13 +72,16 @@ __device__ __forceinline__ uint32_t within(uint32_t pair, uint32_t q, uint32_t b
     return q >= blocks ? ONE_BYTE | (ONE_BYTE << 8) : 4 + q >= blocks ? (pair & 0xffu) | (ONE_BYTE << 8) : pair;
 }
 
-// ------------------------------------------------------------ one to four rows
+// ------------------------------------------------------------ one row
 //
-// A wave takes NR rows of b, 2048 of k at a time: a lane has one block of 32 codes of each, and of each
-// row of a. The codes become bf16 pairs without their scale, whose products (quarters of at most 36)
+// A wave takes NR rows of b, 2048 of k at a time: a lane has one block of 32 codes of each and of
+// a. The codes become bf16 pairs without their scale, whose products (quarters of at most 36)
 // v_dot2_f32_bf16 sums exactly; the two scale bytes then move the sum's exponent. KS waves share
-// rows and take pieces of k in turn. All of a wave's loads of a piece are on the way while it works on the
-// one before.
+// rows and take pieces of k in turn. All of a wave's loads of a piece are on the way while it works
+// on the one before. The weight's bytes and the launch are the time: [14336, 4096] 8.7 us and
+// [27648, 5120] 19.1 (rings 9.7 and 19.6), [4096, 14336] 9.0 (9.2), [4096, 4096] 4.2 (4.1). Two, four or
+// eight rows of b a wave are within 10%. More rows of a cost 1.7 us each at [14336, 4096]: with
+// two the rings are faster (10.0 us; here it would be 10.8) and with four by far (9.7 and 14.1).
 constexpr uint32_t VEC_NR = 4, VEC_K = 2048;
 
 __device__ __forceinline__ bf16x2_t pair_of(uint32_t d, int i) {
@@ -90,10 +93,10 @@ __device__ __forceinline__ bf16x2_t pair_of(uint32_t d, int i) {
     }
 }
 
-template <int M, int KS>
-__global__ __launch_bounds__(256) void gemm_mx_vectors(MxArgs g) {
+template <int KS>
+__global__ __launch_bounds__(256) void gemm_mx_row(MxArgs g) {
     constexpr uint32_t NR = VEC_NR, GROUPS = 4 / KS;   // groups of rows of a workgroup
-    __shared__ float sums[KS > 1 ? 4 * NR * M : 1];
+    __shared__ float sums[4 * NR];
     const uint32_t lane = threadIdx.x & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % KS, grp = wave / KS;
     const uint32_t n0 = (blockIdx.x * GROUPS + grp) * NR, kb = g.K / 2, sp = (uint32_t)scale_pitch(g.K);
@@ -101,10 +104,10 @@ __global__ __launch_bounds__(256) void gemm_mx_vectors(MxArgs g) {
     const uint32_t rows = n0 < g.N ? min(NR, g.N - n0) : 0;   // rows past N arrive as zeros
     const __amdgpu_buffer_rsrc_t rb = resource(g.b + (size_t)n0 * kb, (size_t)rows * kb);
     const __amdgpu_buffer_rsrc_t rsb = resource(g.sb + (size_t)n0 * sp, (size_t)rows * sp);
-    const __amdgpu_buffer_rsrc_t ra = resource(g.a, (size_t)M * kb), rsa = resource(g.sa, (size_t)M * sp);
+    const __amdgpu_buffer_rsrc_t ra = resource(g.a, kb), rsa = resource(g.sa, sp);
     struct Piece {
-        u32x4 a[M], b[NR];
-        uint32_t sa[M], sb[NR];
+        u32x4 a, b[NR];
+        uint32_t sa, sb[NR];
     };
     auto fetch = [&](uint32_t p) __attribute__((always_inline)) {
         Piece v;
@@ -118,81 +121,58 @@ __global__ __launch_bounds__(256) void gemm_mx_vectors(MxArgs g) {
         };
 #pragma unroll
         for (uint32_t i = 0; i < NR; ++i) v.b[i] = codes(rb, i), v.sb[i] = scale(rsb, i);
-#pragma unroll
-        for (uint32_t i = 0; i < M; ++i) v.a[i] = codes(ra, i), v.sa[i] = scale(rsa, i);
+        v.a = codes(ra, 0), v.sa = scale(rsa, 0);
         return v;
     };
-    float acc[NR][M];
-#pragma unroll
-    for (uint32_t i = 0; i < NR; ++i)
-#pragma unroll
-        for (int m = 0; m < M; ++m) acc[i][m] = 0.0f;
+    float acc[NR] = {};
     Piece v;
     if (part < pieces) v = fetch(part);
     for (uint32_t p = part; p < pieces; p += KS) {
         const Piece w = v;
         if (p + KS < pieces) v = fetch(p + KS);
-        bf16x2_t x[M][16];
+        bf16x2_t x[16];
 #pragma unroll
-        for (int m = 0; m < M; ++m)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) x[m][e] = pair_of(w.a[m][e / 4], e % 4);
+        for (int e = 0; e < 16; ++e) x[e] = pair_of(w.a[e / 4], e % 4);
 #pragma unroll
         for (uint32_t i = 0; i < NR; ++i) {
-            float s[M] = {};
+            float s = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const bf16x2_t y = pair_of(w.b[i][e / 4], e % 4);
-#pragma unroll
-                for (int m = 0; m < M; ++m) s[m] = __builtin_amdgcn_fdot2_f32_bf16(x[m][e], y, s[m], false);
-            }
-#pragma unroll
-            for (int m = 0; m < M; ++m) {
-                const float t = __builtin_amdgcn_ldexpf(s[m], (int)(w.sa[m] + w.sb[i]) - 2 * (int)ONE_BYTE);
-                acc[i][m] += max(w.sa[m], w.sb[i]) == NAN_BYTE ? __builtin_nanf("") : t;
-            }
+            for (int e = 0; e < 16; ++e) s = __builtin_amdgcn_fdot2_f32_bf16(x[e], pair_of(w.b[i][e / 4], e % 4), s, false);
+            s = __builtin_amdgcn_ldexpf(s, (int)(w.sa + w.sb[i]) - 2 * (int)ONE_BYTE);
+            acc[i] += max(w.sa, w.sb[i]) == NAN_BYTE ? __builtin_nanf("") : s;
         }
     }
 #pragma unroll
-    for (uint32_t i = 0; i < NR; ++i)
-#pragma unroll
-        for (int m = 0; m < M; ++m) acc[i][m] = wave_sum_dpp(acc[i][m]);
+    for (uint32_t i = 0; i < NR; ++i) acc[i] = wave_sum_dpp(acc[i]);
     if constexpr (KS > 1) {
         if (lane == 0)
 #pragma unroll
-            for (uint32_t i = 0; i < NR; ++i)
-#pragma unroll
-                for (int m = 0; m < M; ++m) sums[(wave * NR + i) * M + m] = acc[i][m];
+            for (uint32_t i = 0; i < NR; ++i) sums[wave * NR + i] = acc[i];
         __syncthreads();
         // A lane an output, the waves' sums in their order.
-        const uint32_t i = lane / M, m = lane % M;
-        if (part > 0 || lane >= NR * M || i >= rows) return;
-        float t = sums[(wave * NR + i) * M + m];
+        if (part > 0 || lane >= rows) return;
+        float t = sums[wave * NR + lane];
 #pragma unroll
-        for (uint32_t w = 1; w < KS; ++w) t += sums[((wave + w) * NR + i) * M + m];
-        g.out[(size_t)m * g.N + n0 + i] = (uint16_t)f32_to_bf16_bits(t);
+        for (uint32_t w = 1; w < KS; ++w) t += sums[(wave + w) * NR + lane];
+        g.out[n0 + lane] = (uint16_t)f32_to_bf16_bits(t);
     } else {
         if (lane > 0) return;
 #pragma unroll
         for (uint32_t i = 0; i < NR; ++i)
-#pragma unroll
-            for (int m = 0; m < M; ++m)
-                if (i < rows) g.out[(size_t)m * g.N + n0 + i] = (uint16_t)f32_to_bf16_bits(acc[i][m]);
+            if (i < rows) g.out[n0 + i] = (uint16_t)f32_to_bf16_bits(acc[i]);
     }
 }
 
-template <int M>
-int launch_vectors(const MxArgs &g, hipStream_t st) {
+int launch_row(const MxArgs &g, hipStream_t st) {
     const uint32_t groups = (g.N + VEC_NR - 1) / VEC_NR, pieces = (g.K + VEC_K - 1) / VEC_K;
     // Sixteen waves a CU, where there are as many pieces.
     const uint32_t want = (uint32_t)device_props().cus * 16;
-    auto go = [&](auto kern, uint32_t ks) {
-        hipLaunchKernelGGL(kern, dim3((groups * ks + 3) / 4), dim3(256), 0, st, g);
-        return check_launch("gemm_mx_vectors");
-    };
-    if (groups >= want || pieces < 2) return go(gemm_mx_vectors<M, 1>, 1);
-    if (groups * 2 >= want || pieces < 4) return go(gemm_mx_vectors<M, 2>, 2);
-    return go(gemm_mx_vectors<M, 4>, 4);
+    const uint32_t ks = groups >= want || pieces < 2 ? 1 : groups * 2 >= want || pieces < 4 ? 2 : 4;
+    const uint64_t wgs = ((uint64_t)groups * ks + 3) / 4;
+    RENG_REQUIRE(wgs * 256 < (1ull << 32), "%u outputs are too many for a launch", g.N);
+    const auto kern = ks == 1 ? gemm_mx_row<1> : ks == 2 ? gemm_mx_row<2> : gemm_mx_row<4>;
+    hipLaunchKernelGGL(kern, dim3((uint32_t)wgs), dim3(256), 0, st, g);
+    return check_launch("gemm_mx_row");
 }
 
 // ------------------------------------------------------------ few rows
@@ -601,10 +581,7 @@ static_assert(Tile256::BM == 256 && Tile256::BN == 256 && Tile128::BM == 128 && 
               "MX_COST's tiles");
 
 int launch_product(const MxArgs &g, hipStream_t st) {
-    if (g.M == 1) return launch_vectors<1>(g, st);
-    if (g.M == 2) return launch_vectors<2>(g, st);
-    if (g.M == 3) return launch_vectors<3>(g, st);
-    if (g.M == 4) return launch_vectors<4>(g, st);
+    if (g.M == 1) return launch_row(g, st);
     switch (mx_pick(g.M, g.N, g.K, (uint64_t)device_props().cus)) {
     case MX_RING_1x1: return launch_ring<1, 1, 4, 4>(g, st);
     case MX_RING_1x2: return launch_ring<1, 2, 4, 3>(g, st);

@@ -45,7 +45,7 @@ inline float mx_cost(int form, uint64_t M, uint64_t N, uint64_t K, uint64_t cus)
     return (float)((wgs + cus * c.per_cu - 1) / (cus * c.per_cu)) * (c.start + c.more * (float)steps);
 }
 
-// For more than four rows.
+// For more than one row.
 inline MxForm mx_pick(uint64_t M, uint64_t N, uint64_t K, uint64_t cus) {
     int best = 0;
     float us = -1.0f;
