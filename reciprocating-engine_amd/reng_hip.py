@@ -690,7 +690,7 @@ def _rows16(t, what, tokens, width):
                          f"not {t.dtype} {tuple(t.shape)} of strides {t.stride()}")
     if _T.several and t.get_device() != _T.current_device():
         raise ValueError(f"{what} is on cuda:{t.get_device()}, the current device is cuda:{_T.current_device()}")
-    return t.data_ptr(), t.stride(0)
+    return t.data_ptr(), t.stride(0) if tokens > 1 else width   # one row has no pitch
 
 
 def _heads_args(T, q, k, v, tokens, n_heads, n_kv_heads, head_dim, q_gamma, k_gamma, rope, positions, q_out):
@@ -698,7 +698,7 @@ def _heads_args(T, q, k, v, tokens, n_heads, n_kv_heads, head_dim, q_gamma, k_ga
     nq, nk = n_heads * head_dim, n_kv_heads * head_dim
     kp, k_ld = _rows16(k, "k", tokens, nk)
     vp, v_ld = (None, k_ld) if v is None else _rows16(v, "v", tokens, nk)
-    if k_ld != v_ld and tokens > 1:
+    if k_ld != v_ld:
         raise ValueError(f"k and v must have one row pitch, not {k_ld} and {v_ld}")
     qp, q_ld = (None, 0) if q is None else _rows16(q, "q", tokens, nq)
     if q is not None and q_out is None:

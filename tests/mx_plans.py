@@ -8,12 +8,16 @@ CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
 CUS = 256   # an MI355X
 SOURCE = """
 #include "mx_attention_plan.h"
+#include "mx_forms.h"
 using namespace reng;
 extern "C" void plan(size_t nh, size_t nkv, size_t hd, size_t len, size_t tokens, size_t cus, uint64_t *out) {
     const MxAttnPlan p = mxa_plan(nh, nkv, hd, len, tokens, cus);
     const uint64_t v[] = {p.hdp, (uint64_t)p.form, p.row_blocks, p.splits, p.tiles, mxa_part_bytes(p, nkv, tokens * (nh / nkv))};
     for (int i = 0; i < 6; ++i) out[i] = v[i];
 }
+extern "C" int pick(uint64_t M, uint64_t N, uint64_t K, uint64_t cus) { return mx_pick(M, N, K, cus); }
+extern "C" int forms() { return MX_FORMS; }
+extern "C" void outputs(int form, uint32_t *out) { out[0] = MX_COST[form].bm, out[1] = MX_COST[form].bn; }
 extern "C" void shape(uint32_t hdp, int form, uint32_t *out) {
     out[0] = mxa_shape(hdp, form).rows, out[1] = mxa_shape(hdp, form).tile;
 }
@@ -32,6 +36,7 @@ def lib():
                            check=True)
             _lib = ctypes.CDLL(so)
         _lib.plan.argtypes = [ctypes.c_size_t] * 6 + [ctypes.c_void_p]
+        _lib.pick.argtypes = [ctypes.c_uint64] * 4
     return _lib
 
 
@@ -46,3 +51,15 @@ def shape(hdp, form):
     out = (ctypes.c_uint32 * 2)()
     lib().shape(hdp, form, out)
     return tuple(out)
+
+
+def mx_form(M, N, K, cus=CUS):
+    """The product's form for more than one row, and the outputs of one of its workgroups."""
+    out = (ctypes.c_uint32 * 2)()
+    form = lib().pick(M, N, K, cus)
+    lib().outputs(form, out)
+    return form, tuple(out)
+
+
+def mx_forms():
+    return lib().forms()

@@ -183,3 +183,15 @@ def test_plans_cover_the_cache_within_the_workspace():
         seen.add((p["hdp"], p["form"], p["splits"] > 1))
     assert seen == {(64, f, s) for f in range(4) for s in (False, True)} | {(128, f, s) for f in range(4) for s in (False, True)} | {
         (256, f, s) for f in range(3) for s in (False, True)}   # every kernel, with and without a merge
+
+
+def test_every_form_of_the_product_is_chosen():
+    """No form is left that no product reaches, and none wastes three quarters of its rows."""
+    rng = random.Random(2)
+    seen = set()
+    for _ in range(20000):
+        M, N, K = int(2 ** rng.uniform(1, 13)), int(2 ** rng.uniform(4, 15)), 32 * int(2 ** rng.uniform(0, 10))
+        form, (bm, _) = D.mx_form(M, N, K)
+        assert bm == 16 or bm < 4 * M
+        seen.add(form)
+    assert seen == set(range(D.mx_forms()))
