@@ -27,7 +27,7 @@ constexpr MxAttnShape MXA_SHAPES[3][MXA_FORMS] = {
 };
 // The merge's launch, and its share of a megabyte of partials. Fitted with the shapes' times to graph replays of
 // every form with up to 64 splits on 24 calls (64, 128 and 256 dimensions, 1 to 1024 tokens, 0 to
-// 131071 rows); on these the choice is the fastest or within 6% of it (one: 10%).
+// 131071 rows); on these the choice is the fastest or within 5% of it (one: 8%).
 constexpr float MXA_MERGE_US = 5.5f, MXA_MERGE_US_MB = 0.55f;
 
 // Query rows that splits leave, at most (68 MB of 128 dimensions), and the cache rows of a split, at least.
