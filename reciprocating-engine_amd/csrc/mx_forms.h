@@ -21,28 +21,26 @@ enum MxForm {
     MX_FORMS,
 };
 
-// Outputs of a workgroup, stages of 256 k it takes a step, workgroups that share a CU; the start of a
-// round and a step's time (us) where there is a workgroup a CU at most, and where there are
-// more. Fitted to graph-replayed timings of every form on 32 products (M 5 to 4096, N 1024 to
-// 27648, K 576 to 27648); on these the choice is the fastest one or within 14% of it, but for
-// 64 rows [3584, 18944] (27.2 us, and 19.6 on the 32 x 32 ring).
+// Outputs of a workgroup, stages of 256 k that it takes a step, and times (us): the start and a step of a
+// CU's first workgroup, and what each further one of that CU adds to them. Fitted to graph-replayed
+// timings of every form on 156 products (M 2 to 6000, N 1024 to 27648, K 576 to 27648); on these the
+// choice is the fastest form or within 6% of it (0.3% in the mean).
 struct MxCost {
-    uint32_t bm, bn, step, per_cu;
-    float start, one, more;
+    uint32_t bm, bn, step;
+    float start, start_more, one, more;
 };
 constexpr MxCost MX_COST[MX_FORMS] = {
-    {16, 16, 4, 3, 3.0f, 0.48f, 0.64f}, {16, 32, 4, 3, 3.0f, 0.64f, 1.22f}, {32, 16, 4, 2, 2.5f, 0.64f, 0.86f},
-    {32, 32, 4, 3, 2.5f, 0.86f, 1.30f}, {64, 16, 4, 1, 2.0f, 1.04f, 0.64f}, {64, 32, 4, 1, 3.0f, 1.08f, 0.70f},
-    {64, 64, 4, 3, 4.0f, 1.40f, 3.34f}, {64, 64, 1, 3, 4.0f, 0.46f, 0.64f}, {128, 128, 1, 1, 4.5f, 0.86f, 0.50f},
-    {256, 256, 1, 1, 8.5f, 1.58f, 2.00f},
+    {16, 16, 4, 2.94f, 0.38f, 0.41f, 0.31f}, {16, 32, 4, 3.00f, 1.32f, 0.52f, 0.55f}, {32, 16, 4, 3.01f, 0.96f, 0.51f, 0.45f},
+    {32, 32, 4, 2.81f, 0.61f, 0.70f, 0.54f}, {64, 16, 4, 3.23f, 1.11f, 0.73f, 0.67f}, {64, 32, 4, 3.25f, 1.73f, 0.94f, 0.78f},
+    {64, 64, 4, 3.71f, 2.75f, 1.46f, 1.09f}, {64, 64, 1, 3.57f, 1.08f, 0.45f, 0.20f}, {128, 128, 1, 3.66f, 0.78f, 0.82f, 0.58f},
+    {256, 256, 1, 12.11f, 13.75f, 1.46f, 1.42f},
 };
 
 inline float mx_cost(int form, uint64_t M, uint64_t N, uint64_t K, uint64_t cus) {
     const MxCost &c = MX_COST[form];
     const uint64_t wgs = ((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn);
-    const uint64_t steps = ((K + 255) / 256 + c.step - 1) / c.step;
-    if (wgs <= cus) return c.start + c.one * (float)steps;
-    return (float)((wgs + cus * c.per_cu - 1) / (cus * c.per_cu)) * (c.start + c.more * (float)steps);
+    const float further = (float)((wgs + cus - 1) / cus - 1), steps = (float)(((K + 255) / 256 + c.step - 1) / c.step);
+    return c.start + c.start_more * further + steps * (c.one + c.more * further);
 }
 
 // For more than one row.
