@@ -225,15 +225,17 @@ __global__ __launch_bounds__(256) void head_norm_rope(const HeadsArgs a, uint32_
 template <int L, bool VEC, bool MX>
 int launch_lanes(const HeadsArgs &a, hipStream_t st) {
     const uint32_t heads = a.nh + 2 * a.nkv;
-    auto go = [&](auto kern, uint32_t it) {
-        const uint32_t parts = (heads + it * (256 / L) - 1) / (it * (256 / L));
-        RENG_REQUIRE((uint64_t)a.tokens * parts < (1u << 24), "%u tokens of %u heads are too many for a launch", a.tokens, heads);
-        hipLaunchKernelGGL(kern, dim3(a.tokens * parts), dim3(256), 0, st, a, parts);
-        return check_launch("head_norm_rope");
-    };
-    // Four heads a group of lanes where that leaves four workgroups a CU.
-    if ((uint64_t)a.tokens * heads >= (uint64_t)device_props().cus * 16 * (256 / L)) return go(head_norm_rope<L, 4, VEC, MX>, 4);
-    return go(head_norm_rope<L, 1, VEC, MX>, 1);
+    constexpr uint32_t G = 256 / L;
+    const uint32_t parts1 = (heads + G - 1) / G, parts4 = (heads + 4 * G - 1) / (4 * G);
+    // Four heads a group of lanes, where that fills more than half of the workgroups' lanes and leaves four
+    // workgroups a CU: 1024 tokens of 56 heads of 128 12.7 us for 13.7; but 300 tokens of 48 6.4 for
+    // 5.2, and 4000 of 15 heads of 64 20.6 for 11.8.
+    const bool four = heads > 2 * G && (uint64_t)a.tokens * parts4 >= (uint64_t)device_props().cus * 4;
+    const uint32_t parts = four ? parts4 : parts1;
+    RENG_REQUIRE((uint64_t)a.tokens * parts < (1u << 24), "%u tokens of %u heads are too many for a launch", a.tokens, heads);
+    const auto kern = four ? head_norm_rope<L, 4, VEC, MX> : head_norm_rope<L, 1, VEC, MX>;
+    hipLaunchKernelGGL(kern, dim3(a.tokens * parts), dim3(256), 0, st, a, parts);
+    return check_launch("head_norm_rope");
 }
 
 template <bool MX>
