@@ -650,9 +650,8 @@ class MxCache:
     def read(self, first, rows, k=None, v=None):
         """(k, v) bf16 [rows * n_kv_heads * head_dim] of rows first .. first + rows - 1."""
         T, n = _torch(), rows * self.n_kv_heads * self.head_dim
-        k = T.empty(n, dtype=T.bf16, device=self.device) if k is None else k
-        v = T.empty(n, dtype=T.bf16, device=self.device) if v is None else v
-        _check(lib().reng_hip_cache_read_mxfp4(self._here(), first, rows, _16bit(k, "k", n), _16bit(v, "v", n), T.stream()))
+        (k, kp), (v, vp) = _out16(T, k, "k", n, self.tensors[0]), _out16(T, v, "v", n, self.tensors[0])
+        _check(lib().reng_hip_cache_read_mxfp4(self._here(), first, rows, kp, vp, T.stream()))
         return k, v
 
 
@@ -685,34 +684,41 @@ def _rows16(t, what, tokens, width):
     with contiguous columns."""
     if t.dim() != 2:
         return _16bit(t, what, tokens * width), width
-    if t.dtype not in _T.is16 or not t.is_cuda or t.stride(1) != 1 or t.shape[0] < tokens or t.shape[1] < width:
+    (rows, cols), (ld, one) = t.shape, t.stride()
+    if t.dtype not in _T.is16 or not t.is_cuda or one != 1 or rows < tokens or cols < width:
         raise ValueError(f"{what} must be bf16 (or its bits) rows on the GPU, [{tokens}, {width}] with contiguous columns, "
                          f"not {t.dtype} {tuple(t.shape)} of strides {t.stride()}")
     if _T.several and t.get_device() != _T.current_device():
         raise ValueError(f"{what} is on cuda:{t.get_device()}, the current device is cuda:{_T.current_device()}")
-    return t.data_ptr(), t.stride(0) if tokens > 1 else width   # one row has no pitch
+    return t.data_ptr(), ld if tokens > 1 else width   # one row has no pitch
 
 
-def _heads_args(T, q, k, v, tokens, n_heads, n_kv_heads, head_dim, q_gamma, k_gamma, rope, positions, q_out):
-    """What both calls share: the rows' addresses and pitches, gammas, rope, positions, and q_out."""
-    nq, nk = n_heads * head_dim, n_kv_heads * head_dim
+def _out16(T, t, what, n, like):
+    """(t, its address), allocated like `like` where t is None."""
+    if t is None:
+        t = T.empty(n, dtype=T.bf16, device=like.device)
+        return t, t.data_ptr()
+    return t, _16bit(t, what, n)
+
+
+def _heads_args(T, q, k, v, tokens, n_heads, n_kv_heads, head_dim, q_gamma, k_gamma, rope, positions):
+    """What both calls share: the rows' addresses and pitches, and gammas, rope and positions."""
+    nk = n_kv_heads * head_dim
     kp, k_ld = _rows16(k, "k", tokens, nk)
     vp, v_ld = (None, k_ld) if v is None else _rows16(v, "v", tokens, nk)
     if k_ld != v_ld:
         raise ValueError(f"k and v must have one row pitch, not {k_ld} and {v_ld}")
-    qp, q_ld = (None, 0) if q is None else _rows16(q, "q", tokens, nq)
-    if q is not None and q_out is None:
-        q_out = T.empty(tokens * nq, dtype=T.bf16, device=q.device)
+    qp, q_ld = (None, 0) if q is None else _rows16(q, "q", tokens, n_heads * head_dim)
     ref = pos = None
     if rope is not None:
-        if _T.several and rope.device.index != _T.current_device():
-            raise ValueError(f"the tables are on {rope.device}, the current device is cuda:{_T.current_device()}")
+        if T.several and rope.device.index != T.current_device():
+            raise ValueError(f"the tables are on {rope.device}, the current device is cuda:{T.current_device()}")
         if positions is None or positions.dtype != T.i32:
             raise ValueError("positions must be int32 [axes, tokens]")
         ref, pos = rope._ref, _at(positions, "positions", rope.axes * tokens, 4)
     gq = None if q_gamma is None else _f32(q_gamma, "q_gamma", head_dim)
     gk = None if k_gamma is None else _f32(k_gamma, "k_gamma", head_dim)
-    return (qp, q_ld, kp, vp, k_ld, gq, gk, ref, pos, None if q_out is None else _16bit(q_out, "q_out", tokens * nq)), q_out
+    return (qp, q_ld, kp, vp, k_ld), (gq, gk), (ref, pos)
 
 
 def head_norm_rope_bf16(q, k, v, tokens, n_heads, n_kv_heads, head_dim, q_gamma=None, k_gamma=None, eps=1e-6, rope=None,
@@ -721,14 +727,16 @@ def head_norm_rope_bf16(q, k, v, tokens, n_heads, n_kv_heads, head_dim, q_gamma=
     (rope, a Rope, at positions int32 [axes, tokens]), values as they are, bf16 [tokens, heads * head_dim]. q, k and v
     are bf16 rows, which may be column ranges of a wider tensor; k_rows and v_rows a bf16 cache's rows."""
     T = _torch()
-    nk = n_kv_heads * head_dim
-    a, q_out = _heads_args(T, q, k, v, tokens, n_heads, n_kv_heads, head_dim, q_gamma, k_gamma, rope, positions, q_out)
-    k_rows = T.empty(tokens * nk, dtype=T.bf16, device=k.device) if k_rows is None else k_rows
-    if v is not None and v_rows is None:
-        v_rows = T.empty(tokens * nk, dtype=T.bf16, device=k.device)
-    _check(lib().reng_hip_head_norm_rope_bf16(*a[:5], tokens, n_heads, n_kv_heads, head_dim, *a[5:7], eps, *a[7:],
-                                              _16bit(k_rows, "k_rows", tokens * nk),
-                                              None if v_rows is None else _16bit(v_rows, "v_rows", tokens * nk), T.stream()))
+    nq, nk = tokens * n_heads * head_dim, tokens * n_kv_heads * head_dim
+    rows, gammas, at = _heads_args(T, q, k, v, tokens, n_heads, n_kv_heads, head_dim, q_gamma, k_gamma, rope, positions)
+    qp = vp = None
+    if q is not None or q_out is not None:
+        q_out, qp = _out16(T, q_out, "q_out", nq, k)
+    k_rows, kp = _out16(T, k_rows, "k_rows", nk, k)
+    if v is not None or v_rows is not None:
+        v_rows, vp = _out16(T, v_rows, "v_rows", nk, k)
+    _check(lib().reng_hip_head_norm_rope_bf16(*rows, tokens, n_heads, n_kv_heads, head_dim, *gammas, eps, *at, qp, kp, vp,
+                                              T.stream()))
     return q_out, k_rows, v_rows
 
 
@@ -736,9 +744,12 @@ def head_norm_rope_mxfp4(q, k, v, tokens, n_heads, cache, first, q_gamma=None, k
                          positions=None, q_out=None):
     """q_out: head_norm_rope_bf16 with keys and values quantized into rows first .. first + tokens - 1 of an MxCache."""
     T = _torch()
-    a, q_out = _heads_args(T, q, k, v, tokens, n_heads, cache.n_kv_heads, cache.head_dim, q_gamma, k_gamma, rope, positions,
-                           q_out)
-    _check(lib().reng_hip_head_norm_rope_mxfp4(*a[:5], tokens, n_heads, *a[5:7], eps, *a[7:], cache._here(), first, T.stream()))
+    hd = cache.head_dim
+    rows, gammas, at = _heads_args(T, q, k, v, tokens, n_heads, cache.n_kv_heads, hd, q_gamma, k_gamma, rope, positions)
+    qp = None
+    if q is not None or q_out is not None:
+        q_out, qp = _out16(T, q_out, "q_out", tokens * n_heads * hd, k)
+    _check(lib().reng_hip_head_norm_rope_mxfp4(*rows, tokens, n_heads, *gammas, eps, *at, qp, cache._here(), first, T.stream()))
     return q_out
 
 
