@@ -469,11 +469,12 @@ typedef struct reng_hip_rope {
  * columns; k and v [tokens, kv_ld] (the columns of a fused projection's output row, for
  * one); q_gamma, k_gamma f32 [head_dim], NULL for no norm; rope NULL for no rotation,
  * else positions device int32 [axes, tokens]: a token with a position outside the
- * tables gets NaN in the values it would rotate. Out: q_out bf16 [tokens, n_heads * head_dim] (may be q with that
- * pitch), k_rows and v_rows [tokens, n_kv_heads * head_dim] (may be k, v with that pitch;
- * these rows of a bf16 cache; v and v_rows may both be NULL). n_heads may be 0, with q
- * and q_out NULL. head_dim a multiple of 32 up to 256, tokens < 2^22, at most 4096 heads
- * of each; fastest on 16-byte aligned rows. */
+ * tables gets NaN in the values it would rotate. Out: q_out bf16 [tokens, n_heads *
+ * head_dim] (may be q with that pitch), k_rows and v_rows [tokens, n_kv_heads *
+ * head_dim] (may be k, v with that pitch; these rows of a bf16 cache; v and v_rows may
+ * both be NULL). n_heads may be 0, with q and q_out NULL. head_dim a multiple of 32 up
+ * to 256, tokens < 2^22, at most 4096 heads of each, eps finite and at least 0; fastest
+ * on 16-byte aligned rows. */
 RENG_HIP_API int reng_hip_head_norm_rope_bf16(const uint16_t *q, size_t q_ld, const uint16_t *k, const uint16_t *v,
                                               size_t kv_ld, size_t tokens, size_t n_heads, size_t n_kv_heads,
                                               size_t head_dim, const float *q_gamma, const float *k_gamma, float eps,
@@ -497,14 +498,15 @@ RENG_HIP_API size_t reng_hip_attention_mxfp4_workspace_bytes(size_t n_heads, siz
 /* reng_hip_attention_tree over a cache held in 4 bits, for one token or many: rows 0 ..
  * len - 1 are context, rows len .. len + tokens - 1 the tokens' own, mask as there (NULL:
  * a chain). Scores, their maxima and sums are f32; each weight is rounded to bf16 where
- * it meets its value, and values up to 2^102 in magnitude overflow none, as there. Rows a token does not
- * see take no part, whatever they hold. A row that is seen and has a scale byte of 253 or more
- * in its key or its value (a NaN block, or magnitudes of some 2^128) makes all of the token's
- * outputs NaN; so does a NaN or +inf score. A token that sees nothing gives zeros, one whose scores are all
- * -inf NaN. q and out bf16 [tokens, n_heads * head_dim], 16-byte aligned; 1 <= tokens <=
- * RENG_HIP_TREE_MAX_TOKENS, len + tokens at most RENG_HIP_ATTENTION_MAX_LEN and the
- * capacity; workspace 16-byte aligned. Asynchronous on stream; calls that share a
- * workspace must be ordered (one stream). */
+ * it meets its value, and values up to 2^102 in magnitude overflow none, as there. Rows
+ * a token does not see take no part, whatever they hold. A row that is seen and has a
+ * scale byte of 253 or more in its key or its value (a NaN block, or magnitudes of some
+ * 2^128) makes all of the token's outputs NaN; so does a NaN or +inf score those of its
+ * head. A token that sees nothing gives zeros, one whose scores are all -inf NaN. q and
+ * out bf16 [tokens, n_heads * head_dim], 16-byte aligned; scale finite, of any sign;
+ * 1 <= tokens <= RENG_HIP_TREE_MAX_TOKENS, len + tokens at most
+ * RENG_HIP_ATTENTION_MAX_LEN and the capacity; workspace 16-byte aligned. Asynchronous
+ * on stream; calls that share a workspace must be ordered (one stream). */
 RENG_HIP_API int reng_hip_attention_mxfp4(const uint16_t *q, const reng_hip_mx_cache *cache, size_t n_heads, size_t len,
                                           size_t tokens, const uint32_t *mask, float scale, void *workspace,
                                           size_t workspace_bytes, uint16_t *out, void *stream);

@@ -9,9 +9,9 @@
 // rounded on the way to the matrix cores.
 //
 // The query rows of a key/value head (row r: token r / per, query head r % per of the per
-// that share it) go 16 to a wave, eight waves taking tiles of 32 cache rows of their own in turn, or, where there are many,
-// 32 to a wave over tiles that a workgroup shares in LDS. Splits of the cache merge in a
-// second kernel (mx_attention_plan.h).
+// that share it) go 16 to a wave, eight waves taking tiles of 32 cache rows of their own in
+// turn, or, where there are many, 32 to a wave over tiles that a workgroup shares in LDS.
+// Splits of the cache merge in a second kernel (mx_attention_plan.h).
 //
 // Few rows: per tile a wave forms S^T = K Q^T on v_mfma_f32_16x16x32_bf16. Lane l has key l % 16 and,
 // of its dimensions, the quarter l / 16: the order in which dimensions are summed is free, so
@@ -20,9 +20,14 @@
 // 4 (l / 16), which is how O^T = V^T P^T takes the weights. V^T comes from LDS, where a
 // wave puts a tile's values as bf16, by transposing reads.
 //
-// A row whose key or value holds a scale from 253 on (NaN, or magnitudes bf16 ends at) counts as NaN: its
-// key's scale becomes NaN and its value's 1, so that its score decides who meets it, and a
-// weight of 0 takes nothing from a value.
+// A row whose key or value holds a scale from 253 on (NaN, or magnitudes bf16 ends at)
+// counts as NaN: its key's scale becomes NaN and its value's 1, so that its score decides
+// who meets it, and a weight of 0 takes nothing from a value.
+//
+// What bounds it: one token after 32768 rows (32 heads on 8, 36 MB of cache) 15.7 us, 12.9 of
+// them the rows' kernel and 3.9 the merge: two launches and the start of each; 131071 rows
+// 29 to 37. A chain of 1024 after 16384 (40 on 8) 351 us, 1.0 PFLOP/s: the matrix cores and, in
+// turn with them, the exponentials.
 #include <type_traits>
 
 #include "common.h"
@@ -128,8 +133,9 @@ __device__ __forceinline__ uint32_t value_slot(uint32_t r, uint32_t c) {
 
 // ------------------------------------------------------------ few query rows
 //
-// NW waves, each with the same 16 query rows and tiles of its own, whose codes are on the way while the
-// one before is worked on.
+// NW waves, each with the same 16 query rows and tiles of its own, whose codes are on the
+// way while the one before is worked on. One token after 32768: two and four tiles ahead 18.3 and
+// 19.9 us where one takes 17.5; four and sixteen waves 19.2 and 19.3 where eight take 17.5.
 template <int HD, int NW>
 __global__ __launch_bounds__(64 * NW) void attention_mxfp4(const MxAttn a) {
     constexpr int ST = HD / 32, DT = HD / 16;   // products a score; tiles of dimensions
@@ -189,15 +195,18 @@ __global__ __launch_bounds__(64 * NW) void attention_mxfp4(const MxAttn a) {
     const __amdgpu_buffer_rsrc_t rkc = rows_of(a.kc, head, rows, rowb), rks = rows_of(a.ks, head, rows, a.sp);
     const __amdgpu_buffer_rsrc_t rvc = rows_of(a.vc, head, rows, rowb), rvs = rows_of(a.vs, head, rows, a.sp);
     auto fetch = [&](uint32_t tile) __attribute__((always_inline)) {
-        auto load = [&](Codes &v, const __amdgpu_buffer_rsrc_t &rc, const __amdgpu_buffer_rsrc_t &rs, uint32_t j) __attribute__((always_inline)) {
+        auto load = [&](Codes &v, const __amdgpu_buffer_rsrc_t &rc, const __amdgpu_buffer_rsrc_t &rs,
+                        uint32_t j) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < CH; ++i) {
                 v.s[i] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(rs, at_scale[i] + j * a.sp, 0, 0);
                 if constexpr (LB == 8) {
-                    const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rc, at_codes[i] + j * rowb, 0, 0));
+                    const u32x2 x =
+                        __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rc, at_codes[i] + j * rowb, 0, 0));
                     v.w[0] = x.x, v.w[1] = x.y;
                 } else {
-                    const u32x4 x = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rc, at_codes[i] + j * rowb, 0, 0));
+                    const u32x4 x =
+                        __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rc, at_codes[i] + j * rowb, 0, 0));
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v.w[4 * i + e] = x[e];
                 }

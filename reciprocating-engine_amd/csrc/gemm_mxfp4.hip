@@ -4,7 +4,8 @@
 //
 // a [M, K], b [N, K] codes with a scale byte for 32 of k. v_mfma_scale_f32_16x16x128
 // takes both as they lie: lane l holds row l % 16 of either operand and the block of 32 codes
-// l / 16 of 128, with that block's scale byte.
+// l / 16 of 128, with that block's scale byte. One row runs on dot products, more on rings or
+// tiles (mx_forms.h).
 #include <type_traits>
 
 #include "common.h"
@@ -183,6 +184,12 @@ int launch_row(const MxArgs &g, hipStream_t st) {
 // its own, S - 1 of them in flight, and waits for nobody until the end. The copies are 8 rows x
 // 128 bytes an instruction. The weight is the matrix instruction's first operand, so the
 // result's lane has activation row l % 16 and the four weight rows from 4 (l / 16).
+//
+// What bounds it: the fetch of the weight and, beside it, of the rows of a, which every workgroup
+// brings through L2 once more: [3584, 18944] with 16, 24 and 32 rows 13.5, 15.2 and 16.4 us, one row
+// on dot products 10.9. Not the depth of the rings: four to eight waves of two to four stages take
+// 15.2 to 15.9 at 24 rows. Operands fetched straight into registers (64 bytes of a row an
+// instruction) took 18 to 23.
 template <int MT, int NT, int S>
 struct RingShape {
     static constexpr int ROWS = 16 * (MT + NT), STAGE = ROWS * ROWB, COPIES = ROWS / 8;
@@ -306,6 +313,11 @@ int launch_ring(const MxArgs &g, hipStream_t st) {
 // fragments; the next stage's first fragments and scales are read behind the barrier before
 // this stage's last two rows of products. Rows past M and N and codes past K lie outside the
 // tile's buffer resources and arrive as zeros.
+//
+// What bounds the 256 x 256 tile: the copies, at the clock that random data leaves (3.1 PFLOP/s;
+// the instruction out of registers 6.5, of zeros 8.7). [4096]^3 takes 44.5 us and [1024, 27648, 5120]
+// 94; without its copies 41 and 83, without three of four products 36 and 80, with zeros for
+// data 38 and 86. Tried: no turns 47 and 102, four waves of 128 x 128 43 and 96 at best.
 template <int TM_, int TN_, int WGM_, int WGN_, int S_>
 struct MxTile {
     static constexpr int TM = TM_, TN = TN_, WGM = WGM_, WGN = WGN_, S = S_, NW = WGM * WGN;
@@ -319,7 +331,8 @@ struct MxTile {
     static constexpr int LDS = RING > OUT ? RING : OUT;
     static constexpr bool TURNS = TM == 8;   // the halves of the rows take turns
     static_assert(!TURNS || (WGM == 2 && WGN == 4 && S == 2 && LS == 1), "a wave of each half on a SIMD");
-    static_assert(LA * 8 * NW == BM && LB * 8 * NW == BN && LS * 64 * NW == BM + BN && BM % 64 == 0, "copies split evenly");
+    static_assert(LA * 8 * NW == BM && LB * 8 * NW == BN && LS * 64 * NW == BM + BN && BM % 64 == 0,
+                  "copies split evenly");
     static_assert(TM % 2 == 0 && (S - 1) * LOADS + LS < 64 && S >= 2 && S <= 3 && LDS <= 160 * 1024, "vmcnt range, LDS");
 };
 
@@ -341,7 +354,8 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_mx_tiles(MxArgs g, uint32_t t
     const __amdgpu_buffer_rsrc_t rsb = resource(g.sb + (size_t)n0 * sp, (size_t)rows_b * sp);
     // A copy brings 8 rows: lane l the chunk of row l / 8 that lands in slot l % 8. The whole
     // offset is the lane's (a scalar one would not count in the range check).
-    auto copy_rows = [&](const __amdgpu_buffer_rsrc_t &rs, uint8_t *to, uint32_t r, uint32_t step) __attribute__((always_inline)) {
+    auto copy_rows = [&](const __amdgpu_buffer_rsrc_t &rs, uint8_t *to, uint32_t r,
+                         uint32_t step) __attribute__((always_inline)) {
         step = min(step, KB - 1);   // past the last stage: that one again, into a slot that is not read
         const uint32_t ko = step * ROWB, left = kb - ko;
         const uint32_t ch = 16 * ((lane % 8) ^ pipe::swz<8>((r + lane / 8) & 31));

@@ -4,9 +4,10 @@
 //   code = e2m1(x / s), to nearest, ties to the even code
 //
 // A quotient below 7 rounds to 6 at most, so nothing is clipped; a scale one step
-// smaller would clip, one larger would lose a bit. The conversions of gfx950 take the scale's
-// exponent byte in the place of a float's exponent, its 0 for 2^-127 and its 255 for NaN
-// (checked on the card over all bf16 values and scale bytes whose quotient is below 7, and all codes and scale bytes).
+// smaller would clip, one larger would lose a bit. The conversions of gfx950 take the
+// scale's exponent byte in the place of a float's exponent, its 0 for 2^-127 and its 255
+// for NaN (checked on the card over all bf16 values and scale bytes whose quotient is
+// below 7, and over all codes and scale bytes).
 #pragma once
 
 #include "common.h"

@@ -3,7 +3,8 @@
 //
 // Bound: HBM. The quantizer reads a value once (2 or 4 bytes) and writes 17/32 of a
 // byte; a lane holds 8 values, four lanes a block, sixteen the 128 columns whose four
-// scales are a word.
+// scales are a word. bf16 [14336, 4096]: 28.2 us (5.3 TB/s), the values back 22.8 us (6.5);
+// a copy of 1 GiB reaches 5.1. 24 rows of 18944: 3.0 and 2.7 us, the launch.
 #include "mx.h"
 
 namespace reng {
@@ -194,7 +195,9 @@ RENG_HIP_API int reng_hip_quantize_mxfp4(const void *w, int dtype, size_t rows, 
     const dim3 grid(grid_of(rows * units, 256 / LANES, 32));
     hipStream_t st = static_cast<hipStream_t>(stream);
     uint32_t *sc = reinterpret_cast<uint32_t *>(scales);
-    auto launch = [&](auto kern, auto *in) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, in, rows, cols, ld, units, codes, sc); };
+    auto launch = [&](auto kern, auto *in) {
+        hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, in, rows, cols, ld, units, codes, sc);
+    };
     if (dtype == RENG_HIP_BF16) {
         const uint16_t *in = static_cast<const uint16_t *>(w);
         vec ? launch(quantize_mx<uint16_t, true>, in) : launch(quantize_mx<uint16_t, false>, in);
