@@ -713,8 +713,8 @@ def _heads_args(T, q, k, v, tokens, n_heads, n_kv_heads, head_dim, q_gamma, k_ga
     if rope is not None:
         if T.several and rope.device.index != T.current_device():
             raise ValueError(f"the tables are on {rope.device}, the current device is cuda:{T.current_device()}")
-        if positions is None or positions.dtype != T.i32:
-            raise ValueError("positions must be int32 [axes, tokens]")
+        if positions is None or positions.dtype != T.i32 or (rope.axes > 1 and positions.numel() != rope.axes * tokens):
+            raise ValueError(f"positions must be int32 [{rope.axes}, {tokens}]")
         ref, pos = rope._ref, _at(positions, "positions", rope.axes * tokens, 4)
     gq = None if q_gamma is None else _f32(q_gamma, "q_gamma", head_dim)
     gk = None if k_gamma is None else _f32(k_gamma, "k_gamma", head_dim)

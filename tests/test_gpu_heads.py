@@ -281,3 +281,11 @@ def test_read_one_of_both(R):
         args = (None, out.data_ptr()) if i else (out.data_ptr(), None)
         assert L.reng_hip_cache_read_mxfp4(cache._ref, 2, 4, *args, T.stream()) == 0
         assert torch.equal(out, both[i])
+
+
+def test_positions_of_another_number_of_tokens_are_refused(R):
+    """With several axes an axis' positions start where the one before it ends: more of them than tokens would shift them."""
+    c = Case(6, 2, 2, 64, 64, 2, True, seed=12)
+    for tokens, positions in ((5, c.positions), (6, c.positions[:1]), (6, c.positions.long()), (6, None)):
+        with pytest.raises(ValueError, match="positions"):
+            R.head_norm_rope_bf16(c.q, c.k, c.v, tokens, 2, 2, 64, **dict(c.args(R), positions=positions))

@@ -47,6 +47,8 @@ def test_product_refusals():
     refused(g(P, P, P, P, 4, 8, (1 << 22) + 32, P, None), "too large")
     refused(g(P, P, P, P, 2**31, 8, 32, P, None), "too large")
     refused(g(P, P, P, P, 2**31 - 1, 2**31 - 1, 32, P, None), "too many for a launch")
+    refused(g(P, P, P, P, 1, 2**31 - 1, 32, P, None), "too many for a launch")
+    refused(g(P, P, P, P, 16, 2**31 - 1, 32, P, None), "too many for a launch")
     refused(g(P, None, P, P, 4, 8, 64, P, None), "null")
     refused(g(P, P, ctypes.c_void_p(72), P, 4, 8, 64, P, None), "16-byte")
     refused(g(P, P, P, ctypes.c_void_p(65), 4, 8, 64, P, None), "4-byte")
@@ -155,6 +157,8 @@ def test_the_binding_refuses_rows_that_are_too_short():
             R._rows16(t, "k", tokens, width)
     with pytest.raises(ValueError, match="32 pairs|pairs"):
         R.Rope(torch.zeros(4, 64), torch.zeros(4, 64), sections=(16, 17))
+    with pytest.raises(ValueError, match="pitch"):
+        R._heads_args(R._T, dev(4, 64), dev(4, 64)[:, :32], dev(4, 32), 4, 2, 1, 32, None, None, None, None)
     with pytest.raises(ValueError, match="shapes"):
         R.Rope(torch.zeros(4, 64), torch.zeros(4, 32))
 
