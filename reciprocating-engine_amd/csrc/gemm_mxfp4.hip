@@ -4,8 +4,8 @@
 //
 // a [M, K], b [N, K] codes with a scale byte for 32 of k. v_mfma_scale_f32_16x16x128
 // takes both as they lie: lane l holds row l % 16 of either operand and the block of 32 codes
-// l / 16 of 128, with that block's scale byte. One row runs on dot products, more on rings or
-// tiles (mx_forms.h).
+// l / 16 of 128, with that block's scale byte. One row of a runs on its diagonal, more on rings
+// or tiles (mx_forms.h).
 #include <type_traits>
 
 #include "common.h"
@@ -75,80 +75,63 @@ __device__ __forceinline__ uint32_t within(uint32_t pair, uint32_t q, uint32_t b
 
 // ------------------------------------------------------------ one row
 //
-// A wave takes NR rows of b, 2048 of k at a time: a lane has one block of 32 codes of each and of
-// a. The codes become bf16 pairs without their scale, whose products (quarters of at most 36)
-// v_dot2_f32_bf16 sums exactly; the two scale bytes then move the sum's exponent. KS waves share
-// rows and take pieces of k in turn. All of a wave's loads of a piece are on the way while it works
-// on the one before. The weight's bytes and the launch are the time: [14336, 4096] 8.7 us and
-// [27648, 5120] 19.1 (rings 9.7 and 19.6), [4096, 14336] 9.0 (9.2), [4096, 4096] 4.2 (4.1). Two, four or
-// eight rows of b a wave are within 10%. More rows of a cost 1.7 us each at [14336, 4096]: with
-// two the rings are faster (10.0 us; here it would be 10.8) and with four by far (9.7 and 14.1).
-constexpr uint32_t VEC_NR = 4, VEC_K = 2048;
-
-__device__ __forceinline__ bf16x2_t pair_of(uint32_t d, int i) {
-    switch (i) {
-    case 0: return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, 1.0f, 0);
-    case 1: return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, 1.0f, 1);
-    case 2: return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, 1.0f, 2);
-    default: return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, 1.0f, 3);
-    }
-}
+// A wave takes NR rows of b, 2048 of k at a time: lane l has block l of 32 codes of each and of a. The
+// matrix instruction pairs row i of one operand, lanes i, 16 + i, 32 + i and 48 + i, with row j of
+// the other: on the diagonal i = j are the products of a block with its own, whose sum, over the
+// diagonal too, is the output. The rest of the tile is not used, and costs less than decoding would
+// (codes to bf16 and dot products: [14336, 4096] 8.8 us). KS waves share rows and take pieces of k in
+// turn. The weight's bytes and the launch are the time: [14336, 4096] 8.4 us, [4096, 14336] 8.9,
+// [27648, 5120] 17.1, [4096, 4096] 3.9 (rings 9.7, 9.2, 19.6 and 4.1), [128256, 4096] 50.6, 5.5 TB/s. One
+// row of b a wave takes 8.7 us on the first, four 8.7, eight 10.0; the next piece's loads ahead are
+// equal. Of a more rows than one are faster on the rings on most products (two: 9.3 us, 9.9 and
+// 4.6 here, 10.1, 9.3 and 4.1 there; four 12.9 and 10.1).
+constexpr uint32_t ROW_NR = 2, ROW_K = 2048;
 
 template <int KS>
 __global__ __launch_bounds__(256) void gemm_mx_row(MxArgs g) {
-    constexpr uint32_t NR = VEC_NR, GROUPS = 4 / KS;   // groups of rows of a workgroup
+    constexpr uint32_t NR = ROW_NR, GROUPS = 4 / KS;   // groups of rows of a workgroup
     __shared__ float sums[4 * NR];
     const uint32_t lane = threadIdx.x & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % KS, grp = wave / KS;
     const uint32_t n0 = (blockIdx.x * GROUPS + grp) * NR, kb = g.K / 2, sp = (uint32_t)scale_pitch(g.K);
-    const uint32_t pieces = (g.K + VEC_K - 1) / VEC_K;
+    const uint32_t pieces = (g.K + ROW_K - 1) / ROW_K;
     const uint32_t rows = n0 < g.N ? min(NR, g.N - n0) : 0;   // rows past N arrive as zeros
     const __amdgpu_buffer_rsrc_t rb = resource(g.b + (size_t)n0 * kb, (size_t)rows * kb);
     const __amdgpu_buffer_rsrc_t rsb = resource(g.sb + (size_t)n0 * sp, (size_t)rows * sp);
     const __amdgpu_buffer_rsrc_t ra = resource(g.a, kb), rsa = resource(g.sa, sp);
-    struct Piece {
-        u32x4 a, b[NR];
-        uint32_t sa, sb[NR];
-    };
-    auto fetch = [&](uint32_t p) __attribute__((always_inline)) {
-        Piece v;
-        const uint32_t at = p * (VEC_K / 2) + lane * 16, blk = p * (VEC_K / BLOCK) + lane;
-        const bool on = at < kb;   // past K codes of zeros
+    f32x4 acc[NR];
+#pragma unroll
+    for (uint32_t i = 0; i < NR; ++i) acc[i] = f32x4{0, 0, 0, 0};
+    for (uint32_t p = part; p < pieces; p += KS) {
+        const uint32_t at = p * (ROW_K / 2) + lane * 16, blk = p * (ROW_K / BLOCK) + lane;
+        const bool on = at < kb;   // past K zeros
         auto codes = [&](const __amdgpu_buffer_rsrc_t &r, uint32_t row) __attribute__((always_inline)) {
             return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, on ? at + row * kb : NOTHING, 0, 0));
         };
         auto scale = [&](const __amdgpu_buffer_rsrc_t &r, uint32_t row) __attribute__((always_inline)) {
             return (uint32_t)(uint8_t)__builtin_amdgcn_raw_buffer_load_b8(r, on ? blk + row * sp : NOTHING, 0, 0);
         };
+        u32x4 b[NR];
+        uint32_t sb[NR];
 #pragma unroll
-        for (uint32_t i = 0; i < NR; ++i) v.b[i] = codes(rb, i), v.sb[i] = scale(rsb, i);
-        v.a = codes(ra, 0), v.sa = scale(rsa, 0);
-        return v;
-    };
-    float acc[NR] = {};
-    Piece v;
-    if (part < pieces) v = fetch(part);
-    for (uint32_t p = part; p < pieces; p += KS) {
-        const Piece w = v;
-        if (p + KS < pieces) v = fetch(p + KS);
-        bf16x2_t x[16];
+        for (uint32_t i = 0; i < NR; ++i) b[i] = codes(rb, i), sb[i] = scale(rsb, i);
+        const u32x4 a = codes(ra, 0);
+        const uint32_t sa = scale(rsa, 0);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = pair_of(w.a[e / 4], e % 4);
-#pragma unroll
-        for (uint32_t i = 0; i < NR; ++i) {
-            float s = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s = __builtin_amdgcn_fdot2_f32_bf16(x[e], pair_of(w.b[i][e / 4], e % 4), s, false);
-            s = __builtin_amdgcn_ldexpf(s, (int)(w.sa + w.sb[i]) - 2 * (int)ONE_BYTE);
-            acc[i] += max(w.sa, w.sb[i]) == NAN_BYTE ? __builtin_nanf("") : s;
-        }
+        for (uint32_t i = 0; i < NR; ++i) acc[i] = mma<0>(b[i], sb[i], a, sa, acc[i]);
     }
+    // Lane l has rows 4 (l / 16) + e of column l % 16.
+    const uint32_t e = lane % 16 - 4 * (lane / 16);
+    float sum[NR];
 #pragma unroll
-    for (uint32_t i = 0; i < NR; ++i) acc[i] = wave_sum_dpp(acc[i]);
+    for (uint32_t i = 0; i < NR; ++i) {
+        const f32x4 x = acc[i];
+        sum[i] = wave_sum_dpp(e == 0 ? x[0] : e == 1 ? x[1] : e == 2 ? x[2] : e == 3 ? x[3] : 0.0f);
+    }
     if constexpr (KS > 1) {
         if (lane == 0)
 #pragma unroll
-            for (uint32_t i = 0; i < NR; ++i) sums[wave * NR + i] = acc[i];
+            for (uint32_t i = 0; i < NR; ++i) sums[wave * NR + i] = sum[i];
         __syncthreads();
         // A lane an output, the waves' sums in their order.
         if (part > 0 || lane >= rows) return;
@@ -160,13 +143,13 @@ __global__ __launch_bounds__(256) void gemm_mx_row(MxArgs g) {
         if (lane > 0) return;
 #pragma unroll
         for (uint32_t i = 0; i < NR; ++i)
-            if (i < rows) g.out[n0 + i] = (uint16_t)f32_to_bf16_bits(acc[i]);
+            if (i < rows) g.out[n0 + i] = (uint16_t)f32_to_bf16_bits(sum[i]);
     }
 }
 
 int launch_row(const MxArgs &g, hipStream_t st) {
-    const uint32_t groups = (g.N + VEC_NR - 1) / VEC_NR, pieces = (g.K + VEC_K - 1) / VEC_K;
-    // Sixteen waves a CU, where there are as many pieces.
+    const uint32_t groups = (g.N + ROW_NR - 1) / ROW_NR, pieces = (g.K + ROW_K - 1) / ROW_K;
+    // Sixteen waves a CU, where there are as many pieces (eight: [4096, 14336] 9.8 us for 8.9).
     const uint32_t want = (uint32_t)device_props().cus * 16;
     const uint32_t ks = groups >= want || pieces < 2 ? 1 : groups * 2 >= want || pieces < 4 ? 2 : 4;
     const uint64_t wgs = ((uint64_t)groups * ks + 3) / 4;
@@ -187,7 +170,7 @@ int launch_row(const MxArgs &g, hipStream_t st) {
 //
 // What bounds it: the fetch of the weight and, beside it, of the rows of a, which every workgroup
 // brings through L2 once more: [3584, 18944] with 16, 24 and 32 rows 13.5, 15.2 and 16.4 us, one row
-// on dot products 10.9. Not the depth of the rings: four to eight waves of two to four stages take
+// by itself 10.1. Not the depth of the rings: four to eight waves of two to four stages take
 // 15.2 to 15.9 at 24 rows. Operands fetched straight into registers (64 bytes of a row an
 // instruction) took 18 to 23.
 template <int MT, int NT, int S>

@@ -170,6 +170,19 @@ def test_a_nan_block_is_its_rows_alone(R, M, N, K):
     assert torch.equal(torch.isnan(out), want)
 
 
+@pytest.mark.parametrize("N,K", [(101, 4096), (33, 1056), (7, 18944)])
+def test_nan_blocks_of_one_row(R, N, K):
+    """With one row of activations, NaN weights are their outputs alone, a NaN activation is all of them."""
+    a, b = operand(1, K, 3), operand(N, K, 4)
+    b[1][5, 0], b[1][N - 1, -1] = 255, 255
+    out = R.gemm_mxfp4(*X.pack(*a), *X.pack(*b), 1, N, K)
+    want = torch.zeros(N, dtype=torch.bool, device="cuda")
+    want[5] = want[N - 1] = True
+    assert torch.equal(torch.isnan(out), want)
+    a[1][0, K // 64] = 255
+    assert torch.isnan(R.gemm_mxfp4(*X.pack(*a), *X.pack(*b), 1, N, K)).all()
+
+
 def test_scales_of_both_ends(R):
     """Scales whose product is far from 1: 2^-126 by 2^100, and products that leave f32."""
     M, N, K = 4, 32, 256
