@@ -406,11 +406,13 @@ class _Torch:
         self.i32 = torch.int32
         self.several = torch.cuda.device_count() > 1
         self.current_device = torch.cuda.current_device
+        # Without a look at whether the GPU is initialised, which tensors on it say.
+        self.device_index = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         self.raw_stream = raw or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
     def stream(self):
-        return self.raw_stream(self.current_device())
+        return self.raw_stream(self.device_index())
 
 
 def _torch():
@@ -569,6 +571,14 @@ MX_BLOCK = 32
 ROPE_MAX_AXES = 4
 
 
+def _out16(T, t, what, n, like):
+    """(t, its address), allocated like `like` where t is None."""
+    if t is None:
+        t = T.empty(n, dtype=T.bf16, device=like.device)
+        return t, t.data_ptr()
+    return t, _16bit(t, what, n)
+
+
 def mx_scale_pitch(cols):
     """Bytes of a row's scales: one for 32 columns, in words of four."""
     return 4 * _nblocks(cols)
@@ -588,10 +598,12 @@ def quantize_mxfp4(w, rows, cols, ld=None):
     """(codes [rows * ceil(cols / 2)], scales [rows * mx_scale_pitch(cols)]) of a device tensor of bf16 (or its
     int16 bits) or f32, [rows, ld] row-major: e2m1 codes under the smallest power of two that leaves a block's
     largest magnitude below 7."""
-    T, dev = _torch(), w.device
-    codes = T.empty(rows * _nblocks(cols, 2), dtype=T.u8, device=dev)
-    scales = T.empty(rows * mx_scale_pitch(cols), dtype=T.u8, device=dev)
-    quantize_mxfp4_into(w, rows, cols, codes, scales, ld)
+    T, ld = _torch(), cols if ld is None else ld
+    dt = _dtype_code(w)
+    at = _at(w, "weight", _span(rows, cols, ld), 2 if dt == BF16 else 4)
+    codes = T.empty(rows * _nblocks(cols, 2), dtype=T.u8, device=w.device)
+    scales = codes.new_empty(rows * mx_scale_pitch(cols))
+    _check(lib().reng_hip_quantize_mxfp4(at, dt, rows, cols, ld, codes.data_ptr(), scales.data_ptr(), T.stream()))
     return codes, scales
 
 
@@ -609,13 +621,10 @@ def dequantize_mxfp4(codes, scales, rows, cols, out=None):
 
 def gemm_mxfp4(a, scale_a, b, scale_b, M, N, K, out=None):
     """bf16 out[M, N] of codes a [M, K / 2] and b [N, K / 2] with their scales, as quantize_mxfp4 gives them."""
-    T = _torch()
-    if out is None:
-        out = T.empty(M * N, dtype=T.bf16, device=a.device)
-    sp = mx_scale_pitch(K)
-    _check(lib().reng_hip_gemm_mxfp4(_8bit(a, "a", M * _nblocks(K, 2)), _8bit(scale_a, "scale_a", M * sp),
-                                     _8bit(b, "b", N * _nblocks(K, 2)), _8bit(scale_b, "scale_b", N * sp), M, N, K,
-                                     _16bit(out, "out", M * N), T.stream()))
+    T, sp, kb = _torch(), mx_scale_pitch(K), _nblocks(K, 2)
+    out, op = _out16(T, out, "out", M * N, a)
+    _check(lib().reng_hip_gemm_mxfp4(_8bit(a, "a", M * kb), _8bit(scale_a, "scale_a", M * sp), _8bit(b, "b", N * kb),
+                                     _8bit(scale_b, "scale_b", N * sp), M, N, K, op, T.stream()))
     return out
 
 
@@ -693,14 +702,6 @@ def _rows16(t, what, tokens, width):
     return t.data_ptr(), ld if tokens > 1 else width   # one row has no pitch
 
 
-def _out16(T, t, what, n, like):
-    """(t, its address), allocated like `like` where t is None."""
-    if t is None:
-        t = T.empty(n, dtype=T.bf16, device=like.device)
-        return t, t.data_ptr()
-    return t, _16bit(t, what, n)
-
-
 def _heads_args(T, q, k, v, tokens, n_heads, n_kv_heads, head_dim, q_gamma, k_gamma, rope, positions):
     """What both calls share: the rows' addresses and pitches, and gammas, rope and positions."""
     nk = n_kv_heads * head_dim
@@ -764,8 +765,7 @@ def attention_mxfp4(q, cache, n_heads, length, tokens, scale, mask=None, workspa
     at least attention_mxfp4_workspace_bytes(...) bytes (allocated here when None)."""
     T = _torch()
     nq = tokens * n_heads * cache.head_dim
-    if out is None:
-        out = T.empty(nq, dtype=T.bf16, device=q.device)
+    out, op = _out16(T, out, "out", nq, q)
     if workspace is None:
         wb = attention_mxfp4_workspace_bytes(n_heads, cache.n_kv_heads, cache.head_dim, length, tokens)
         workspace = T.empty(wb, dtype=T.u8, device=q.device) if wb else None
@@ -776,7 +776,7 @@ def attention_mxfp4(q, cache, n_heads, length, tokens, scale, mask=None, workspa
     _check(lib().reng_hip_attention_mxfp4(
         _16bit(q, "q", nq), cache._here(), n_heads, length, tokens,
         None if mask is None else _at(mask, "mask", tokens * _nblocks(tokens, 32), 4), scale,
-        None if workspace is None else _at(workspace, "workspace", 0, 1), wb, _16bit(out, "out", nq), T.stream()))
+        None if workspace is None else _at(workspace, "workspace", 0, 1), wb, op, T.stream()))
     return out
 
 
