@@ -63,3 +63,20 @@ def mx_form(M, N, K, cus=CUS):
 
 def mx_forms():
     return lib().forms()
+
+
+# (heads, kv, hd, length, tokens): with the attention tests' other cases every kernel, with and without a merge.
+ATTENTION_SHAPES = [
+    (8, 1, 32, 0, 65), (4, 1, 32, 910, 140), (7, 1, 32, 6262, 77), (5, 1, 64, 120, 436), (4, 1, 32, 162, 563),
+    (4, 1, 32, 8227, 275), (16, 2, 64, 0, 556), (5, 1, 64, 0, 989), (7, 1, 32, 14568, 343), (15, 3, 96, 21, 214),
+    (10, 2, 96, 1128, 279), (4, 1, 96, 4516, 148), (7, 1, 96, 2, 423), (4, 1, 96, 151, 942), (7, 1, 96, 6373, 151),
+    (14, 2, 96, 45, 814), (16, 2, 128, 0, 542), (8, 1, 96, 39, 518), (5, 1, 128, 6331, 429), (21, 3, 160, 4, 106),
+    (15, 3, 160, 646, 117), (5, 1, 160, 3007, 104), (8, 1, 160, 28, 264), (7, 1, 160, 28, 340), (5, 1, 256, 172, 690),
+    (7, 1, 224, 5576, 153),
+]
+# (M, N, K): every form of the product, with edges inside tiles and stages.
+PRODUCT_SHAPES = [
+    (9, 33, 64), (2, 4169, 32), (2, 4435, 2240), (21, 2147, 1088), (17, 2058, 32), (4131, 21, 2016), (4255, 36, 32),
+    (2185, 102, 2016), (39, 5111, 288), (41, 4469, 2432), (33, 8307, 928), (46, 9844, 2048), (33, 4584, 32), (42, 9667, 2144),
+    (67, 8538, 32), (138, 11009, 2112), (1451, 8248, 1312), (2323, 5357, 1344),
+]

@@ -10,6 +10,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
+import mx_plans as D  # noqa: E402
 import mx_reference as X  # noqa: E402
 from test_gpu_attention_tree import pack, reference, tree_mask  # noqa: E402
 
@@ -84,6 +85,15 @@ def test_chain_against_float64(R, heads, kv, hd, length, tokens):
     check(R, heads, kv, hd, length, tokens, None, seed=hd + length + 1)
 
 
+@pytest.mark.parametrize("heads,kv,hd,length,tokens", D.ATTENTION_SHAPES)
+def test_every_kernel(R, heads, kv, hd, length, tokens):
+    check(R, heads, kv, hd, length, tokens, None, seed=length + tokens)
+    vis = tree_mask(tokens, length, empty=(0, tokens // 2, tokens - 1))
+    out = check(R, heads, kv, hd, length, tokens, vis, seed=length + tokens + 1).view(tokens, -1)
+    if length == 0:
+        assert (out[[0, tokens // 2, tokens - 1]] == 0).all()
+
+
 @pytest.mark.parametrize("length", [1, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 511, 1023, 2049])
 def test_lengths(R, length):
     check(R, 8, 2, 128, length, 1, seed=length)
@@ -104,7 +114,7 @@ def test_scales(R, scale):
     check(R, 8, 2, 64, 3000, 1, scale=scale)
 
 
-@pytest.mark.parametrize("length,tokens", [(0, 40), (37, 40), (2000, 5), (5000, 70)])
+@pytest.mark.parametrize("length,tokens", [(0, 40), (37, 40), (2000, 5), (5000, 70), (100, 600), (0, 200)])
 @pytest.mark.parametrize("hd", [64, 128, 256])
 def test_rows_that_are_not_seen_take_no_part(R, hd, length, tokens):
     """Rows of NaN scales and the largest values that a token does not see change none of its bits; those that it sees make it NaN."""

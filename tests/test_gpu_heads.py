@@ -171,6 +171,37 @@ def test_cache_rows(R, tokens, heads, kv, hd, rot, axes, norm, first, spare):
         assert torch.equal(t.view(tokens, kv, hd).double(), want.view(kv, tokens, hd).transpose(0, 1))
 
 
+@pytest.mark.parametrize("heads,kv,hd,rot,axes,off", [(140, 3, 32, 32, 1, 0), (60, 7, 64, 32, 3, 0), (28, 4, 128, 128, 3, 0),
+                                                      (9, 5, 160, 160, 2, 0), (31, 2, 96, 96, 1, 1), (40, 8, 128, 128, 1, 3)])
+def test_many_tokens_are_the_same_as_few(R, heads, kv, hd, rot, axes, off):
+    """Many tokens, of which a group of lanes takes several heads: the bits of calls of a few, rows and cache, in place too."""
+    tokens = 1100
+    c = Case(tokens, heads, kv, hd, rot, axes, True, seed=hd)
+    n, nq, nk = c.qkv.shape[1], heads * hd, kv * hd
+    wide = torch.zeros(tokens, n + off, dtype=torch.bfloat16, device="cuda")
+    wide[:, off:] = c.qkv
+    q, k, v = wide[:, off:off + nq], wide[:, off + nq:off + nq + nk], wide[:, off + nq + nk:]
+    got = R.head_norm_rope_bf16(q, k, v, tokens, heads, kv, hd, **c.args(R))
+    caches = [R.MxCache(kv, hd, tokens + 9) for _ in range(2)]
+    for t in caches[0].tensors + caches[1].tensors:
+        t.fill_(0x5A)
+    q4 = R.head_norm_rope_mxfp4(q, k, v, tokens, heads, caches[0], 4, **c.args(R))
+    for a in range(0, tokens, 50):
+        b = a + 50
+        args = dict(c.args(R), positions=c.positions[:, a:b].contiguous())
+        want = R.head_norm_rope_bf16(q[a:b], k[a:b], v[a:b], 50, heads, kv, hd, **args)
+        for g, w, h in zip(got, want, (heads, kv, kv)):
+            assert torch.equal(g.view(tokens, -1)[a:b].reshape(-1), w), a
+        R.head_norm_rope_mxfp4(q[a:b], k[a:b], v[a:b], 50, heads, caches[1], 4 + a, **args)
+    assert torch.equal(q4, got[0])
+    for g, w in zip(caches[0].tensors, caches[1].tensors):
+        assert torch.equal(g, w)
+    q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    R.head_norm_rope_bf16(q, k, v, tokens, heads, kv, hd, **c.args(R), q_out=q, k_rows=k, v_rows=v)
+    for g, w in zip((q, k, v), got):
+        assert torch.equal(g.view(-1), w)
+
+
 @pytest.mark.parametrize("hd,kv", [(32, 1), (64, 3), (128, 8), (256, 2), (96, 5)])
 def test_a_plain_write_is_the_quantizer(R, hd, kv):
     """Without gammas and rotation the cache holds the quantizer's codes and scales of each head's rows."""

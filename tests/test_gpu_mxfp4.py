@@ -13,6 +13,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
+import mx_plans as D  # noqa: E402
 import mx_reference as X  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -154,12 +155,18 @@ def test_larger_products(R, M, N, K):
     check_product(R, M, N, K, K)
 
 
+@pytest.mark.parametrize("M,N,K", D.PRODUCT_SHAPES)
+def test_every_form(R, M, N, K):
+    check_product(R, M, N, K, K + 1)
+
+
 def test_product_to_an_odd_address(R):
     check_product(R, 33, 640, 256, off=1)
     check_product(R, 300, 640, 256, off=3)
 
 
-@pytest.mark.parametrize("M,N,K", [(2, 100, 4096), (70, 333, 1056), (300, 600, 288)])
+@pytest.mark.parametrize("M,N,K", [(2, 100, 4096), (70, 333, 1056), (300, 600, 288), (138, 11009, 2112),
+                                   (1451, 8248, 1312)])
 def test_a_nan_block_is_its_rows_alone(R, M, N, K):
     """A NaN scale reaches its row's outputs and no others, also in the last block of a row that ends inside a tile."""
     a, b = operand(M, K, 1), operand(N, K, 2)

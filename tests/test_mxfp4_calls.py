@@ -199,3 +199,13 @@ def test_every_form_of_the_product_is_chosen():
         assert bm == 16 or bm < 4 * M
         seen.add(form)
     assert seen == set(range(D.mx_forms()))
+
+
+def test_the_shapes_of_the_gpu_tests_reach_every_kernel():
+    from test_gpu_attention_mxfp4 import CASES
+
+    plans = [D.mx_attention_plan(*c) for c in CASES + D.ATTENTION_SHAPES]
+    assert {(p["hdp"], p["form"], p["splits"] > 1) for p in plans} == {
+        (h, f, s) for h, forms in ((64, 4), (128, 4), (256, 3)) for f in range(forms) for s in (False, True)}
+    assert {p["splits"] > 16 for p in plans} == {False, True}   # both merges
+    assert {D.mx_form(*c)[0] for c in D.PRODUCT_SHAPES} == set(range(D.mx_forms()))
