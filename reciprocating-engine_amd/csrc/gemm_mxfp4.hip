@@ -85,11 +85,9 @@ __device__ __forceinline__ uint32_t within(uint32_t pair, uint32_t q, uint32_t b
 // row of b a wave takes 8.7 us on the first, four 8.7, eight 10.0; the next piece's loads ahead are
 // equal. Of a more rows than one are faster on the rings on most products (two: 9.3 us, 9.9 and
 // 4.6 here, 10.1, 9.3 and 4.1 there; four 12.9 and 10.1).
-constexpr uint32_t ROW_NR = 2, ROW_K = 2048;
-
 template <int KS>
 __global__ __launch_bounds__(256) void gemm_mx_row(MxArgs g) {
-    constexpr uint32_t NR = ROW_NR, GROUPS = 4 / KS;   // groups of rows of a workgroup
+    constexpr uint32_t NR = MX_ROW_NR, ROW_K = MX_ROW_K, GROUPS = 4 / KS;   // groups of rows of a workgroup
     __shared__ float sums[4 * NR];
     const uint32_t lane = threadIdx.x & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % KS, grp = wave / KS;
@@ -148,10 +146,7 @@ __global__ __launch_bounds__(256) void gemm_mx_row(MxArgs g) {
 }
 
 int launch_row(const MxArgs &g, hipStream_t st) {
-    const uint32_t groups = (g.N + ROW_NR - 1) / ROW_NR, pieces = (g.K + ROW_K - 1) / ROW_K;
-    // Sixteen waves a CU, where there are as many pieces (eight: [4096, 14336] 9.8 us for 8.9).
-    const uint32_t want = (uint32_t)device_props().cus * 16;
-    const uint32_t ks = groups >= want || pieces < 2 ? 1 : groups * 2 >= want || pieces < 4 ? 2 : 4;
+    const uint32_t groups = (g.N + MX_ROW_NR - 1) / MX_ROW_NR, ks = mx_row_waves(g.N, g.K, (uint64_t)device_props().cus);
     const uint64_t wgs = ((uint64_t)groups * ks + 3) / 4;
     RENG_REQUIRE(wgs * 256 < (1ull << 32), "%u outputs are too many for a launch", g.N);
     const auto kern = ks == 1 ? gemm_mx_row<1> : ks == 2 ? gemm_mx_row<2> : gemm_mx_row<4>;

@@ -16,6 +16,7 @@ extern "C" void plan(size_t nh, size_t nkv, size_t hd, size_t len, size_t tokens
     for (int i = 0; i < 6; ++i) out[i] = v[i];
 }
 extern "C" int pick(uint64_t M, uint64_t N, uint64_t K, uint64_t cus) { return mx_pick(M, N, K, cus); }
+extern "C" uint32_t row_waves(uint64_t N, uint64_t K, uint64_t cus) { return mx_row_waves(N, K, cus); }
 extern "C" int forms() { return MX_FORMS; }
 extern "C" void outputs(int form, uint32_t *out) { out[0] = MX_COST[form].bm, out[1] = MX_COST[form].bn; }
 extern "C" void shape(uint32_t hdp, int form, uint32_t *out) {
@@ -37,6 +38,7 @@ def lib():
             _lib = ctypes.CDLL(so)
         _lib.plan.argtypes = [ctypes.c_size_t] * 6 + [ctypes.c_void_p]
         _lib.pick.argtypes = [ctypes.c_uint64] * 4
+        _lib.row_waves.argtypes = [ctypes.c_uint64] * 3
     return _lib
 
 
@@ -65,6 +67,11 @@ def mx_forms():
     return lib().forms()
 
 
+def mx_row_waves(N, K, cus=CUS):
+    """The waves that share an output's k where a has one row."""
+    return lib().row_waves(N, K, cus)
+
+
 # (heads, kv, hd, length, tokens): with the attention tests' other cases every kernel, with and without a merge.
 ATTENTION_SHAPES = [
     (8, 1, 32, 0, 65), (4, 1, 32, 910, 140), (7, 1, 32, 6262, 77), (5, 1, 64, 120, 436), (4, 1, 32, 162, 563),
@@ -79,4 +86,9 @@ PRODUCT_SHAPES = [
     (9, 33, 64), (2, 4169, 32), (2, 4435, 2240), (21, 2147, 1088), (17, 2058, 32), (4131, 21, 2016), (4255, 36, 32),
     (2185, 102, 2016), (39, 5111, 288), (41, 4469, 2432), (33, 8307, 928), (46, 9844, 2048), (33, 4584, 32), (42, 9667, 2144),
     (67, 8538, 32), (138, 11009, 2112), (1451, 8248, 1312), (2323, 5357, 1344),
+]
+# (N, K) of products of one row: one, two and four waves an output, even and odd N, whole and cut pieces of k.
+ROW_SHAPES = [
+    (1, 32), (7, 96), (129, 2048), (8193, 2080), (8194, 2080), (8192, 8192), (9001, 14336), (33, 4096), (1022, 6144), (4099, 8192),
+    (4098, 8224), (4095, 6176), (1, 8192), (62, 9248), (7, 18944), (1021, 8224), (2048, 10240), (2049, 14336),
 ]
