@@ -502,7 +502,8 @@ RENG_HIP_API size_t reng_hip_attention_mxfp4_workspace_bytes(size_t n_heads, siz
  * a token does not see take no part, whatever they hold. A row that is seen and has a
  * scale byte of 253 or more in its key or its value (a NaN block, or magnitudes of some
  * 2^128) makes all of the token's outputs NaN; so does a NaN or +inf score those of its
- * head. A token that sees nothing gives zeros, one whose scores are all -inf NaN. q and
+ * head. A token that sees nothing gives zeros, one whose scores are all -inf NaN. Scores
+ * count in base 2: one that leaves f32 when multiplied by log2 e is an infinity. q and
  * out bf16 [tokens, n_heads * head_dim], 16-byte aligned; scale finite, of any sign;
  * 1 <= tokens <= RENG_HIP_TREE_MAX_TOKENS, len + tokens at most
  * RENG_HIP_ATTENTION_MAX_LEN and the capacity; workspace 16-byte aligned. Asynchronous

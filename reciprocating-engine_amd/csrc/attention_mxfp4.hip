@@ -28,6 +28,8 @@
 // them the rows' kernel and 3.9 the merge: two launches and the start of each; 131071 rows
 // 29 to 37. A chain of 1024 after 16384 (40 on 8) 351 us, 1.0 PFLOP/s: the matrix cores and, in
 // turn with them, the exponentials.
+#include <float.h>
+
 #include <type_traits>
 
 #include "common.h"
@@ -292,8 +294,8 @@ __global__ __launch_bounds__(64 * NW) void attention_mxfp4(const MxAttn a) {
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[d] *= f;
         }
-        // With nothing above -inf so far, exponents are taken against 0: they are 0.
-        const float mc = m == -INFINITY ? 0.0f : m * c;
+        // Against the lowest value where the maximum has none or, in base 2, lies below f32: exponentials of 0 then.
+        const float mc = fmaxf(m * c, -FLT_MAX);
         float p[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -531,8 +533,8 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_mxfp4_tiles(const MxAt
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] *= f;
         }
-        // With nothing above -inf so far, exponents are taken against 0: they are 0.
-        const float mc = m == -INFINITY ? 0.0f : m * c;
+        // Against the lowest value where the maximum has none or, in base 2, lies below f32: exponentials of 0 then.
+        const float mc = fmaxf(m * c, -FLT_MAX);
         float l4[4] = {l, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)

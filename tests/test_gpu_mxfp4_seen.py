@@ -1,0 +1,42 @@
+"""Scores near the end of f32's range in the attention over a 4-bit cache."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def R():
+    import reng_hip
+
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    reng_hip.lib()
+    return reng_hip
+
+
+# (heads, kv, hd, length, tokens): every form of 64, 128 and 256 dimensions, with and without a merge.
+SHAPES = [
+    (2, 2, 64, 64, 1), (2, 2, 64, 3000, 1), (14, 2, 64, 64, 74), (14, 2, 64, 1000, 74), (14, 2, 64, 64, 293), (8, 2, 64, 200, 707),
+    (14, 2, 64, 65, 596), (14, 2, 64, 200, 677), (2, 2, 96, 64, 1), (2, 2, 96, 3000, 1), (14, 2, 96, 64, 154), (6, 3, 96, 1000, 285),
+    (14, 2, 96, 65, 295), (6, 3, 96, 1000, 530), (14, 2, 96, 64, 586), (14, 2, 96, 200, 592), (2, 2, 160, 64, 1), (2, 2, 160, 1000, 1),
+    (14, 2, 160, 64, 74), (2, 2, 160, 64, 523), (14, 2, 160, 65, 293), (14, 2, 160, 100, 322),
+]
+
+
+@pytest.mark.parametrize("heads,kv,hd,length,tokens", SHAPES)
+def test_scores_near_the_lowest_value_weigh_nothing(R, heads, kv, hd, length, tokens):
+    """Whole tiles of rows with scores of -1.75 2^127, which times log2 e lie below f32's range, and rows of score 0
+    behind them: the outputs are the mean of the latter's values, 1, exactly."""
+    cache = R.MxCache(kv, hd, length + tokens)
+    for t, byte in zip(cache.tensors, (0, 127, 0x22, 127)):   # keys 0, values 1
+        t.fill_(byte)
+    bad = 64
+    codes, scales = (t.view(kv, length + tokens, -1) for t in cache.tensors[:2])
+    codes[:, :bad, 0], scales[:, :bad, 0] = 0x0A, 127 + 27    # -1 times 2^27 on dimension 0
+    cache.tensors[2].view(kv, length + tokens, -1)[:, :bad] = 0x77   # values of 6
+    q = torch.zeros(tokens * heads, hd, dtype=torch.bfloat16, device="cuda")
+    q[:, 0] = 1.75 * 2.0**100
+    out = R.attention_mxfp4(q.view(-1), cache, heads, length, tokens, 1.0)
+    assert (out == 1.0).all(), out[out != 1.0][:4]
