@@ -361,7 +361,8 @@ RENG_HIP_API size_t reng_hip_attention_tree_workspace_bytes(size_t n_heads, size
  * nothing gives zeros, one whose scores are all -inf, or with a NaN among them,
  * gives NaN. An infinite value of a row seen gives an infinity, however small the
  * row's weight; NaN where its score is -inf (a weight of 0) or where infinities of
- * both signs meet.
+ * both signs meet. On the matrix cores scores count in base 2: one that leaves f32
+ * when multiplied by log2 e is an infinity.
  * len >= 0, 1 <= tokens <= RENG_HIP_TREE_MAX_TOKENS, len + tokens <=
  * RENG_HIP_ATTENTION_MAX_LEN; pointers 4-byte aligned, workspace 16-byte aligned with workspace_bytes >=
  * reng_hip_attention_tree_workspace_bytes(...). At most 4096 query heads. On the

@@ -15,6 +15,8 @@
 // its row's weight, and NaN where the weight is exactly 0 (a score of -inf) or
 // infinities of both signs meet: settle() decides it by this rule where a sum has
 // become NaN, so that it does not depend on how the cache is cut.
+#include <float.h>
+
 #include <type_traits>
 
 #include "common.h"
@@ -492,8 +494,8 @@ __global__ __launch_bounds__(64 * RW * KW) void attention_tree_tiles(TreeTiles t
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] *= f;
         }
-        // With nothing above -inf so far, exponents are taken against 0: they are 0.
-        const float mc = m == -INFINITY ? 0.0f : m * c;
+        // Against the lowest value where the maximum has none or, in base 2, lies below f32: exponentials of 0 then.
+        const float mc = fmaxf(m * c, -FLT_MAX);
         float l4[4] = {l, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
