@@ -505,8 +505,8 @@ RENG_HIP_API size_t reng_hip_attention_mxfp4_workspace_bytes(size_t n_heads, siz
  * 2^128) makes all of the token's outputs NaN; so does a NaN or +inf score those of its
  * head. A token that sees nothing gives zeros, one whose scores are all -inf NaN. Scores
  * count in base 2: one that leaves f32 when multiplied by log2 e is an infinity. q and
- * out bf16 [tokens, n_heads * head_dim], 16-byte aligned; scale finite, of any sign;
- * 1 <= tokens <= RENG_HIP_TREE_MAX_TOKENS, len + tokens at most
+ * out bf16 [tokens, n_heads * head_dim], 16-byte aligned; scale of any sign, of
+ * magnitude up to 2^127; 1 <= tokens <= RENG_HIP_TREE_MAX_TOKENS, len + tokens at most
  * RENG_HIP_ATTENTION_MAX_LEN and the capacity; workspace 16-byte aligned. Asynchronous
  * on stream; calls that share a workspace must be ordered (one stream). */
 RENG_HIP_API int reng_hip_attention_mxfp4(const uint16_t *q, const reng_hip_mx_cache *cache, size_t n_heads, size_t len,

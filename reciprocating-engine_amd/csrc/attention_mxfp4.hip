@@ -879,6 +879,7 @@ RENG_HIP_API int reng_hip_attention_mxfp4(const uint16_t *q, const reng_hip_mx_c
                  "%zu context rows and %zu tokens; at most %d rows", len, tokens, RENG_HIP_ATTENTION_MAX_LEN);
     RENG_REQUIRE(len + tokens <= c.capacity, "%zu context rows and %zu tokens in a cache of %zu", len, tokens, c.capacity);
     RENG_REQUIRE(scale - scale == 0.0f, "scale is not finite");
+    RENG_REQUIRE(fabsf(scale) <= 0x1p127f, "scale %g is above 2^127: times log2 e it leaves f32", (double)scale);
     RENG_REQUIRE(q && out, "null pointer");
     RENG_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) == 0 &&
                      (reinterpret_cast<uintptr_t>(mask) & 3) == 0,

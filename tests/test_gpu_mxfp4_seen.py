@@ -40,3 +40,14 @@ def test_scores_near_the_lowest_value_weigh_nothing(R, heads, kv, hd, length, to
     q[:, 0] = 1.75 * 2.0**100
     out = R.attention_mxfp4(q.view(-1), cache, heads, length, tokens, 1.0)
     assert (out == 1.0).all(), out[out != 1.0][:4]
+
+
+@pytest.mark.parametrize("scale", [2.0**127, -2.0**127])
+@pytest.mark.parametrize("heads,kv,hd,length,tokens", SHAPES[::3])
+def test_the_largest_scale(R, heads, kv, hd, length, tokens, scale):
+    """Products of 0 are scores of 0 under it: the mean of equal values."""
+    cache = R.MxCache(kv, hd, length + tokens)
+    for t, byte in zip(cache.tensors, (0x22, 127, 0x33, 127)):   # keys 1, values 1.5
+        t.fill_(byte)
+    q = torch.zeros(tokens * heads * hd, dtype=torch.bfloat16, device="cuda")
+    assert (R.attention_mxfp4(q, cache, heads, length, tokens, scale) == 1.5).all()

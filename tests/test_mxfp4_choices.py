@@ -1,4 +1,8 @@
-"""The rules of the 4-bit operators' launchers, on the host."""
+"""The rules of the 4-bit operators' launchers, on the host, and what they refuse."""
+import ctypes
+
+import pytest
+
 import mx_plans as D
 
 
@@ -21,3 +25,13 @@ def test_the_shapes_of_the_seen_rows_reach_every_attention_kernel():
     plans = [D.mx_attention_plan(*c) for c in SHAPES]
     assert {(p["hdp"], p["form"], p["splits"] > 1) for p in plans} == {
         (h, f, s) for h, forms in ((64, 4), (128, 4), (256, 3)) for f in range(forms) for s in (False, True)}
+
+
+@pytest.mark.parametrize("scale", [1.01 * 2.0**127, -3e38])
+def test_a_scale_that_base_2_cannot_hold_is_refused(scale):
+    """Times log2 e it is an infinity, which made NaN of a score of 0."""
+    import reng_hip as R
+
+    c, p = R._MxCache(64, 64, 64, 64, 2, 128, 100), ctypes.c_void_p(64)
+    assert R.lib().reng_hip_attention_mxfp4(p, ctypes.byref(c), 4, 10, 1, None, scale, p, 1 << 30, p, None) == R.EINVAL
+    assert "above 2^127" in R.lib().reng_hip_last_error().decode()
