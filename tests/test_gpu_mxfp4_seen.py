@@ -1,7 +1,10 @@
-"""Scores near the end of f32's range in the attention over a 4-bit cache."""
+"""Which outputs of the attention over a 4-bit cache a row reaches, and scores near the end of f32's range."""
 import pytest
 
 torch = pytest.importorskip("torch")
+
+import mx_reference as X  # noqa: E402
+from test_gpu_attention_mxfp4 import make, pack, tree_mask  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -23,6 +26,30 @@ SHAPES = [
     (14, 2, 96, 65, 295), (6, 3, 96, 1000, 530), (14, 2, 96, 64, 586), (14, 2, 96, 200, 592), (2, 2, 160, 64, 1), (2, 2, 160, 1000, 1),
     (14, 2, 160, 64, 74), (2, 2, 160, 64, 523), (14, 2, 160, 65, 293), (14, 2, 160, 100, 322),
 ]
+
+
+@pytest.mark.parametrize("heads,kv,hd,length,tokens", SHAPES)
+def test_a_nan_row_reaches_its_own_heads_alone(R, heads, kv, hd, length, tokens):
+    """A NaN block of one key/value head makes the query heads that share it NaN, of the tokens that see its row;
+    the other heads' bits stay."""
+    q, cache, _, _ = make(R, heads, kv, hd, length, tokens, 31)
+    vis = tree_mask(tokens, 4)
+    mask = pack(vis)
+    clean = R.attention_mxfp4(q, cache, heads, length, tokens, hd**-0.5, mask).view(tokens, kv, -1).clone()
+    assert not torch.isnan(clean).any()
+    see = torch.from_numpy(vis[:, tokens - 1]).cuda()
+    for which, byte in ((1, 255), (3, 253)):
+        for g in range(kv):
+            scales = cache.tensors[which].view(kv, -1, X.pitch(hd))
+            old = scales[g, length + tokens - 1].clone()
+            scales[g, length + tokens - 1, hd // 32 - 1] = byte
+            got = R.attention_mxfp4(q, cache, heads, length, tokens, hd**-0.5, mask).view(tokens, kv, -1)
+            want = clean.clone()
+            want[see, g] = float("nan")
+            assert torch.equal(torch.isnan(got), torch.isnan(want)), (which, g)
+            keep = ~torch.isnan(want)
+            assert torch.equal(got[keep].view(torch.int16), clean[keep].view(torch.int16)), (which, g)
+            scales[g, length + tokens - 1] = old
 
 
 @pytest.mark.parametrize("heads,kv,hd,length,tokens", SHAPES)
