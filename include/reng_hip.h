@@ -474,8 +474,10 @@ typedef struct reng_hip_rope {
  * head_dim] (may be q with that pitch), k_rows and v_rows [tokens, n_kv_heads *
  * head_dim] (may be k, v with that pitch; these rows of a bf16 cache; v and v_rows may
  * both be NULL). n_heads may be 0, with q and q_out NULL. head_dim a multiple of 32 up
- * to 256, tokens < 2^22, at most 4096 heads of each, eps finite and at least 0; fastest
- * on 16-byte aligned rows. */
+ * to 256, tokens < 2^22, at most 4096 heads of each, eps finite and at least 0; a launch
+ * takes tokens * ceil((n_heads + 2 n_kv_heads) * D / 8192) below 2^24, D the head_dim
+ * rounded up to 32, 64, 128 or 256 (4 million tokens of up to 256 heads of 128). Fastest on
+ * 16-byte aligned rows. */
 RENG_HIP_API int reng_hip_head_norm_rope_bf16(const uint16_t *q, size_t q_ld, const uint16_t *k, const uint16_t *v,
                                               size_t kv_ld, size_t tokens, size_t n_heads, size_t n_kv_heads,
                                               size_t head_dim, const float *q_gamma, const float *k_gamma, float eps,

@@ -35,3 +35,21 @@ def test_a_scale_that_base_2_cannot_hold_is_refused(scale):
     c, p = R._MxCache(64, 64, 64, 64, 2, 128, 100), ctypes.c_void_p(64)
     assert R.lib().reng_hip_attention_mxfp4(p, ctypes.byref(c), 4, 10, 1, None, scale, p, 1 << 30, p, None) == R.EINVAL
     assert "above 2^127" in R.lib().reng_hip_last_error().decode()
+
+
+def test_heads_are_refused_where_the_header_says():
+    """tokens * ceil(heads D / 8192) of 2^24 and more, for D of 32, 64, 128 and 256."""
+    import reng_hip as R
+
+    p = ctypes.c_void_p(64)   # never dereferenced: refused before any device work
+    for hd in range(32, 257, 32):
+        D = next(d for d in (32, 64, 128, 256) if d >= hd)
+        for nh, nkv in ((4096, 4096), (4000, 7), (16 * 256 // D * 32, 1), (16 * 256 // D * 32 - 2, 1)):
+            parts = -(-(nh + 2 * nkv) * D // 8192)
+            if nh > 4096 or parts * (2**22 - 1) < 2**24:
+                continue
+            least = -(-2**24 // parts)
+            for tokens in (least, 2**22 - 1):
+                rc = R.lib().reng_hip_head_norm_rope_bf16(p, nh * hd, p, p, nkv * hd, tokens, nh, nkv, hd, None, None, 1e-6,
+                                                          None, None, p, p, p, None)
+                assert rc == R.EINVAL and "too many for a launch" in R.lib().reng_hip_last_error().decode(), (hd, nh, nkv, tokens)
