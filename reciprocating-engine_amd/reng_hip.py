@@ -12,6 +12,7 @@ Argument errors that reng-fp8 turns into panics (lib.rs:527-532) raise
 `ValueError` with the library's message.
 """
 import ctypes
+import operator
 import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -677,10 +678,16 @@ class Rope:
         if sections is not None:
             if pair_axis is not None:
                 raise ValueError("sections and pair_axis both given")
+            if any(n < 0 for n in sections):
+                raise ValueError(f"sections {tuple(sections)}; expected numbers of pairs")
             pair_axis = [a for a, n in enumerate(sections) for _ in range(n)]
-        if pair_axis is not None and len(pair_axis) != rot // 2:
-            raise ValueError(f"axes for {len(pair_axis)} pairs; the tables rotate {rot // 2}")
+        if pair_axis is not None:
+            pair_axis = [operator.index(a) for a in pair_axis]   # an array's own bytes would be its elements' words
+            if len(pair_axis) != rot // 2:
+                raise ValueError(f"axes for {len(pair_axis)} pairs; the tables rotate {rot // 2}")
         self.axes = 1 if pair_axis is None else len(sections) if sections is not None else max(pair_axis) + 1
+        if self.axes > ROPE_MAX_AXES or (pair_axis is not None and min(pair_axis) < 0):
+            raise ValueError(f"pairs of axes {min(pair_axis)} to {self.axes - 1}; expected 0 to {ROPE_MAX_AXES - 1} at most")
         self.device, self.tables = sin.device, (sin, cos)
         # ctypes keeps the bytes alive with the descriptor; one axis needs no map.
         self._struct = _Rope(_f32(sin, "sin", rows * rot), _f32(cos, "cos", rows * rot), rows, rot, self.axes,

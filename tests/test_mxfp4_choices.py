@@ -53,3 +53,30 @@ def test_heads_are_refused_where_the_header_says():
                 rc = R.lib().reng_hip_head_norm_rope_bf16(p, nh * hd, p, p, nkv * hd, tokens, nh, nkv, hd, None, None, 1e-6,
                                                           None, None, p, p, p, None)
                 assert rc == R.EINVAL and "too many for a launch" in R.lib().reng_hip_last_error().decode(), (hd, nh, nkv, tokens)
+
+
+def test_axes_of_pairs_come_in_any_sequence():
+    """A list, an array of any whole type or a tensor name the same axes; what is no axis is refused."""
+    import numpy as np
+    import torch
+
+    import reng_hip as R
+
+    class Dev(torch.Tensor):
+        is_cuda = property(lambda self: True)
+
+    tables = [torch.zeros(4, 32).as_subclass(Dev) for _ in range(2)]
+    axes = [0, 1, 2, 3] * 4
+    for pairs in (axes, tuple(axes), np.array(axes), np.array(axes, dtype=np.int32), np.array(axes, dtype=np.uint8), torch.tensor(axes)):
+        rope = R.Rope(*tables, pair_axis=pairs)
+        assert rope.axes == 4 and rope._struct.axes == 4
+        at = ctypes.c_void_p.from_buffer(rope._struct, R._Rope.pair_axis.offset).value
+        assert list(ctypes.string_at(at, 16)) == axes
+    assert R.Rope(*tables, pair_axis=[0] * 16).axes == 1
+    assert R.Rope(*tables, sections=np.array([4, 5, 7])).axes == 3
+    for pairs in ([0] * 15 + [-1], [0] * 15 + [4], [0, 300] * 8, [0.5] * 16):
+        with pytest.raises((ValueError, TypeError)):
+            R.Rope(*tables, pair_axis=pairs)
+    for sections in ((16, -3), (20, -4), (4, 4, 4, 2, 2), ()):
+        with pytest.raises(ValueError):
+            R.Rope(*tables, sections=sections)
