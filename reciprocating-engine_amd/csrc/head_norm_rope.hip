@@ -12,8 +12,10 @@
 // groups take consecutive heads, so a token's row is read as it lies. Of a rotation's tables a
 // lane reads its dimensions' entries once a token, whatever the heads it goes through.
 //
-// Bound: HBM for many tokens (1024 of 56 heads of 128, 31 MB: 12.7 us, 2.5 TB/s), the launch
-// and a chain of loads, position then table, for few (one token 3.8 us).
+// What bounds it: the launch and a chain of loads, position then table, for few tokens (one 3.8 us); for
+// many too while they are one round of workgroups (1024 of 56 heads of 128, 31 MB: 12.7 us, 2.5 TB/s),
+// HBM beyond (4096: 31.8 us, 3.8 TB/s; a copy reaches 5.1).
+#include "head_forms.h"
 #include "mx.h"
 
 namespace reng {
@@ -34,6 +36,7 @@ struct HeadsArgs {
     reng_hip_mx_cache cache;
     size_t first;
     uint64_t axes8;       // of each 8 pairs their axis, four bits; MIXED: pair_axis says it pair by pair
+    bool mixed;           // whether some are
     uint8_t pair_axis[128];
 };
 constexpr uint32_t MIXED = 15;
@@ -76,7 +79,7 @@ __device__ __forceinline__ void load8f(const float *p, float (&x)[8]) {
 __device__ __forceinline__ void tables(const HeadsArgs &a, uint32_t token, uint32_t d, uint32_t pair, float (&sn)[8],
                                        float (&cs)[8]) {
     auto row_of = [&](uint32_t axis) { return (uint32_t)a.positions[(size_t)axis * a.tokens + token]; };
-    // A row outside the tables is read as row 0 and then made NaN: no branch holds the loads up.
+    // A row outside the tables is read as row 0 and then made NaN, without a branch on the position.
     const uint32_t axis = (uint32_t)(a.axes8 >> (pair / 2)) & 15;
     if (axis != MIXED) {
         const uint32_t row = row_of(axis);
@@ -229,13 +232,9 @@ template <int L, bool VEC, bool MX>
 int launch_lanes(const HeadsArgs &a, hipStream_t st) {
     const uint32_t heads = a.nh + 2 * a.nkv;
     constexpr uint32_t G = 256 / L;
-    const uint32_t parts1 = (heads + G - 1) / G, parts4 = (heads + 4 * G - 1) / (4 * G);
-    // Four heads a group of lanes, where that fills more than half of the workgroups' lanes and leaves four
-    // workgroups a CU: 1024 tokens of 56 heads of 128 12.7 us for 13.7; but 300 tokens of 48 6.4 for
-    // 5.2, and 4000 of 15 heads of 64 20.6 for 11.8.
-    const bool four = heads > 2 * G && (uint64_t)a.tokens * parts4 >= (uint64_t)device_props().cus * 4;
-    const uint32_t parts = four ? parts4 : parts1;
-    RENG_REQUIRE((uint64_t)a.tokens * parts < (1u << 24), "%u tokens of %u heads are too many for a launch", a.tokens, heads);
+    const bool four = heads_by_four(a.tokens, heads, G, a.sin_table, a.mixed, (uint64_t)device_props().cus);
+    const uint32_t parts = head_parts(heads, G, four);
+    RENG_REQUIRE((uint64_t)a.tokens * parts < HEAD_LAUNCH, "%u tokens of %u heads are too many for a launch", a.tokens, heads);
     const auto kern = four ? head_norm_rope<L, 4, VEC, MX> : head_norm_rope<L, 1, VEC, MX>;
     hipLaunchKernelGGL(kern, dim3(a.tokens * parts), dim3(256), 0, st, a, parts);
     return check_launch("head_norm_rope");
@@ -292,6 +291,7 @@ int heads_args(HeadsArgs &a, const uint16_t *q, size_t q_ld, const uint16_t *k, 
             a.pair_axis[i] = r.pair_axis[i];
             const uint64_t eight = r.pair_axis[i / 8 * 8] == r.pair_axis[i] ? r.pair_axis[i] : MIXED;
             a.axes8 |= eight << (i / 8 * 4);
+            a.mixed |= eight == MIXED;
         }
     return RENG_HIP_OK;
 }

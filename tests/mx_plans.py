@@ -7,6 +7,7 @@ import tempfile
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "reciprocating-engine_amd", "csrc")
 CUS = 256   # an MI355X
 SOURCE = """
+#include "head_forms.h"
 #include "mx_attention_plan.h"
 #include "mx_forms.h"
 using namespace reng;
@@ -17,6 +18,9 @@ extern "C" void plan(size_t nh, size_t nkv, size_t hd, size_t len, size_t tokens
 }
 extern "C" int pick(uint64_t M, uint64_t N, uint64_t K, uint64_t cus) { return mx_pick(M, N, K, cus); }
 extern "C" uint32_t row_waves(uint64_t N, uint64_t K, uint64_t cus) { return mx_row_waves(N, K, cus); }
+extern "C" int by_four(uint64_t tokens, uint32_t heads, uint32_t group, int rotates, int mixed, uint64_t cus) {
+    return heads_by_four(tokens, heads, group, rotates, mixed, cus);
+}
 extern "C" int forms() { return MX_FORMS; }
 extern "C" void outputs(int form, uint32_t *out) { out[0] = MX_COST[form].bm, out[1] = MX_COST[form].bn; }
 extern "C" void shape(uint32_t hdp, int form, uint32_t *out) {
@@ -38,6 +42,7 @@ def lib():
             _lib = ctypes.CDLL(so)
         _lib.plan.argtypes = [ctypes.c_size_t] * 6 + [ctypes.c_void_p]
         _lib.pick.argtypes = [ctypes.c_uint64] * 4
+        _lib.by_four.argtypes = [ctypes.c_uint64, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_int, ctypes.c_int, ctypes.c_uint64]
         _lib.row_waves.argtypes = [ctypes.c_uint64] * 3
     return _lib
 
@@ -70,6 +75,16 @@ def mx_forms():
 def mx_row_waves(N, K, cus=CUS):
     """The waves that share an output's k where a has one row."""
     return lib().row_waves(N, K, cus)
+
+
+def head_lanes(hd):
+    """Lanes of a head, eight values each."""
+    return next(n // 8 for n in (32, 64, 128, 256) if hd <= n)
+
+
+def heads_by_four(tokens, heads, hd, rotates=True, mixed=False, cus=CUS):
+    """Whether a group of lanes takes four of a token's heads (queries, keys and values)."""
+    return bool(lib().by_four(tokens, heads, 256 // head_lanes(hd), rotates, mixed, cus))
 
 
 # (heads, kv, hd, length, tokens): with the attention tests' other cases every kernel, with and without a merge.

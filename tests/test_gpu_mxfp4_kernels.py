@@ -29,11 +29,16 @@ def test_one_row(R, N, K):
     check_product(R, 1, N, K, N)
 
 
-@pytest.mark.parametrize("tokens", [13, 1100])
-@pytest.mark.parametrize("heads,kv,hd,rot,axes,off", [
+# Heads, their size, rotation and axes, and where rows start; of 1100 tokens some take four heads a group of lanes.
+ROWS = [
     (4, 2, 32, 32, 1, 1), (140, 3, 32, 16, 2, 3), (5, 1, 64, 64, 3, 1), (60, 7, 64, 32, 1, 5), (3, 1, 96, 96, 1, 2),
     (31, 3, 128, 128, 3, 7), (4, 2, 160, 80, 4, 1), (9, 5, 160, 160, 2, 3), (6, 1, 256, 256, 1, 4), (19, 2, 256, 64, 3, 1),
-    (2, 2, 224, None, 1, 1)])
+    (2, 2, 224, None, 1, 1),
+]
+
+
+@pytest.mark.parametrize("tokens", [13, 1100])
+@pytest.mark.parametrize("heads,kv,hd,rot,axes,off", ROWS)
 def test_unaligned_rows(R, heads, kv, hd, rot, axes, off, tokens):
     """Rows that start anywhere, of an odd pitch: against 64 bits, and the bits of aligned rows, as rows and in the cache."""
     c = Case(tokens, heads, kv, hd, rot, axes, True, seed=hd + off)

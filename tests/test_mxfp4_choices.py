@@ -80,3 +80,17 @@ def test_axes_of_pairs_come_in_any_sequence():
     for sections in ((16, -3), (20, -4), (4, 4, 4, 2, 2), ()):
         with pytest.raises(ValueError):
             R.Rope(*tables, sections=sections)
+
+
+def test_the_heads_rule():
+    """Few tokens take one head a group of lanes, many four where that wastes few groups, and where one would not fit a launch;
+    the GPU tests' shapes reach both for every number of lanes."""
+    four = D.heads_by_four
+    assert [four(t, 56, 128) for t in (1, 300, 639, 640, 1024, 4096)] == [False, False, False, True, True, True]
+    assert [four(t, 56, 128, mixed=True) for t in (1, 383, 384, 640)] == [False, False, True, True]
+    assert not four(4000, 80, 128) and four(4000, 80, 128, mixed=True) and not four(4000, 16, 128) and not four(4000, 36, 128, rotates=False)
+    assert four(2**22 - 1, 80, 128) and not four(2**20, 80, 128)
+    from test_gpu_mxfp4_kernels import ROWS
+
+    seen = {(D.head_lanes(hd), four(t, h + 2 * kv, hd, bool(rot), axes > 1)) for h, kv, hd, rot, axes, _ in ROWS for t in (13, 1100)}
+    assert seen == {(n, f) for n in (4, 8, 16, 32) for f in (False, True)}
