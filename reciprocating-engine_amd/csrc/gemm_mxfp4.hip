@@ -455,7 +455,8 @@ __global__ __launch_bounds__(64 * T::NW) void gemm_mx_tiles(MxArgs g, uint32_t t
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            // In the accumulation registers: left to itself the compiler moves the sums about and spills.
+            // In the accumulation registers: left to itself the compiler moves the sums about and spills in
+            // the loop (so it spills 15 registers ahead of it).
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll

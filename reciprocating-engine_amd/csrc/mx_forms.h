@@ -24,7 +24,10 @@ enum MxForm {
 // Outputs of a workgroup, stages of 256 k that it takes a step, and times (us): the start and a step of a
 // CU's first workgroup, and what each further one of that CU adds to them. Fitted to graph-replayed
 // timings of every form on 156 products (M 2 to 6000, N 1024 to 27648, K 576 to 27648); on these the
-// choice is the fastest form or within 6% of it (0.3% in the mean).
+// choice is the fastest form or within 6% of it (0.3% in the mean). The weight's bytes are no term of
+// their own, so for wider ones its times are too short, and the order less sure: on 75 products of N 49152
+// to 152064 (M 2 to 1024) the choice is 3.6% from the fastest in the mean, 19% at most but for 17 and 24 rows
+// [65536, 8192], 28% and 25%.
 struct MxCost {
     uint32_t bm, bn, step;
     float start, start_more, one, more;
