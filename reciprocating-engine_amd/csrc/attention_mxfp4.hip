@@ -24,10 +24,10 @@
 // counts as NaN: its key's scale becomes NaN and its value's 1, so that its score decides
 // who meets it, and a weight of 0 takes nothing from a value.
 //
-// What bounds it: one token after 32768 rows (32 heads on 8, 36 MB of cache) 15.0 us, 12.3 of
-// them the rows' kernel and 3.9 the merge: two launches and the start of each; 131071 rows
-// 29 to 37. A chain of 1024 after 16384 (40 on 8) 351 us, 1.0 PFLOP/s: the matrix cores and, in
-// turn with them, the exponentials.
+// What bounds it: one token after 32768 rows (32 heads on 8, 36 MB of cache) 14.7 us, 11.6 of
+// them the rows' kernel and 3.7 the merge: two launches and the start of each; after 131071 31.5.
+// A chain of 1024 after 16384 (40 on 8) 349 us, 1.0 PFLOP/s: the matrix cores and, in turn with them,
+// the exponentials; after none 45.8, masked steps without turns.
 #include <float.h>
 
 #include <type_traits>

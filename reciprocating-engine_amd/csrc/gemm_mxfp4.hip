@@ -164,9 +164,10 @@ int launch_row(const MxArgs &g, hipStream_t st) {
 // result's lane has activation row l % 16 and the four weight rows from 4 (l / 16).
 //
 // What bounds it: the fetch of the weight and, beside it, of the rows of a, which every workgroup
-// brings through L2 once more: [3584, 18944] with 16, 24 and 32 rows 13.5, 15.2 and 16.4 us, one row
-// by itself 10.1. Not the depth of the rings: four to eight waves of two to four stages take
-// 15.2 to 15.9 at 24 rows. Operands fetched straight into registers (64 bytes of a row an
+// brings through L2 once more: [3584, 18944] with 16, 24 and 32 rows 13.4, 15.0 and 16.2 us, one row
+// by itself 10.1. What the two cost each other is not settled: with the weight in the Infinity Cache, and as
+// much of a to bring, 24 rows take 9.3. Not the depth of the rings: four to eight waves of two to four
+// stages take 15.2 to 15.9 at 24 rows. Operands fetched straight into registers (64 bytes of a row an
 // instruction) took 18 to 23.
 template <int MT, int NT, int S>
 struct RingShape {

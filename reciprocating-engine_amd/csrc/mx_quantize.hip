@@ -3,8 +3,9 @@
 //
 // Bound: HBM. The quantizer reads a value once (2 or 4 bytes) and writes 17/32 of a
 // byte; a lane holds 8 values, four lanes a block, sixteen the 128 columns whose four
-// scales are a word. bf16 [14336, 4096]: 28.2 us (5.3 TB/s), the values back 22.8 us (6.5);
-// a copy of 1 GiB reaches 5.1. 24 rows of 18944: 3.0 and 2.7 us, the launch.
+// scales are a word. bf16 [14336, 4096]: 26.6 us (5.6 TB/s), the values back 22.6 us (6.5), f32
+// 52.8 us (5.0); a copy of 1 GiB reaches 5.1. 24 rows of 18944: 2.9 and 2.6 us, the launch. Odd widths and
+// rows that are not aligned go by single values: bf16 [14336, 4095] 70.6 us, back 76.4, f32 106.
 #include "mx.h"
 
 namespace reng {
