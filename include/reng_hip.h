@@ -500,18 +500,18 @@ RENG_HIP_API size_t reng_hip_attention_mxfp4_workspace_bytes(size_t n_heads, siz
 
 /* reng_hip_attention_tree over a cache held in 4 bits, for one token or many: rows 0 ..
  * len - 1 are context, rows len .. len + tokens - 1 the tokens' own, mask as there (NULL:
- * a chain). Scores, their maxima and sums are f32; each weight is rounded to bf16 where
- * it meets its value, and values up to 2^102 in magnitude overflow none, as there. Rows
- * a token does not see take no part, whatever they hold. A row that is seen and has a
- * scale byte of 253 or more in its key or its value (a NaN block, or magnitudes of some
- * 2^128) makes the token's outputs NaN on the query heads of that key/value head; so does
- * a NaN or +inf score those of its query head. A token that sees nothing gives zeros, a
- * head whose scores are all -inf NaN. Scores count in base 2: one that leaves f32 when
- * multiplied by log2 e is an infinity. q and out bf16 [tokens, n_heads * head_dim],
- * 16-byte aligned; scale of any sign, of magnitude up to 2^127; 1 <= tokens <=
- * RENG_HIP_TREE_MAX_TOKENS, len + tokens at most RENG_HIP_ATTENTION_MAX_LEN and the
- * capacity; workspace 16-byte aligned. Asynchronous on stream; calls that share a
- * workspace must be ordered (one stream). */
+ * a chain). Scores, their maxima and sums are f32; each weight is rounded to bf16 where it
+ * meets its value, and values up to 2^102 in magnitude overflow none, as there; a weight
+ * below 2^-118 of the largest may count as 0. Rows a token does not see take no part,
+ * whatever they hold. A row that is seen and has a scale byte of 253 or more in its key or
+ * its value (a NaN block, or magnitudes of some 2^128) makes the token's outputs NaN on
+ * the query heads of that key/value head; so does a NaN or +inf score those of its query
+ * head. A token that sees nothing gives zeros, a head whose scores are all -inf NaN.
+ * Scores count in base 2: one that leaves f32 when multiplied by log2 e is an infinity. q
+ * and out bf16 [tokens, n_heads * head_dim], 16-byte aligned; scale of any sign, of
+ * magnitude up to 2^127; 1 <= tokens <= RENG_HIP_TREE_MAX_TOKENS, len + tokens at most
+ * RENG_HIP_ATTENTION_MAX_LEN and the capacity; workspace 16-byte aligned. Asynchronous on
+ * stream; calls that share a workspace must be ordered (one stream). */
 RENG_HIP_API int reng_hip_attention_mxfp4(const uint16_t *q, const reng_hip_mx_cache *cache, size_t n_heads, size_t len,
                                           size_t tokens, const uint32_t *mask, float scale, void *workspace,
                                           size_t workspace_bytes, uint16_t *out, void *stream);

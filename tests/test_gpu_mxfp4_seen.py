@@ -4,7 +4,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import mx_reference as X  # noqa: E402
-from test_gpu_attention_mxfp4 import make, pack, tree_mask  # noqa: E402
+from test_gpu_attention_mxfp4 import make, pack, reference, tree_mask  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +78,18 @@ def test_the_largest_scale(R, heads, kv, hd, length, tokens, scale):
         t.fill_(byte)
     q = torch.zeros(tokens * heads * hd, dtype=torch.bfloat16, device="cuda")
     assert (R.attention_mxfp4(q, cache, heads, length, tokens, scale) == 1.5).all()
+
+
+@pytest.mark.parametrize("scale", [1.0, -3.0])
+@pytest.mark.parametrize("heads,kv,hd,length,tokens", SHAPES)
+def test_weights_that_vanish(R, heads, kv, hd, length, tokens, scale):
+    """Scores hundreds apart, within the tolerance of test_gpu_attention_tree.py and what may vanish: the sums of waves and
+    splits are each held against a maximum of their own, which their largest weight passes by up to 2^8, and meet
+    under a factor that f32 ends at 2^-126. So a weight below 2^-118 of the token's largest may be lost, sum |v| of them at most."""
+    for seed in range(3):
+        q, cache, k, v = make(R, heads, kv, hd, length, tokens, seed)
+        vis = tree_mask(tokens, seed)
+        want, bound = reference(q, k, v, heads, kv, hd, length, tokens, vis, scale)
+        got = R.attention_mxfp4(q, cache, heads, length, tokens, scale, pack(vis)).view(tokens, heads, hd).double()
+        lost = 2.0**-118 * v.abs().view(-1, kv, hd).sum(0).repeat_interleave(heads // kv, 0)
+        assert ((got - want).abs() <= bound + 2.0**-8 * want.abs() + lost).all()
